@@ -395,6 +395,69 @@ int kvr_exchange_open(const unsigned char* handle, void** ptr);
 int kvr_exchange_close(void* ptr);
 int kvr_exchange_free(void* ptr);
 
+/* ------------------------------------------------------- paged KV cache
+ * The target model's side of a speculation round (no reference counterpart:
+ * the reference leaves the target's cache to transformers).  Keys and
+ * values live in pages of page_size tokens,
+ *   key_pages, value_pages  [num_pages, kv_heads, page_size, D]  bf16 or fp16
+ * addressed through the given strides (elements, multiples of 8; D
+ * contiguous), so any order of the first three axes and pools that hold
+ * both kinds are accepted.  block_table[b*table_stride + j/page_size] is
+ * the page of token j of sequence b; lengths[b] is its length.  Both are
+ * read on the device.
+ *
+ * kvr_paged_append: the T = new_tokens newest tokens of every sequence,
+ * positions lengths[b]-T .. lengths[b]-1 (lengths already count them), from
+ * key/value [B, HKV, T, D] (strides in elements, multiples of 8).  Positions
+ * below 0 and rows whose page number is not in [0, num_pages) are skipped. */
+typedef struct {
+  const void* key; int64_t key_b_stride, key_h_stride, key_t_stride;
+  const void* value; int64_t value_b_stride, value_h_stride, value_t_stride;
+  void* key_pages; int64_t key_page_stride, key_head_stride, key_row_stride;
+  void* value_pages; int64_t value_page_stride, value_head_stride, value_row_stride;
+  const int* block_table; int64_t table_stride; int table_width; int num_pages;
+  const int* lengths;
+  int batch, kv_heads, head_dim, new_tokens, page_size;
+} kvr_paged_append_args;
+int kvr_paged_append(const kvr_paged_append_args* a, kvr_stream_t stream);
+
+/* Attention of the T newest tokens of every sequence over its pages, in one
+ * pass split over the cache's length and joined in the same launch.  Query t
+ * stands at i = lengths[b]-T+t and sees the tokens j <= i; with window > 0
+ * only those with j > i-window or j < sinks.  A query that sees nothing
+ * gives zeros (lse -inf).  A sequence longer than its table row, or with a
+ * page number outside the pool among the tokens it sees, gives NaN.
+ *   query [B, HQ, T, D] (strides in elements, multiples of 8), out
+ *   [B, HQ, T, D] contiguous in the query's type, lse [B, HQ, T] natural
+ *   log or NULL.
+ *   token_weights [B, >= table_width*page_size] fp32 or NULL: the weight
+ *   every cached token got, summed over heads and queries, is added to it
+ *   (a second launch; needs `scores`).
+ * Supported: D in {64, 128}, table_width*page_size <= 2^30.
+ * kvr_paged_attention_plan gives the bytes of workspace, the ints of
+ * counters (zero before the first launch, left zero by every completed one)
+ * and the bytes of scores (0 without token_weights).                       */
+typedef struct {
+  const void* query; int64_t q_b_stride, q_h_stride, q_t_stride;
+  const void* key_pages; int64_t key_page_stride, key_head_stride, key_row_stride;
+  const void* value_pages; int64_t value_page_stride, value_head_stride, value_row_stride;
+  const int* block_table; int64_t table_stride; int table_width; int num_pages;
+  const int* lengths;
+  void* out; float* lse;
+  float* token_weights; int64_t weights_b_stride;
+  int dtype;            /* 0 bf16, 1 fp16: query, pages and out */
+  int batch, q_heads, kv_heads, head_dim, new_tokens, page_size;
+  int window, sinks;    /* window 0: no window (sinks unused) */
+  float scale;          /* multiplies q.k */
+  int num_sms;          /* 0: query the current device */
+  void* workspace; size_t workspace_bytes;
+  int* counters;
+  void* scores; size_t scores_bytes;
+} kvr_paged_attention_args;
+int kvr_paged_attention_plan(const kvr_paged_attention_args* a, size_t* workspace_bytes,
+                             size_t* counter_count, size_t* scores_bytes);
+int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

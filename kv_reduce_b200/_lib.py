@@ -63,6 +63,9 @@ EXPORTED_SYMBOLS = (
     "kvr_exchange_open",
     "kvr_exchange_close",
     "kvr_exchange_free",
+    "kvr_paged_append",
+    "kvr_paged_attention_plan",
+    "kvr_paged_attention",
 )
 
 
@@ -169,6 +172,37 @@ class DecodeArgs(Structure):
     ]
 
 
+class PagedAppendArgs(Structure):
+    _fields_ = [
+        ("key", c_void_p), ("key_b_stride", c_int64), ("key_h_stride", c_int64), ("key_t_stride", c_int64),
+        ("value", c_void_p), ("value_b_stride", c_int64), ("value_h_stride", c_int64), ("value_t_stride", c_int64),
+        ("key_pages", c_void_p), ("key_page_stride", c_int64), ("key_head_stride", c_int64),
+        ("key_row_stride", c_int64),
+        ("value_pages", c_void_p), ("value_page_stride", c_int64), ("value_head_stride", c_int64),
+        ("value_row_stride", c_int64),
+        ("block_table", c_void_p), ("table_stride", c_int64), ("table_width", c_int), ("num_pages", c_int),
+        ("lengths", c_void_p),
+        ("batch", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("new_tokens", c_int), ("page_size", c_int),
+    ]
+
+
+class PagedAttentionArgs(Structure):
+    _fields_ = [
+        ("query", c_void_p), ("q_b_stride", c_int64), ("q_h_stride", c_int64), ("q_t_stride", c_int64),
+        ("key_pages", c_void_p), ("key_page_stride", c_int64), ("key_head_stride", c_int64),
+        ("key_row_stride", c_int64),
+        ("value_pages", c_void_p), ("value_page_stride", c_int64), ("value_head_stride", c_int64),
+        ("value_row_stride", c_int64),
+        ("block_table", c_void_p), ("table_stride", c_int64), ("table_width", c_int), ("num_pages", c_int),
+        ("lengths", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+        ("token_weights", c_void_p), ("weights_b_stride", c_int64), ("dtype", c_int),
+        ("batch", c_int), ("q_heads", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("new_tokens", c_int),
+        ("page_size", c_int), ("window", c_int), ("sinks", c_int), ("scale", ctypes.c_float), ("num_sms", c_int),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("counters", c_void_p),
+        ("scores", c_void_p), ("scores_bytes", c_size_t),
+    ]
+
+
 _lib = None
 
 
@@ -219,6 +253,10 @@ def load() -> ctypes.CDLL:
     lib.kvr_exchange_open.argtypes = [ctypes.c_char_p, POINTER(c_void_p)]
     lib.kvr_exchange_close.argtypes = [c_void_p]
     lib.kvr_exchange_free.argtypes = [c_void_p]
+    lib.kvr_paged_append.argtypes = [POINTER(PagedAppendArgs), c_void_p]
+    lib.kvr_paged_attention_plan.argtypes = [POINTER(PagedAttentionArgs), POINTER(c_size_t), POINTER(c_size_t),
+                                             POINTER(c_size_t)]
+    lib.kvr_paged_attention.argtypes = [POINTER(PagedAttentionArgs), c_void_p]
     for name in EXPORTED_SYMBOLS:
         if name not in ("kvr_version", "kvr_status_string", "kvr_last_error"):
             getattr(lib, name).restype = c_int

@@ -18,8 +18,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libkvr.so"
 TORCH_LIB = PKG / "libkvr_torch.so"
-SOURCES = ["kvr_capi.cu", "kvr_pack.cu", "kvr_decode.cu", "kvr_decode_simt.cu", "kvr_exchange.cu"]
-TORCH_SOURCE = "kvr_torch.cpp"
+SOURCES = ["kvr_capi.cu", "kvr_pack.cu", "kvr_decode.cu", "kvr_decode_simt.cu", "kvr_exchange.cu", "kvr_paged.cu"]
+TORCH_SOURCES = ["kvr_torch.cpp", "kvr_torch_paged.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -49,12 +49,12 @@ def _torch_stale() -> bool:
     if not TORCH_LIB.exists():
         return True
     mtime = TORCH_LIB.stat().st_mtime
-    deps = [CSRC / TORCH_SOURCE, ROOT / "include" / "kvr.h", LIB]
+    deps = [*(CSRC / s for s in TORCH_SOURCES), ROOT / "include" / "kvr.h", LIB]
     return any(p.stat().st_mtime > mtime for p in deps if p.exists())
 
 
 def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
-    """libkvr_torch.so: the torch.ops.kvr operators (kvr_torch.cpp, host C++
+    """libkvr_torch.so: the torch.ops.kvr operators (kvr_torch*.cpp, host C++
     over libkvr.so's C ABI), compiled against this interpreter's torch."""
     if not force and not _torch_stale():
         return TORCH_LIB
@@ -68,7 +68,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
            "-DTORCH_EXTENSION_NAME=kvr_torch"]
     for inc in cpp_extension.include_paths():
         cmd += ["-isystem", inc]
-    cmd += ["-isystem", str(cuda_home / "include"), "-I", str(ROOT / "include"), str(CSRC / TORCH_SOURCE)]
+    cmd += ["-isystem", str(cuda_home / "include"), "-I", str(ROOT / "include"), *(str(CSRC / s) for s in TORCH_SOURCES)]
     for libdir in cpp_extension.library_paths():
         cmd += ["-L", libdir, f"-Wl,-rpath,{libdir}"]
     cmd += ["-L", str(PKG), "-lkvr", "-Wl,-rpath,$ORIGIN", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",

@@ -1,0 +1,227 @@
+// torch.ops.kvr.* operators of the target model's side of a speculation
+// round, over libkvr.so's C ABI:
+//
+//   kvr::paged_append     new tokens' keys and values into their pages
+//   kvr::paged_attention  attention of the new tokens over the pages
+//
+// Checks raise ValueError before anything is allocated or launched.  Outputs
+// come from the caching allocator.  The join's scratch is cached per
+// (device, stream): launches on one stream follow each other, and a completed
+// launch leaves the counters at zero.  Inside a CUDA graph capture a call
+// takes its scratch from the graph's own memory (a memset node zeroes the
+// counters on each replay), so a graph never depends on a cached buffer.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/library.h>
+
+#include <cmath>
+#include <cstring>
+#include <map>
+#include <mutex>
+#include <string>
+#include <utility>
+#include <vector>
+
+#include "../../include/kvr.h"
+
+namespace {
+
+void raise_status(const char* fn, int st) {
+  if (st == KVR_OK) return;
+  const std::string text = kvr_status_string(st);
+  if (st == KVR_ERR_INVALID_ARGUMENT || st == KVR_ERR_UNSUPPORTED || st == KVR_ERR_MISALIGNED)
+    TORCH_CHECK_VALUE(false, fn, " failed: ", text, " (status ", st, ")");
+  TORCH_CHECK(false, fn, " failed: ", text, " (status ", st, ")", st == KVR_ERR_CUDA ? ": " : "",
+              st == KVR_ERR_CUDA ? kvr_last_error() : "");
+}
+
+// A stride the kernels multiply an index with; an axis of one element is
+// never stepped along, and torch lets it have any stride.
+int64_t step(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+bool rows16(const at::Tensor& t) {
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (step(t, d) % 8) return false;
+  return (t.size(t.dim() - 1) <= 1 || t.stride(t.dim() - 1) == 1) &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+// Keys, values and queries may have any strides as long as the head's
+// elements are contiguous and rows start on 16 bytes; others are copied.
+at::Tensor rows(const at::Tensor& t) { return rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+struct Scratch {
+  at::Tensor workspace, counters;
+};
+std::mutex g_mu;
+std::map<std::pair<int, uintptr_t>, Scratch> g_scratch;
+// Buffers outgrown by a later call; launches in flight may still hold them,
+// and the growth is geometric, so they are kept.
+std::vector<at::Tensor> g_outgrown;
+
+Scratch scratch_for(const at::Device& dev, cudaStream_t stream, int64_t bytes, int64_t counters) {
+  const auto u8 = at::TensorOptions().dtype(at::kByte).device(dev);
+  const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    return {at::empty({std::max<int64_t>(bytes, 16)}, u8), at::zeros({std::max<int64_t>(counters, 1)}, i32)};
+  std::lock_guard<std::mutex> lock(g_mu);
+  Scratch& s = g_scratch[{dev.index(), reinterpret_cast<uintptr_t>(stream)}];
+  if (!s.workspace.defined() || s.workspace.numel() < bytes) {
+    if (s.workspace.defined()) g_outgrown.push_back(s.workspace);
+    s.workspace = at::empty({std::max<int64_t>(2 * bytes, 1 << 20)}, u8);
+  }
+  if (!s.counters.defined() || s.counters.numel() < counters) {
+    if (s.counters.defined()) g_outgrown.push_back(s.counters);
+    s.counters = at::zeros({std::max<int64_t>(2 * counters, 4096)}, i32);
+  }
+  return s;
+}
+
+bool is_half_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+
+void check_pages(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& table, const at::Tensor& lengths,
+                 const at::Device& dev) {
+  TORCH_CHECK_VALUE(dev.is_cuda(), "kv_reduce_b200 operates on CUDA tensors only (no CPU fallback).");
+  for (const at::Tensor* t : {&kp, &vp, &table, &lengths})
+    TORCH_CHECK_VALUE(t->device() == dev, "All tensors must be on the same CUDA device.");
+  TORCH_CHECK_VALUE(kp.dim() == 4 && kp.sizes() == vp.sizes(),
+                    "key_pages and value_pages must be [num_pages, kv_heads, page_size, head_dim] of one shape.");
+  TORCH_CHECK_VALUE(is_half_type(kp.scalar_type()) && vp.scalar_type() == kp.scalar_type(),
+                    "key_pages and value_pages must be bf16 or fp16, both the same.");
+  TORCH_CHECK_VALUE(kp.size(1) > 0 && kp.size(2) > 0, "key_pages must have at least one head and one row per page.");
+  TORCH_CHECK_VALUE(rows16(kp) && rows16(vp),
+                    "pages must have contiguous head elements and rows that start on 16 bytes.");
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.scalar_type() == at::kInt && (table.size(1) <= 1 || table.stride(1) == 1),
+                    "block_table must be int32 [batch, pages] with contiguous rows.");
+  TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.scalar_type() == at::kInt && lengths.size(0) == table.size(0) &&
+                        (lengths.size(0) <= 1 || lengths.stride(0) == 1),
+                    "lengths must be a contiguous int32 [batch] tensor.");
+}
+
+void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tensor& kp, const at::Tensor& vp,
+                  const at::Tensor& table, const at::Tensor& lengths) {
+  check_pages(kp, vp, table, lengths, key.device());
+  TORCH_CHECK_VALUE(value.device() == key.device(), "All tensors must be on the same CUDA device.");
+  TORCH_CHECK_VALUE(key.dim() == 4 && key.sizes() == value.sizes() && key.size(0) == lengths.size(0) &&
+                        key.size(1) == kp.size(1) && key.size(3) == kp.size(3),
+                    "key and value must be [batch, kv_heads, new_tokens, head_dim] and match the pages.");
+  TORCH_CHECK_VALUE(key.scalar_type() == kp.scalar_type() && value.scalar_type() == kp.scalar_type(),
+                    "key and value must have the pages' dtype.");
+  TORCH_CHECK_VALUE(key.size(3) % 8 == 0, "head_dim must be a multiple of 8.");
+  c10::cuda::CUDAGuard guard(key.device());
+  if (key.numel() == 0) return;
+  const at::Tensor k = rows(key), v = rows(value);
+  kvr_paged_append_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.key = k.data_ptr();
+  a.key_b_stride = step(k, 0), a.key_h_stride = step(k, 1), a.key_t_stride = step(k, 2);
+  a.value = v.data_ptr();
+  a.value_b_stride = step(v, 0), a.value_h_stride = step(v, 1), a.value_t_stride = step(v, 2);
+  a.key_pages = kp.data_ptr();
+  a.key_page_stride = step(kp, 0), a.key_head_stride = step(kp, 1), a.key_row_stride = step(kp, 2);
+  a.value_pages = vp.data_ptr();
+  a.value_page_stride = step(vp, 0), a.value_head_stride = step(vp, 1), a.value_row_stride = step(vp, 2);
+  a.block_table = table.data_ptr<int>();
+  a.table_stride = step(table, 0);
+  a.table_width = (int)table.size(1);
+  a.num_pages = (int)kp.size(0);
+  a.lengths = lengths.data_ptr<int>();
+  a.batch = (int)k.size(0), a.kv_heads = (int)k.size(1), a.new_tokens = (int)k.size(2), a.head_dim = (int)k.size(3);
+  a.page_size = (int)kp.size(2);
+  raise_status("kvr_paged_append", kvr_paged_append(&a, c10::cuda::getCurrentCUDAStream().stream()));
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& query, const at::Tensor& kp, const at::Tensor& vp,
+                                                   const at::Tensor& table, const at::Tensor& lengths,
+                                                   std::optional<double> scale, int64_t window, int64_t sinks,
+                                                   const std::optional<at::Tensor>& token_weights, bool with_lse) {
+  const at::Device dev = query.device();
+  check_pages(kp, vp, table, lengths, dev);
+  TORCH_CHECK_VALUE(query.dim() == 4, "query must have shape [batch, query_heads, new_tokens, head_dim].");
+  TORCH_CHECK_VALUE(query.scalar_type() == kp.scalar_type(), "query must have the pages' dtype.");
+  TORCH_CHECK_VALUE(query.size(0) == lengths.size(0), "Query and cache batch dimensions must match.");
+  TORCH_CHECK_VALUE(query.size(3) == kp.size(3), "Query and cache head dimensions must match.");
+  TORCH_CHECK_VALUE(query.size(1) > 0 && query.size(1) % kp.size(1) == 0, "Query heads must be divisible by KV heads.");
+  TORCH_CHECK_VALUE(query.size(2) > 0, "query must hold at least one new token.");
+  TORCH_CHECK_VALUE(query.size(3) == 64 || query.size(3) == 128, "head_dim must be one of [64, 128].");
+  TORCH_CHECK_VALUE(window >= 0 && sinks >= 0 && window <= INT32_MAX / 2 && sinks <= INT32_MAX / 2,
+                    "window and sinks must not be negative.");
+  TORCH_CHECK_VALUE(table.size(1) * kp.size(2) <= (1 << 30), "block_table addresses more than 2^30 tokens.");
+  const bool weighted = token_weights.has_value() && token_weights->defined();
+  if (weighted) {
+    const at::Tensor& w = *token_weights;
+    TORCH_CHECK_VALUE(w.device() == dev && w.scalar_type() == at::kFloat && w.dim() == 2 &&
+                          w.size(0) == query.size(0) && w.size(1) >= table.size(1) * kp.size(2) &&
+                          (w.size(1) <= 1 || w.stride(1) == 1),
+                      "token_weights must be fp32 [batch, >= block_table.shape[1] * page_size] with contiguous rows.");
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor out = at::empty(query.sizes(), query.options().memory_format(at::MemoryFormat::Contiguous));
+  const auto f32 = query.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor lse;
+  if (with_lse) lse = at::empty({query.size(0), query.size(1), query.size(2)}, f32);
+  if (query.numel() > 0) {
+    const at::Tensor q = rows(query);
+    kvr_paged_attention_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.query = q.data_ptr();
+    a.q_b_stride = step(q, 0), a.q_h_stride = step(q, 1), a.q_t_stride = step(q, 2);
+    a.key_pages = kp.data_ptr();
+    a.key_page_stride = step(kp, 0), a.key_head_stride = step(kp, 1), a.key_row_stride = step(kp, 2);
+    a.value_pages = vp.data_ptr();
+    a.value_page_stride = step(vp, 0), a.value_head_stride = step(vp, 1), a.value_row_stride = step(vp, 2);
+    a.block_table = table.data_ptr<int>();
+    a.table_stride = step(table, 0);
+    a.table_width = (int)table.size(1);
+    a.num_pages = (int)kp.size(0);
+    a.lengths = lengths.data_ptr<int>();
+    a.out = out.data_ptr();
+    a.lse = with_lse ? lse.data_ptr<float>() : nullptr;
+    a.token_weights = weighted ? token_weights->data_ptr<float>() : nullptr;
+    a.weights_b_stride = weighted ? step(*token_weights, 0) : 0;
+    a.dtype = q.scalar_type() == at::kHalf ? 1 : 0;
+    a.batch = (int)q.size(0), a.q_heads = (int)q.size(1), a.new_tokens = (int)q.size(2), a.head_dim = (int)q.size(3);
+    a.kv_heads = (int)kp.size(1), a.page_size = (int)kp.size(2);
+    a.window = (int)window, a.sinks = (int)sinks;
+    a.scale = scale.has_value() ? (float)*scale : (float)(1.0 / std::sqrt((double)q.size(3)));
+    size_t ws = 0, counters = 0, scores = 0;
+    raise_status("kvr_paged_attention_plan", kvr_paged_attention_plan(&a, &ws, &counters, &scores));
+    cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
+    const Scratch s = scratch_for(dev, stream, (int64_t)ws, (int64_t)counters);
+    a.workspace = s.workspace.data_ptr();
+    a.workspace_bytes = (size_t)s.workspace.numel();
+    a.counters = s.counters.data_ptr<int>();
+    at::Tensor x;
+    if (scores > 0) {
+      x = at::empty({(int64_t)scores}, at::TensorOptions().dtype(at::kByte).device(dev));
+      a.scores = x.data_ptr();
+      a.scores_bytes = scores;
+    }
+    raise_status("kvr_paged_attention", kvr_paged_attention(&a, stream));
+  }
+  if (!with_lse) lse = at::empty({0}, f32);
+  return {out, lse};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(kvr, m) {
+  m.def("paged_append(Tensor key, Tensor value, Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor block_table, "
+        "Tensor lengths) -> ()");
+  m.def("paged_attention(Tensor query, Tensor key_pages, Tensor value_pages, Tensor block_table, Tensor lengths, "
+        "float? scale=None, int window=0, int sinks=0, Tensor(a!)? token_weights=None, bool return_lse=False) "
+        "-> (Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(kvr, CUDA, m) {
+  m.impl("paged_append", &paged_append);
+  m.impl("paged_attention", &paged_attention);
+}
+
+// Host tensors reach the same functions, whose first check raises ValueError.
+TORCH_LIBRARY_IMPL(kvr, CPU, m) {
+  m.impl("paged_append", &paged_append);
+  m.impl("paged_attention", &paged_attention);
+}
