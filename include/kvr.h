@@ -458,6 +458,61 @@ int kvr_paged_attention_plan(const kvr_paged_attention_args* a, size_t* workspac
                              size_t* counter_count, size_t* scores_bytes);
 int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream_t stream);
 
+/* Eviction by accumulated attention weight: a sequence longer than keep
+ * keeps its first `first` tokens, its last `recent` and the heaviest of those
+ * between (ties: the lowest index; NaN counts as heaviest), `keep` in all;
+ * a shorter one keeps everything.  The kept tokens' rows are copied, in
+ * order, into the pages of new_block_table, which must not be pages that a
+ * block table still uses.  Writes kept [B, keep] (old positions, rising, -1
+ * behind the last), new_lengths [B], new_weights [B, keep] (0 behind the
+ * last).  Rows whose page number is not in the pool are not copied.
+ * table_width*page_size <= 320000; new_table_width*page_size must hold
+ * min(keep, table_width*page_size) tokens (KVR_ERR_CAPACITY).              */
+typedef struct {
+  void* key_pages; int64_t key_page_stride, key_head_stride, key_row_stride;
+  void* value_pages; int64_t value_page_stride, value_head_stride, value_row_stride;
+  const int* block_table; int64_t table_stride; int table_width; int num_pages;
+  const int* new_block_table; int64_t new_table_stride; int new_table_width;
+  const int* lengths;
+  const float* token_weights; int64_t weights_b_stride;
+  int* kept; int* new_lengths; float* new_weights;
+  int batch, kv_heads, head_dim, page_size, keep, recent, first;
+} kvr_paged_evict_args;
+int kvr_paged_evict(const kvr_paged_evict_args* a, kvr_stream_t stream);
+
+/* ------------------------------------------------ draft verification
+ * Speculative sampling from given random numbers: p = softmax(target / t),
+ * q = softmax(draft / t); drafted token x_k is accepted while
+ * u_k < min(1, p_k(x_k)/q_k(x_k)); then one more token: at the first refusal
+ * j the argmax of max(p_j - q_j, 0)/e (of p_j/e where nothing is left), after
+ * a full acceptance the argmax of p_K/e, e > 0 exponential numbers [B, V].
+ * t = 0: accepted while x_k is target_k's argmax (draft, uniforms and noise
+ * unused).  Ties: the lowest index.
+ *   target [B, K+1, V], draft [B, K, V] (strides in elements, V contiguous,
+ *   any alignment), tokens int64 [B, K], uniforms [B, K], draft_lengths [B]
+ *   or NULL: positions in use of each sequence.
+ *   out_tokens int64 [B, K+1]: the accepted tokens, the new one, then -1
+ *   (-1 also where a row has no weight at all); accepted int [B];
+ *   accept_prob [B, K]: min(1, p/q), 0 behind the first refusal.
+ * kvr_verify_plan: bytes of `zeroed` (zero before the first call, left zero
+ * by every completed one) and of workspace.                               */
+typedef struct {
+  const void* target; int64_t target_b_stride, target_k_stride;
+  const void* draft; int64_t draft_b_stride, draft_k_stride;
+  const int64_t* tokens; int64_t tokens_b_stride;
+  const float* uniforms; int64_t uniforms_b_stride;
+  const float* noise; int64_t noise_b_stride;
+  const int* draft_lengths;
+  int64_t* out_tokens; int* accepted; float* accept_prob;
+  int dtype;            /* 0 bf16, 1 fp16, 2 fp32: target and draft */
+  int batch, draft_tokens, vocab;
+  float temperature;
+  void* zeroed; size_t zeroed_bytes;
+  void* workspace; size_t workspace_bytes;
+} kvr_verify_args;
+int kvr_verify_plan(const kvr_verify_args* a, size_t* zeroed_bytes, size_t* workspace_bytes);
+int kvr_verify(const kvr_verify_args* a, kvr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,7 +30,8 @@ from .packed_kv_attention import (  # noqa: F401
     packed_kv_decode_attention_simt,
     theoretical_attention_flops,
 )
-from .paged import paged_append, paged_decode_attention  # noqa: F401
+from .paged import paged_append, paged_decode_attention, paged_evict  # noqa: F401
+from .speculative import VerifyResult, verify_draft_tokens  # noqa: F401
 from .streaming import PackedCache, PackedKVCache, PackedKVCacheLayer, PackedLayer  # noqa: F401
 
 __version__ = "0.1.0"

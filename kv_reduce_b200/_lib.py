@@ -66,6 +66,9 @@ EXPORTED_SYMBOLS = (
     "kvr_paged_append",
     "kvr_paged_attention_plan",
     "kvr_paged_attention",
+    "kvr_paged_evict",
+    "kvr_verify_plan",
+    "kvr_verify",
 )
 
 
@@ -203,6 +206,34 @@ class PagedAttentionArgs(Structure):
     ]
 
 
+class PagedEvictArgs(Structure):
+    _fields_ = [
+        ("key_pages", c_void_p), ("key_page_stride", c_int64), ("key_head_stride", c_int64),
+        ("key_row_stride", c_int64),
+        ("value_pages", c_void_p), ("value_page_stride", c_int64), ("value_head_stride", c_int64),
+        ("value_row_stride", c_int64),
+        ("block_table", c_void_p), ("table_stride", c_int64), ("table_width", c_int), ("num_pages", c_int),
+        ("new_block_table", c_void_p), ("new_table_stride", c_int64), ("new_table_width", c_int),
+        ("lengths", c_void_p), ("token_weights", c_void_p), ("weights_b_stride", c_int64),
+        ("kept", c_void_p), ("new_lengths", c_void_p), ("new_weights", c_void_p),
+        ("batch", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("page_size", c_int), ("keep", c_int),
+        ("recent", c_int), ("first", c_int),
+    ]
+
+
+class VerifyArgs(Structure):
+    _fields_ = [
+        ("target", c_void_p), ("target_b_stride", c_int64), ("target_k_stride", c_int64),
+        ("draft", c_void_p), ("draft_b_stride", c_int64), ("draft_k_stride", c_int64),
+        ("tokens", c_void_p), ("tokens_b_stride", c_int64), ("uniforms", c_void_p), ("uniforms_b_stride", c_int64),
+        ("noise", c_void_p), ("noise_b_stride", c_int64), ("draft_lengths", c_void_p),
+        ("out_tokens", c_void_p), ("accepted", c_void_p), ("accept_prob", c_void_p),
+        ("dtype", c_int), ("batch", c_int), ("draft_tokens", c_int), ("vocab", c_int),
+        ("temperature", ctypes.c_float),
+        ("zeroed", c_void_p), ("zeroed_bytes", c_size_t), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 _lib = None
 
 
@@ -257,6 +288,9 @@ def load() -> ctypes.CDLL:
     lib.kvr_paged_attention_plan.argtypes = [POINTER(PagedAttentionArgs), POINTER(c_size_t), POINTER(c_size_t),
                                              POINTER(c_size_t)]
     lib.kvr_paged_attention.argtypes = [POINTER(PagedAttentionArgs), c_void_p]
+    lib.kvr_paged_evict.argtypes = [POINTER(PagedEvictArgs), c_void_p]
+    lib.kvr_verify_plan.argtypes = [POINTER(VerifyArgs), POINTER(c_size_t), POINTER(c_size_t)]
+    lib.kvr_verify.argtypes = [POINTER(VerifyArgs), c_void_p]
     for name in EXPORTED_SYMBOLS:
         if name not in ("kvr_version", "kvr_status_string", "kvr_last_error"):
             getattr(lib, name).restype = c_int

@@ -18,7 +18,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libkvr.so"
 TORCH_LIB = PKG / "libkvr_torch.so"
-SOURCES = ["kvr_capi.cu", "kvr_pack.cu", "kvr_decode.cu", "kvr_decode_simt.cu", "kvr_exchange.cu", "kvr_paged.cu"]
+SOURCES = ["kvr_capi.cu", "kvr_pack.cu", "kvr_decode.cu", "kvr_decode_simt.cu", "kvr_exchange.cu", "kvr_paged.cu",
+           "kvr_evict.cu", "kvr_verify.cu"]
 TORCH_SOURCES = ["kvr_torch.cpp", "kvr_torch_paged.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -3,6 +3,8 @@
 //
 //   kvr::paged_append     new tokens' keys and values into their pages
 //   kvr::paged_attention  attention of the new tokens over the pages
+//   kvr::paged_evict      the kept tokens of every sequence into new pages
+//   kvr::verify_draft     accepted drafted tokens and the next one
 //
 // Checks raise ValueError before anything is allocated or launched.  Outputs
 // come from the caching allocator.  The join's scratch is cached per
@@ -16,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <map>
@@ -205,6 +208,129 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& query, cons
   return {out, lse};
 }
 
+std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_evict(const at::Tensor& kp, const at::Tensor& vp,
+                                                           const at::Tensor& table, const at::Tensor& lengths,
+                                                           const at::Tensor& weights, const at::Tensor& new_table,
+                                                           int64_t keep, int64_t recent, int64_t first) {
+  const at::Device dev = kp.device();
+  check_pages(kp, vp, table, lengths, dev);
+  TORCH_CHECK_VALUE(weights.device() == dev && new_table.device() == dev, "All tensors must be on the same CUDA device.");
+  const int64_t B = table.size(0), cap = table.size(1) * kp.size(2);
+  TORCH_CHECK_VALUE(keep > 0 && keep <= INT32_MAX / 2 && recent >= 0 && first >= 0 && first + recent <= keep,
+                    "keep must be positive and hold first + recent tokens.");
+  TORCH_CHECK_VALUE(weights.scalar_type() == at::kFloat && weights.dim() == 2 && weights.size(0) == B &&
+                        weights.size(1) >= cap && (weights.size(1) <= 1 || weights.stride(1) == 1),
+                    "token_weights must be fp32 [batch, >= block_table.shape[1] * page_size] with contiguous rows.");
+  TORCH_CHECK_VALUE(new_table.dim() == 2 && new_table.scalar_type() == at::kInt && new_table.size(0) == B &&
+                        (new_table.size(1) <= 1 || new_table.stride(1) == 1),
+                    "new_block_table must be int32 [batch, pages] with contiguous rows.");
+  TORCH_CHECK_VALUE(new_table.size(1) * kp.size(2) >= std::min(keep, cap),
+                    "new_block_table must hold pages for min(keep, block_table.shape[1] * page_size) tokens.");
+  TORCH_CHECK_VALUE(cap <= 320000, "eviction takes block tables of up to 320000 tokens.");
+  TORCH_CHECK_VALUE(kp.size(3) % 8 == 0, "head_dim must be a multiple of 8.");
+  c10::cuda::CUDAGuard guard(dev);
+  const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
+  at::Tensor kept = at::empty({B, keep}, i32), new_lengths = at::empty({B}, i32);
+  at::Tensor new_weights = at::empty({B, keep}, i32.dtype(at::kFloat));
+  kvr_paged_evict_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.key_pages = kp.data_ptr();
+  a.key_page_stride = step(kp, 0), a.key_head_stride = step(kp, 1), a.key_row_stride = step(kp, 2);
+  a.value_pages = vp.data_ptr();
+  a.value_page_stride = step(vp, 0), a.value_head_stride = step(vp, 1), a.value_row_stride = step(vp, 2);
+  a.block_table = table.data_ptr<int>(), a.table_stride = step(table, 0), a.table_width = (int)table.size(1);
+  a.num_pages = (int)kp.size(0);
+  a.new_block_table = new_table.data_ptr<int>(), a.new_table_stride = step(new_table, 0);
+  a.new_table_width = (int)new_table.size(1);
+  a.lengths = lengths.data_ptr<int>();
+  a.token_weights = weights.data_ptr<float>(), a.weights_b_stride = step(weights, 0);
+  a.kept = kept.data_ptr<int>(), a.new_lengths = new_lengths.data_ptr<int>(), a.new_weights = new_weights.data_ptr<float>();
+  a.batch = (int)B, a.kv_heads = (int)kp.size(1), a.head_dim = (int)kp.size(3), a.page_size = (int)kp.size(2);
+  a.keep = (int)keep, a.recent = (int)recent, a.first = (int)first;
+  raise_status("kvr_paged_evict", kvr_paged_evict(&a, c10::cuda::getCurrentCUDAStream().stream()));
+  return {kept, new_lengths, new_weights};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_draft(const at::Tensor& target,
+                                                            const std::optional<at::Tensor>& draft,
+                                                            const at::Tensor& tokens,
+                                                            const std::optional<at::Tensor>& uniforms,
+                                                            const std::optional<at::Tensor>& noise,
+                                                            double temperature,
+                                                            const std::optional<at::Tensor>& draft_lengths) {
+  const at::Device dev = target.device();
+  TORCH_CHECK_VALUE(dev.is_cuda(), "kv_reduce_b200 operates on CUDA tensors only (no CPU fallback).");
+  TORCH_CHECK_VALUE(target.dim() == 3 && target.size(1) > 0 && target.size(2) > 0,
+                    "target_logits must be [batch, draft + 1, vocab].");
+  const at::ScalarType type = target.scalar_type();
+  TORCH_CHECK_VALUE(is_half_type(type) || type == at::kFloat, "logits must be bf16, fp16 or fp32.");
+  const int64_t B = target.size(0), K = target.size(1) - 1, V = target.size(2);
+  TORCH_CHECK_VALUE(V <= (1 << 30), "vocab must be at most 2^30.");
+  TORCH_CHECK_VALUE(temperature >= 0 && std::isfinite(temperature), "temperature must be 0 or a positive finite number.");
+  TORCH_CHECK_VALUE(tokens.device() == dev && tokens.dim() == 2 && tokens.size(0) == B && tokens.size(1) == K &&
+                        (tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt),
+                    "draft_tokens must be int64 or int32 [batch, draft] on the logits' device.");
+  const bool greedy = temperature == 0;
+  auto given = [](const std::optional<at::Tensor>& t) { return t.has_value() && t->defined(); };
+  if (!greedy) {
+    TORCH_CHECK_VALUE(given(draft) && given(uniforms) && given(noise),
+                      "sampling (temperature > 0) needs draft_logits, uniforms and noise.");
+    TORCH_CHECK_VALUE(draft->device() == dev && draft->scalar_type() == type && draft->dim() == 3 &&
+                          draft->size(0) == B && draft->size(1) == K && draft->size(2) == V,
+                      "draft_logits must be [batch, draft, vocab] of the target's dtype and device.");
+    TORCH_CHECK_VALUE(uniforms->device() == dev && uniforms->scalar_type() == at::kFloat && uniforms->dim() == 2 &&
+                          uniforms->size(0) == B && uniforms->size(1) == K,
+                      "uniforms must be fp32 [batch, draft].");
+    TORCH_CHECK_VALUE(noise->device() == dev && noise->scalar_type() == at::kFloat && noise->dim() == 2 &&
+                          noise->size(0) == B && noise->size(1) == V,
+                      "noise must be fp32 [batch, vocab].");
+  }
+  if (given(draft_lengths))
+    TORCH_CHECK_VALUE(draft_lengths->device() == dev && draft_lengths->scalar_type() == at::kInt &&
+                          draft_lengths->dim() == 1 && draft_lengths->size(0) == B &&
+                          (B <= 1 || draft_lengths->stride(0) == 1),
+                      "draft_lengths must be a contiguous int32 [batch] tensor.");
+  c10::cuda::CUDAGuard guard(dev);
+  const auto f32 = at::TensorOptions().dtype(at::kFloat).device(dev);
+  at::Tensor out = at::empty({B, K + 1}, f32.dtype(at::kLong)), accepted = at::empty({B}, f32.dtype(at::kInt));
+  at::Tensor prob = at::empty({B, K}, f32);
+  if (B == 0) return {out, accepted, prob};
+  // rows with contiguous elements, at any alignment; others are copied
+  auto last_contiguous = [](const at::Tensor& t) {
+    return t.size(t.dim() - 1) <= 1 || t.stride(t.dim() - 1) == 1 ? t : t.contiguous();
+  };
+  const at::Tensor t = last_contiguous(target), x = last_contiguous(tokens.to(at::kLong));
+  at::Tensor d, u, e;
+  kvr_verify_args a;
+  std::memset(&a, 0, sizeof(a));
+  a.target = t.data_ptr(), a.target_b_stride = step(t, 0), a.target_k_stride = step(t, 1);
+  if (K > 0) a.tokens = x.data_ptr<int64_t>(), a.tokens_b_stride = step(x, 0);
+  if (!greedy) {
+    e = last_contiguous(*noise);
+    a.noise = e.data_ptr<float>(), a.noise_b_stride = step(e, 0);
+    if (K > 0) {
+      d = last_contiguous(*draft), u = last_contiguous(*uniforms);
+      a.draft = d.data_ptr(), a.draft_b_stride = step(d, 0), a.draft_k_stride = step(d, 1);
+      a.uniforms = u.data_ptr<float>(), a.uniforms_b_stride = step(u, 0);
+    }
+  }
+  if (given(draft_lengths)) a.draft_lengths = draft_lengths->data_ptr<int>();
+  a.out_tokens = out.data_ptr<int64_t>(), a.accepted = accepted.data_ptr<int>();
+  a.accept_prob = K > 0 ? prob.data_ptr<float>() : nullptr;
+  a.dtype = type == at::kBFloat16 ? 0 : type == at::kHalf ? 1 : 2;
+  a.batch = (int)B, a.draft_tokens = (int)K, a.vocab = (int)V;
+  a.temperature = (float)temperature;
+  TORCH_CHECK_VALUE(greedy || a.temperature >= FLT_MIN, "temperature is too small for fp32.");
+  size_t zeroed = 0, ws = 0;
+  raise_status("kvr_verify_plan", kvr_verify_plan(&a, &zeroed, &ws));
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
+  const Scratch s = scratch_for(dev, stream, (int64_t)ws, (int64_t)(zeroed + 3) / 4);
+  a.zeroed = s.counters.data_ptr(), a.zeroed_bytes = (size_t)s.counters.numel() * 4;
+  a.workspace = s.workspace.data_ptr(), a.workspace_bytes = (size_t)s.workspace.numel();
+  raise_status("kvr_verify", kvr_verify(&a, stream));
+  return {out, accepted, prob};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(kvr, m) {
@@ -213,15 +339,23 @@ TORCH_LIBRARY_FRAGMENT(kvr, m) {
   m.def("paged_attention(Tensor query, Tensor key_pages, Tensor value_pages, Tensor block_table, Tensor lengths, "
         "float? scale=None, int window=0, int sinks=0, Tensor(a!)? token_weights=None, bool return_lse=False) "
         "-> (Tensor, Tensor)");
+  m.def("paged_evict(Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor block_table, Tensor lengths, "
+        "Tensor token_weights, Tensor new_block_table, int keep, int recent, int first) -> (Tensor, Tensor, Tensor)");
+  m.def("verify_draft(Tensor target_logits, Tensor? draft_logits, Tensor draft_tokens, Tensor? uniforms, "
+        "Tensor? noise, float temperature=1.0, Tensor? draft_lengths=None) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(kvr, CUDA, m) {
   m.impl("paged_append", &paged_append);
   m.impl("paged_attention", &paged_attention);
+  m.impl("paged_evict", &paged_evict);
+  m.impl("verify_draft", &verify_draft);
 }
 
 // Host tensors reach the same functions, whose first check raises ValueError.
 TORCH_LIBRARY_IMPL(kvr, CPU, m) {
   m.impl("paged_append", &paged_append);
   m.impl("paged_attention", &paged_attention);
+  m.impl("paged_evict", &paged_evict);
+  m.impl("verify_draft", &verify_draft);
 }

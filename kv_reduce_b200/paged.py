@@ -26,13 +26,15 @@ from . import _lib
 
 _append_op = None
 _attention_op = None
+_evict_op = None
 
 
 def _bind_ops() -> None:
-    global _append_op, _attention_op
+    global _append_op, _attention_op, _evict_op
     _lib.load_torch_ops()
     _append_op = torch.ops.kvr.paged_append.default
     _attention_op = torch.ops.kvr.paged_attention.default
+    _evict_op = torch.ops.kvr.paged_evict.default
 
 
 def paged_append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
@@ -81,3 +83,34 @@ def paged_decode_attention(
     out, lse = _attention_op(query, key_pages, value_pages, block_table, lengths, scale, window, sinks, token_weights,
                              return_lse)
     return (out, lse) if return_lse else out
+
+
+def paged_evict(
+    key_pages: torch.Tensor,
+    value_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    token_weights: torch.Tensor,
+    new_block_table: torch.Tensor,
+    *,
+    keep: int,
+    recent: int = 0,
+    first: int = 0,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Bring every sequence down to ``keep`` tokens by accumulated weight.
+
+    A sequence longer than ``keep`` keeps its first ``first`` tokens, its last
+    ``recent`` ones and the heaviest of those between by ``token_weights``
+    (ties: the lowest position; NaN counts as heaviest); a shorter one keeps
+    all.  The kept rows are copied, in order, into the pages of
+    ``new_block_table`` (int32 [batch, pages]), which must be free: not pages
+    that a block table still uses.  Pages that sequences share stay whole.
+
+    Returns ``kept`` (int32 [batch, keep], old positions, -1 behind the last),
+    the new lengths (int32 [batch]) and the kept tokens' weights (fp32
+    [batch, keep], 0 behind the last).  The keys keep the rotary positions
+    they were written with.
+    """
+    if _evict_op is None:
+        _bind_ops()
+    return _evict_op(key_pages, value_pages, block_table, lengths, token_weights, new_block_table, keep, recent, first)
