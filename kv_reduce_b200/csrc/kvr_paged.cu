@@ -12,27 +12,34 @@
 // and 4*D*R operations for the R = T*q_heads/kv_heads query rows that share
 // it, so R operations per byte, far below the tensor cores' rate for the few
 // rows of a decode step.  The kernel is therefore laid out around keeping
-// loads in flight:
+// loads in flight and the instructions per tile few:
 //  * Work is a flat list of token tiles (sequence, KV head, row tile, tile),
 //    cut into equal ranges, one per CTA.  Lengths are read on the device, so
 //    a ragged batch is balanced to one tile without the host knowing it.
-//  * The tiles stream through a cp.async ring that runs on across sequence
-//    boundaries; page numbers are looked up one step ahead of the copies.
-//  * The four warps of a CTA share each tile: for the scores a warp owns a
-//    quarter of the tokens, for the output a quarter of the head dimension,
-//    so every byte of K and V is read from shared memory once and the
-//    accumulator is complete in the CTA: nothing is merged between warps.
+//  * A producer warp looks up pages and fills a ring of tiles, on across
+//    sequence boundaries; four consumer warps compute.  Pages of a multiple
+//    of 8 tokens come by TMA, a box per page; others row by row (cp.async).
+//  * The consumers share each tile: for the scores a warp owns a quarter of
+//    the tokens, for the output a quarter of the head dimension, so every
+//    byte of K and V is read from shared memory once and the accumulator is
+//    complete in the CTA: nothing is merged between warps.
 //  * A sequence that several CTAs share is joined by the last of them to
 //    arrive, in the order of the CTAs: the result does not depend on timing.
 #include "kvr_common.cuh"
 
+#include <cuda.h>
+
 #include <algorithm>
+#include <cstring>
 
 namespace kvr {
 namespace paged {
 
-constexpr int kThreads = 128;
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;                     // consumers
+constexpr int kConsumers = 32 * kWarps;
+constexpr int kThreads = kConsumers + 32;     // and the producer warp
+constexpr int kGroup = 16;                    // CTAs a join takes at a time
+constexpr long long kWaitLimitNs = 2000000000ll;
 
 // Rows that no mask leaves anything to keep m = -inf; 0 stands in for it
 // wherever it would be subtracted.
@@ -65,6 +72,55 @@ __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r
                : "r"(addr));
 }
 
+// ---- mbarriers.  A wait that runs out (which no input causes) is given up
+// after kWaitLimitNs: every later wait of the thread returns at once, the
+// loops end, and the outputs are NaN.
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_arrive_tx(uint32_t bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, int parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ long long now_ns() {
+  long long t;
+  asm volatile("mov.u64 %0, %globaltimer;\n" : "=l"(t));
+  return t;
+}
+__device__ __noinline__ bool bar_wait_long(uint32_t bar, int parity) {
+  const long long begin = now_ns();
+  while (now_ns() - begin < kWaitLimitNs)
+    for (int i = 0; i < 64; ++i)
+      if (bar_try(bar, parity)) return true;
+  return false;
+}
+__device__ __forceinline__ void bar_wait(uint32_t bar, int parity, bool& failed) {
+  if (bar_try(bar, parity) || failed) return;
+  failed = !bar_wait_long(bar, parity);
+}
+__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); }
+
+// A box of `rows` tokens x 64 elements of one head of one page.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int col, int row, int head,
+                                        int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];\n" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(col), "r"(row), "r"(head), "r"(page)
+      : "memory");
+}
+
 struct Params {
   const uint16_t* q;
   int64_t q_b, q_h, q_t;
@@ -86,39 +142,42 @@ struct Params {
   int ctas, min_tiles;
   float* part_o;    // [2 * ctas][ROWS][D]
   float* part_ml;   // [2 * ctas][ROWS][2]
-  int* counters;    // [ctas], zero on entry and on exit
+  int* counters;    // [2 * ctas], zero on entry and on exit
+  int box;          // tokens of a TMA box
 };
 
 template <int D, int MT>
 struct Cfg {
   static constexpr int TILE = D == 64 ? 128 : 64;   // tokens: 16 KB of K and 16 KB of V either way
   static constexpr int ROWS = 16 * MT;
-  static constexpr int ROW_BYTES = 2 * D;
+  static constexpr int HALVES = D / 64;
   static constexpr int PIECES = D / 8;
-  static constexpr int KV_BYTES = TILE * ROW_BYTES;
+  static constexpr int HALF_BYTES = TILE * 128;     // 64 elements of every token, 128-byte rows
+  static constexpr int KV_BYTES = HALVES * HALF_BYTES;
   static constexpr int STAGE = 2 * KV_BYTES;
   static constexpr int STAGES = MT == 4 ? 2 : 3;    // two CTAs per SM in every case
   static constexpr int NT = TILE / kWarps / 8;      // 8-token score tiles of a warp
   static constexpr int DW = D / kWarps;             // output columns of a warp
   static constexpr int DT = DW / 8;
-  static constexpr int DESCS = 4;
-  // shared memory: ring, Q, P, row offsets, descriptors, row statistics
-  // (MT <= 2 keeps Q in registers and lets P take its place)
-  static constexpr int Q_BYTES = ROWS * ROW_BYTES, P_HALF = ROWS * TILE * 2, P_BYTES = 2 * P_HALF;
+  // shared memory: ring, Q (MT <= 2 keeps it in registers and lets P take its place), P, descriptors, row
+  // statistics, barriers
+  static constexpr int Q_BYTES = ROWS * D * 2, P_HALF = ROWS * TILE * 2, P_BYTES = 2 * P_HALF;
   static constexpr int OFF_Q = STAGES * STAGE;
   static constexpr int OFF_P = MT <= 2 ? OFF_Q : OFF_Q + Q_BYTES;
-  static constexpr int OFF_ROW = OFF_Q + (MT <= 2 ? (Q_BYTES > P_BYTES ? Q_BYTES : P_BYTES) : Q_BYTES + P_BYTES);
-  static constexpr int OFF_DESC = OFF_ROW + STAGES * TILE * 16;
-  static constexpr int OFF_MAX = OFF_DESC + DESCS * 64;
+  static constexpr int OFF_DESC = OFF_Q + (MT <= 2 ? (Q_BYTES > P_BYTES ? Q_BYTES : P_BYTES) : Q_BYTES + P_BYTES);
+  static constexpr int OFF_MAX = OFF_DESC + STAGES * 80;
   static constexpr int OFF_SUM = OFF_MAX + kWarps * ROWS * 4;
-  static constexpr int SMEM = OFF_SUM + kWarps * ROWS * 4 + 64;
+  static constexpr int OFF_BAR = OFF_SUM + kWarps * ROWS * 4;
+  static constexpr int OFF_MISC = OFF_BAR + 2 * STAGES * 8 + 16;
+  static constexpr int SMEM = OFF_MISC + 96 + 1024;   // 1 KB to align the ring
 };
 
 struct Desc {
   int b, h, rt, token0, len, first, last, n_tiles;
   int64_t seg_start;
+  uint32_t bad[4];   // tokens on pages outside the pool, a bit each
 };
-static_assert(sizeof(Desc) <= 64, "");
+static_assert(sizeof(Desc) <= 80, "");
 
 // The tiles a sequence's queries look at: with a window, `ns` tiles that hold
 // the sinks, then the tiles from `lo_tile` on.
@@ -137,25 +196,36 @@ __device__ __forceinline__ Span span_of(const Params& p, int len) {
 }
 __device__ __forceinline__ int length_of(const Params& p, int b) { return min(max(p.lengths[b], 0), p.cap); }
 
-template <bool HALF, int D, int MT>
-__global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_constant__ Params p) {
+template <bool HALF, int D, int MT, bool TMA>
+__global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_constant__ Params p,
+                                                                const __grid_constant__ CUtensorMap kmap,
+                                                                const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<D, MT>;
   constexpr int TILE = C::TILE, ROWS = C::ROWS, S = C::STAGES;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ uint8_t raw_smem[];
+  // the swizzle pattern of a tile follows address bits 7..9: align the ring to 1 KB
+  uint8_t* smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
   const uint32_t sbase = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t* row_off = reinterpret_cast<int64_t*>(smem + C::OFF_ROW);   // [S][TILE][2]
   Desc* descs = reinterpret_cast<Desc*>(smem + C::OFF_DESC);
   float* smax = reinterpret_cast<float*>(smem + C::OFF_MAX);
   float* ssum = reinterpret_cast<float*>(smem + C::OFF_SUM);
+  const uint32_t full = sbase + C::OFF_BAR, empty = full + S * 8;
+  int64_t* s_start = reinterpret_cast<int64_t*>(smem + C::OFF_MISC);   // [3]
+  int64_t* s_scan = s_start + 3;                                       // [kThreads / 32]
+  int* s_last = reinterpret_cast<int*>(s_scan + kThreads / 32);
 
+  if (tid == 0) {
+    for (int i = 0; i < S; ++i) {
+      bar_init(full + 8 * i, TMA ? 1 : 33);
+      bar_init(empty + 8 * i, kWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
   pdl_wait();
 
   // ---- this CTA's range of the flat tile list
   const int HR = p.HKV * p.row_tiles;
-  __shared__ int64_t s_start[4];   // {sequence, tiles before it, total}
-  __shared__ int64_t s_scan[kWarps];
-  __shared__ int s_last;
   int64_t total, g0, g1;
   {
     const int per = (p.B + kThreads - 1) / kThreads;
@@ -173,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
     int64_t base = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) base += s_scan[w];
       total += s_scan[w];
     }
@@ -198,160 +268,180 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
     }
     __syncthreads();
   }
-  const int64_t ctas = s_start[2];
   const int count = (int)(g1 - g0);
+  bool failed = false;
 
-  // ---- loader state: the next tile to look up
-  int ld_b = (int)s_start[0], ld_left = count, ld_hr, ld_tile;
-  int ld_len = length_of(p, ld_b);
-  bool ld_over = p.lengths[ld_b] > p.cap;
-  Span ld_span = span_of<TILE>(p, ld_len);
-  int64_t ld_seg = s_start[1] * HR;
-  {
-    const int64_t off = g0 - ld_seg;
-    ld_hr = (int)(off / ld_span.n);
-    ld_tile = (int)(off - (int64_t)ld_hr * ld_span.n);
-    ld_seg += (int64_t)ld_hr * ld_span.n;
-  }
-  int next_raw = ld_b + 1 < p.B ? p.lengths[ld_b + 1] : 0;
-  bool ld_first = true;
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ producer
+    int ld_b = (int)s_start[0], ld_left = count, ld_hr, ld_tile;
+    int ld_len = length_of(p, ld_b);
+    bool ld_over = p.lengths[ld_b] > p.cap;
+    Span ld_span = span_of<TILE>(p, ld_len);
+    int64_t ld_seg = s_start[1] * HR;
+    {
+      const int64_t off = g0 - ld_seg;
+      ld_hr = (int)(off / ld_span.n);
+      ld_tile = (int)(off - (int64_t)ld_hr * ld_span.n);
+      ld_seg += (int64_t)ld_hr * ld_span.n;
+    }
+    int next_raw = ld_b + 1 < p.B ? p.lengths[ld_b + 1] : 0;
+    bool ld_first = true;
 
-  // One lookup: thread `tid` < TILE finds the page of token tid of the tile.
-  // The page number is loaded here and used in `finish`, one iteration later.
-  struct Lookup {
-    int page_id, row, state;   // state 0: not needed, 1: page_id is valid once loaded, 2: outside the table
-    Desc d;
-    bool any;
-  };
-  auto look = [&]() {
-    Lookup u;
-    u.any = ld_left > 0;
-    u.page_id = 0;
-    u.row = 0;
-    u.state = 0;
-    if (!u.any) return u;
-    const int token0 = (ld_tile < ld_span.ns ? ld_tile : ld_span.lo_tile + ld_tile - ld_span.ns) * TILE;
-    u.d.b = ld_b;
-    u.d.h = ld_hr / p.row_tiles;
-    u.d.rt = ld_hr - u.d.h * p.row_tiles;
-    u.d.token0 = token0;
-    u.d.len = ld_len;
-    u.d.first = ld_first;
-    u.d.n_tiles = ld_span.n;
-    u.d.seg_start = ld_seg;
-    --ld_left;
-    u.d.last = ld_left == 0 || ld_tile + 1 == ld_span.n;
-    if (tid < TILE) {
-      const int j = token0 + tid;
-      if (j < ld_len && (j >= ld_span.lo || j < p.sinks)) {
-        const int pg = j / p.page;
-        u.row = j - pg * p.page;
-        u.state = ld_over ? 2 : 1;
-        u.page_id = __ldg(p.table + (int64_t)ld_b * p.table_b + pg);
-      }
-    }
-    ld_first = false;
-    if (++ld_tile == ld_span.n && ld_left > 0) {
-      ld_first = true;
-      ld_tile = 0;
-      ld_seg += ld_span.n;
-      if (++ld_hr == HR) {
-        ld_hr = 0;
-        ++ld_b;
-        ld_len = min(max(next_raw, 0), p.cap);
-        ld_over = next_raw > p.cap;
-        ld_span = span_of<TILE>(p, ld_len);
-        next_raw = ld_b + 1 < p.B ? p.lengths[ld_b + 1] : 0;
-      }
-    }
-    return u;
-  };
-  auto finish = [&](const Lookup& u, int slot, int dslot) {
-    if (!u.any) return;
-    if (tid < TILE) {
-      int64_t ko = -1, vo = -1;
-      if (u.state) {
-        const bool bad = u.state == 2 || u.page_id < 0 || u.page_id >= p.num_pages;
-        ko = bad ? -2 : (int64_t)u.page_id * p.k_page + (int64_t)u.d.h * p.k_head + (int64_t)u.row * p.k_row;
-        vo = bad ? -1 : (int64_t)u.page_id * p.v_page + (int64_t)u.d.h * p.v_head + (int64_t)u.row * p.v_row;
-      }
-      row_off[(slot * TILE + tid) * 2] = ko;
-      row_off[(slot * TILE + tid) * 2 + 1] = vo;
-    }
-    if (tid == 0) descs[dslot] = u.d;
-  };
-  // Copies of one tile: rows of D elements in 16-byte pieces, piece c of row
-  // r at c ^ (r & 7), so that the 8 rows of an ldmatrix hit 8 bank groups.
-  auto issue = [&](int slot) {
-    constexpr int RPI = kThreads / C::PIECES;   // rows per step
-    const int c = tid % C::PIECES;
-    const uint32_t kdst = sbase + slot * C::STAGE, vdst = kdst + C::KV_BYTES;
+    // A tile's pages: a lane looks up one TMA box, or TILE / 32 rows.  The
+    // page numbers loaded here are used one tile later.
+    constexpr int LU = TMA ? 1 : TILE / 32;
+    struct Lookup {
+      int id[LU], row[LU], state[LU];   // state 0: no query sees it, 1: on page `id`, 2: past the table
+      Desc d;
+    };
+    auto look = [&](Lookup& u) {
+      if (ld_left <= 0) return;
+      const int token0 = (ld_tile < ld_span.ns ? ld_tile : ld_span.lo_tile + ld_tile - ld_span.ns) * TILE;
+      u.d.b = ld_b;
+      u.d.h = ld_hr / p.row_tiles;
+      u.d.rt = ld_hr - u.d.h * p.row_tiles;
+      u.d.token0 = token0;
+      u.d.len = ld_len;
+      u.d.first = ld_first;
+      u.d.n_tiles = ld_span.n;
+      u.d.seg_start = ld_seg;
+      --ld_left;
+      u.d.last = ld_left == 0 || ld_tile + 1 == ld_span.n;
+      const int step = TMA ? p.box : 1;
 #pragma unroll
-    for (int i = 0; i < TILE / RPI; ++i) {
-      const int r = tid / C::PIECES + i * RPI;
-      const longlong2 off = *reinterpret_cast<const longlong2*>(&row_off[(slot * TILE + r) * 2]);
-      const uint32_t at = r * C::ROW_BYTES + ((c ^ (r & 7)) << 4);
-      if (off.x >= 0) {
-        cp_async16(kdst + at, p.k + off.x + c * 8);
-        cp_async16(vdst + at, p.v + off.y + c * 8);
+      for (int x = 0; x < LU; ++x) {
+        const int at = (x * 32 + lane) * step, j = token0 + at;
+        u.state[x] = 0;
+        u.id[x] = 0;
+        u.row[x] = 0;
+        if (at < TILE && j < ld_len && (j + step > ld_span.lo || j < p.sinks)) {
+          const int pg = j / p.page;
+          u.row[x] = j - pg * p.page;
+          u.state[x] = ld_over ? 2 : 1;
+          u.id[x] = __ldg(p.table + (int64_t)ld_b * p.table_b + pg);
+        }
+      }
+      ld_first = false;
+      if (++ld_tile == ld_span.n && ld_left > 0) {
+        ld_first = true;
+        ld_tile = 0;
+        ld_seg += ld_span.n;
+        if (++ld_hr == HR) {
+          ld_hr = 0;
+          ++ld_b;
+          ld_len = min(max(next_raw, 0), p.cap);
+          ld_over = next_raw > p.cap;
+          ld_span = span_of<TILE>(p, ld_len);
+          next_raw = ld_b + 1 < p.B ? p.lengths[ld_b + 1] : 0;
+        }
+      }
+    };
+    Lookup next;
+    look(next);
+    for (int i = 0; i < count; ++i) {
+      Lookup u = next;
+      look(next);
+      const int slot = i % S;
+      if (i >= S) bar_wait(empty + 8 * slot, (i / S - 1) & 1, failed);
+      const uint32_t kdst = sbase + slot * C::STAGE, vdst = kdst + C::KV_BYTES;
+      if constexpr (TMA) {
+        const bool ok = u.state[0] == 1 && u.id[0] >= 0 && u.id[0] < p.num_pages;
+        const uint32_t good = __ballot_sync(0xffffffffu, ok);
+        const uint32_t bad = __ballot_sync(0xffffffffu, u.state[0] != 0 && !ok);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) u.d.bad[w] = 0;
+        if (bad)
+#pragma unroll
+          for (int w = 0; w < TILE / 32; ++w)
+            u.d.bad[w] = __ballot_sync(0xffffffffu, (bad >> ((w * 32 + lane) / p.box)) & 1);
+        if (lane == 0) {
+          descs[slot] = u.d;
+          bar_arrive_tx(full + 8 * slot, __popc(good) * p.box * 128 * C::HALVES * 2);
+        }
+        __syncwarp();
+        if (ok && !failed) {
+          const uint32_t at = lane * p.box * 128;
+#pragma unroll
+          for (int hf = 0; hf < C::HALVES; ++hf) {
+            tma_box(kdst + hf * C::HALF_BYTES + at, &kmap, full + 8 * slot, hf * 64, u.row[0], u.d.h, u.id[0]);
+            tma_box(vdst + hf * C::HALF_BYTES + at, &vmap, full + 8 * slot, hf * 64, u.row[0], u.d.h, u.id[0]);
+          }
+        }
       } else {
-        // no query sees this token: zeros, whatever the page holds there.  A
-        // page outside the pool: NaN keys, so that the rows that see it say so.
-        const uint32_t f = off.x == -2 ? 0x7fff7fffu : 0u;
-        *reinterpret_cast<uint4*>(smem + slot * C::STAGE + at) = make_uint4(f, f, f, f);
-        *reinterpret_cast<uint4*>(smem + slot * C::STAGE + C::KV_BYTES + at) = make_uint4(0, 0, 0, 0);
+        int64_t ko[LU], vo[LU];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) u.d.bad[w] = 0;
+#pragma unroll
+        for (int x = 0; x < LU; ++x) {
+          const bool ok = u.state[x] == 1 && u.id[x] >= 0 && u.id[x] < p.num_pages;
+          u.d.bad[x] = __ballot_sync(0xffffffffu, u.state[x] != 0 && !ok);
+          ko[x] = !ok ? -1 : (int64_t)u.id[x] * p.k_page + (int64_t)u.d.h * p.k_head + (int64_t)u.row[x] * p.k_row;
+          vo[x] = !ok ? -1 : (int64_t)u.id[x] * p.v_page + (int64_t)u.d.h * p.v_head + (int64_t)u.row[x] * p.v_row;
+        }
+        if (lane == 0) descs[slot] = u.d;
+        constexpr int RPI = 32 / C::PIECES;   // rows per step
+        const int c = lane % C::PIECES, sub = lane / C::PIECES;
+#pragma unroll
+        for (int x = 0; x < LU; ++x)
+#pragma unroll 4
+          for (int r0 = 0; r0 < 32; r0 += RPI) {
+            const int64_t k_at = __shfl_sync(0xffffffffu, ko[x], r0 + sub), v_at = __shfl_sync(0xffffffffu, vo[x], r0 + sub);
+            const int r = x * 32 + r0 + sub;
+            const uint32_t at = (c >> 3) * C::HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+            if (k_at >= 0) {
+              cp_async16(kdst + at, p.k + k_at + c * 8);
+              cp_async16(vdst + at, p.v + v_at + c * 8);
+            }
+          }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(full + 8 * slot) : "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(full + 8 * slot);
       }
     }
-  };
-
-  {
-    Lookup u[S];
-#pragma unroll
-    for (int s = 0; s < S; ++s) u[s] = look();
-#pragma unroll
-    for (int s = 0; s < S; ++s) finish(u[s], s, s);
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) {
-      if (s < count) issue(s);
-      cp_async_commit();
-    }
+    // consumers wait for every tile; after a wait that ran out, see the copies in flight off
+    if (failed)
+      for (int i = max(0, count - S); i < count; ++i) bar_wait_long(full + 8 * (i % S), (i / S) & 1);
+    return;
   }
 
-  // ---- compute state
+  // -------------------------------------------------------------- consumers
+  const int64_t ctas = s_start[2];
   uint32_t qf[MT <= 2 ? MT : 1][D / 16][4];   // query fragments (MT = 4 reads them from shared memory)
   float o[MT][C::DT][4];
   float m[MT][2], l[MT][2];
   int back[MT][2];                            // T - t of the thread's rows: position = len - back
+  // Fragment addresses: 128-byte rows, 16-byte piece c of row r at c ^ (r & 7); the rows of a thread's
+  // ldmatrix lanes all have r & 7 = lane & 7.
+  const uint32_t swz = (lane & 7) << 4;
+  const uint32_t k_row = (warp * (TILE / kWarps) + ((lane >> 4) << 3) + (lane & 7)) * 128, k_col = ((lane >> 3) & 1) << 4;
+  const uint32_t v_at = (lane & 15) * 128 + ((warp * C::DW) >> 6) * C::HALF_BYTES;
+  const uint32_t v_col = ((warp * C::DW) & 63) * 2 + ((lane >> 4) << 4);
+  const uint32_t a_row = lane & 15, a_col = (lane >> 4) << 4;   // Q and P operands
 
-  const int64_t part_rows = ROWS;
   for (int i = 0; i < count; ++i) {
-    cp_async_wait<S - 2>();
-    __syncthreads();
     const int slot = i % S;
-    if (i + S - 1 < count) issue((i + S - 1) % S);
-    cp_async_commit();
-    const Lookup ahead = look();
-    const Desc d = descs[i & (C::DESCS - 1)];
+    bar_wait(full + 8 * slot, (i / S) & 1, failed);
+    const Desc& ds = descs[slot];
+    const int len = ds.len, token0 = ds.token0, rt = ds.rt;
 
-    if (d.first) {
+    if (ds.first) {
       // query rows of this segment: row r = t * G + g
-      for (int x = tid; x < ROWS * C::PIECES; x += kThreads) {
+      for (int x = tid; x < ROWS * C::PIECES; x += kConsumers) {
         const int r = x / C::PIECES, c = x % C::PIECES;
-        const int R = d.rt * ROWS + r;
+        const int R = rt * ROWS + r;
         uint4 w = make_uint4(0, 0, 0, 0);
         if (R < p.R) {
           const int t = R / p.G, g = R - t * p.G;
-          w = *reinterpret_cast<const uint4*>(p.q + (int64_t)d.b * p.q_b + (int64_t)(d.h * p.G + g) * p.q_h +
+          w = *reinterpret_cast<const uint4*>(p.q + (int64_t)ds.b * p.q_b + (int64_t)(ds.h * p.G + g) * p.q_h +
                                               (int64_t)t * p.q_t + c * 8);
         }
-        *reinterpret_cast<uint4*>(smem + C::OFF_Q + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4)) = w;
+        *reinterpret_cast<uint4*>(smem + C::OFF_Q + r * D * 2 + ((c ^ (r & 7)) << 4)) = w;
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int R = d.rt * ROWS + mt * 16 + e * 8 + lane / 4;
+          const int R = rt * ROWS + mt * 16 + e * 8 + lane / 4;
           back[mt][e] = p.T - min(R, p.R - 1) / p.G;
           m[mt][e] = -INFINITY;
           l[mt][e] = 0.f;
@@ -361,16 +451,14 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
       }
-      __syncthreads();
+      consumer_sync();
       if constexpr (MT <= 2) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const int r = mt * 16 + (lane & 15), c = kk * 2 + (lane >> 4);
-            ldsm_x4(sbase + C::OFF_Q + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4), qf[mt][kk][0], qf[mt][kk][1],
-                    qf[mt][kk][2], qf[mt][kk][3]);
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            ldsm_x4(sbase + C::OFF_Q + (mt * 16 + a_row) * D * 2 + ((kk * 32 + a_col) ^ swz), qf[mt][kk][0],
+                    qf[mt][kk][1], qf[mt][kk][2], qf[mt][kk][3]);
       }
     }
 
@@ -387,12 +475,9 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
     for (int kk = 0; kk < D / 16; ++kk) {
       uint32_t bf[C::NT][2];
 #pragma unroll
-      for (int n2 = 0; n2 < C::NT / 2; ++n2) {
-        const int r = warp * (TILE / kWarps) + n2 * 16 + ((lane >> 4) << 3) + (lane & 7);
-        const int c = kk * 2 + ((lane >> 3) & 1);
-        ldsm_x4(kb + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4), bf[2 * n2][0], bf[2 * n2][1], bf[2 * n2 + 1][0],
-                bf[2 * n2 + 1][1]);
-      }
+      for (int n2 = 0; n2 < C::NT / 2; ++n2)
+        ldsm_x4(kb + k_row + n2 * 2048 + (kk >> 2) * C::HALF_BYTES + (((kk & 3) * 32 + k_col) ^ swz), bf[2 * n2][0],
+                bf[2 * n2][1], bf[2 * n2 + 1][0], bf[2 * n2 + 1][1]);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint32_t a[4];
@@ -400,17 +485,18 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[e] = qf[mt][kk][e];
         } else {
-          const int r = mt * 16 + (lane & 15), c = kk * 2 + (lane >> 4);
-          ldsm_x4(sbase + C::OFF_Q + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4), a[0], a[1], a[2], a[3]);
+          ldsm_x4(sbase + C::OFF_Q + (mt * 16 + a_row) * D * 2 + ((kk * 32 + a_col) ^ swz), a[0], a[1], a[2], a[3]);
         }
 #pragma unroll
         for (int n = 0; n < C::NT; ++n) mma_e<HALF>(s[mt][n], a[0], a[1], a[2], a[3], bf[n][0], bf[n][1]);
       }
     }
-    const int tok = d.token0 + warp * (TILE / kWarps) + (lane & 3) * 2;   // token of n-tile 0, element 0
+    const int in_tile = warp * (TILE / kWarps) + (lane & 3) * 2;   // token of n-tile 0, element 0
+    const int tok = token0 + in_tile;
     // every row sees every token of the tile: positions run from len - T to len - 1
-    const bool full = d.token0 + TILE <= d.len - p.T + 1 &&
-                      (p.window == 0 || d.token0 > d.len - 1 - p.window || d.token0 + TILE <= p.sinks);
+    const bool full_tile = token0 + TILE <= len - p.T + 1 &&
+                           (p.window == 0 || token0 > len - 1 - p.window || token0 + TILE <= p.sinks) &&
+                           (ds.bad[0] | ds.bad[1] | ds.bad[2] | ds.bad[3]) == 0;
     float mx[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -420,10 +506,11 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x = s[mt][n][e] * p.scale2;
-          if (!full) {
-            const int j = tok + n * 8 + (e & 1), pos = d.len - back[mt][e >> 1];
+          if (!full_tile) {
+            const int at = in_tile + n * 8 + (e & 1), j = token0 + at, pos = len - back[mt][e >> 1];
             const bool seen = j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks);
-            x = seen ? x : -INFINITY;
+            // a page outside the pool: the rows that see it say so
+            x = !seen ? -INFINITY : (ds.bad[at >> 5] >> (at & 31)) & 1 ? NAN : x;
           }
           s[mt][n][e] = x;
           mx[mt][e >> 1] = fmaxf(mx[mt][e >> 1], x);
@@ -440,16 +527,27 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int R = d.rt * ROWS + mt * 16 + e * 8 + lane / 4;
+          const int R = rt * ROWS + mt * 16 + e * 8 + lane / 4;
           if (R < p.R) {
-            float* dst = p.scores + ((int64_t)(d.b * p.HKV + d.h) * p.R + R) * p.score_stride + tok;
+            float* dst = p.scores + ((int64_t)(ds.b * p.HKV + ds.h) * p.R + R) * p.score_stride + tok;
 #pragma unroll
             for (int n = 0; n < C::NT; ++n)
               *reinterpret_cast<float2*>(dst + n * 8) = make_float2(s[mt][n][2 * e], s[mt][n][2 * e + 1]);
           }
         }
     }
-    __syncthreads();
+    if (!full_tile) {
+      // rows of V that no query sees hold whatever the page or an earlier
+      // tile left there, and 0 * NaN is NaN: zero them
+      const int lo = p.window > 0 ? max(0, max(len - p.T, 0) - p.window + 1) : 0;
+      for (int x = tid; x < TILE * C::PIECES; x += kConsumers) {
+        const int r = x / C::PIECES, c = x % C::PIECES, j = token0 + r;
+        if (j < len && (j >= lo || j < p.sinks) && !((ds.bad[r >> 5] >> (r & 31)) & 1)) continue;
+        *reinterpret_cast<uint4*>(smem + slot * C::STAGE + C::KV_BYTES + (c >> 3) * C::HALF_BYTES + r * 128 +
+                                  ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    consumer_sync();
 
     // ---- running maximum and sum; P to shared memory.  The tensor cores
     // take it in the pages' type: as the rounded value and the rounded rest,
@@ -485,41 +583,46 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
           o[mt][n][2 * e + 1] *= alpha;
         }
       }
-    __syncthreads();
+    consumer_sync();
 
     // A token that some rows see and others do not has weight 0 in the
     // others, and 0 * inf is NaN in the product below.  Such tokens exist for
     // T > 1 only, T - 1 of them at either end of the span.  When one of them
     // holds an infinity or NaN, they are added by hand to the rows that see
     // them and then zeroed.
-    if (p.T > 1 && !full) {
-      const int lo = p.window > 0 ? max(0, max(d.len - p.T, 0) - p.window + 1) : 0;
+    if (p.T > 1 && !full_tile) {
+      const int lo = p.window > 0 ? max(0, max(len - p.T, 0) - p.window + 1) : 0;
       const int n_part = (p.window > 0 ? 2 : 1) * (p.T - 1);
       // the n-th such token's row in the tile, or -1
       auto part_row = [&](int n) {
-        const int j = n < p.T - 1 ? d.len - 1 - n : lo + n - (p.T - 1);
-        return j >= 0 && j < d.len && j >= d.token0 && j < d.token0 + TILE ? j - d.token0 : -1;
+        const int j = n < p.T - 1 ? len - 1 - n : lo + n - (p.T - 1);
+        return j >= 0 && j < len && j >= token0 && j < token0 + TILE ? j - token0 : -1;
       };
       uint8_t* vs = smem + slot * C::STAGE + C::KV_BYTES;
       int odd = 0;
-      for (int x = tid; x < n_part * C::PIECES; x += kThreads) {
-        const int r = part_row(x / C::PIECES);
+      for (int x = tid; x < n_part * C::PIECES; x += kConsumers) {
+        const int r = part_row(x / C::PIECES), c = x % C::PIECES;
         if (r < 0) continue;
-        const uint4 w = *reinterpret_cast<const uint4*>(vs + r * C::ROW_BYTES + (x % C::PIECES << 4));
+        const uint4 w = *reinterpret_cast<const uint4*>(vs + (c >> 3) * C::HALF_BYTES + r * 128 + ((c & 7) << 4));
         const uint32_t ones = HALF ? 0x7c00u : 0x7f80u;
         const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int y = 0; y < 4; ++y) odd |= (ws[y] & ones) == ones || ((ws[y] >> 16) & ones) == ones;
       }
-      if (__syncthreads_or(odd)) {
+      int any;
+      asm volatile("{\n.reg .pred a, b;\nsetp.ne.s32 a, %1, 0;\nbar.red.or.pred b, 1, 128, a;\nselp.s32 %0, 1, 0, b;\n}\n"
+                   : "=r"(any)
+                   : "r"(odd)
+                   : "memory");
+      if (any) {
         for (int n = 0; n < n_part; ++n) {
-          const int r = part_row(n), j = d.token0 + r;
-          if (r < 0 || (n >= p.T - 1 && j > d.len - p.T)) continue;   // both ends may name it: once
+          const int r = part_row(n), j = token0 + r;
+          if (r < 0 || (n >= p.T - 1 && j > len - p.T)) continue;   // both ends may name it: once
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int pos = d.len - back[mt][e], row = mt * 16 + e * 8 + lane / 4;
+              const int pos = len - back[mt][e], row = mt * 16 + e * 8 + lane / 4;
               if (!(j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks))) continue;
               const uint8_t* pw = smem + C::OFF_P + row * TILE * 2 + (((r >> 3) ^ (row & 7)) << 4) + (r & 7) * 2;
               const float w = to_float<HALF>(*reinterpret_cast<const uint16_t*>(pw)) +
@@ -528,19 +631,19 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
               for (int x = 0; x < C::DT; ++x) {
                 const int col = warp * C::DW + x * 8 + (lane & 3) * 2;
                 const uint32_t vv = *reinterpret_cast<const uint32_t*>(
-                    vs + r * C::ROW_BYTES + (((col >> 3) ^ (r & 7)) << 4) + (col & 7) * 2);
+                    vs + (col >> 6) * C::HALF_BYTES + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4) + (col & 7) * 2);
                 o[mt][x][2 * e] += w * to_float<HALF>((uint16_t)vv);
                 o[mt][x][2 * e + 1] += w * to_float<HALF>((uint16_t)(vv >> 16));
               }
             }
         }
-        __syncthreads();
-        for (int x = tid; x < n_part * C::PIECES; x += kThreads) {
-          const int r = part_row(x / C::PIECES);
+        consumer_sync();
+        for (int x = tid; x < n_part * C::PIECES; x += kConsumers) {
+          const int r = part_row(x / C::PIECES), c = x % C::PIECES;
           if (r >= 0)
-            *reinterpret_cast<uint4*>(vs + r * C::ROW_BYTES + (x % C::PIECES << 4)) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(vs + (c >> 3) * C::HALF_BYTES + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
         }
-        __syncthreads();
+        consumer_sync();
       }
     }
 
@@ -549,16 +652,12 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
     for (int kk = 0; kk < TILE / 16; ++kk) {
       uint32_t bf[C::DT][2];
 #pragma unroll
-      for (int n2 = 0; n2 < C::DT / 2; ++n2) {
-        const int r = kk * 16 + (lane & 15);
-        const int c = warp * (C::DW / 8) + n2 * 2 + (lane >> 4);
-        ldsm_x4_trans(vb + r * C::ROW_BYTES + ((c ^ (r & 7)) << 4), bf[2 * n2][0], bf[2 * n2][1], bf[2 * n2 + 1][0],
-                      bf[2 * n2 + 1][1]);
-      }
+      for (int n2 = 0; n2 < C::DT / 2; ++n2)
+        ldsm_x4_trans(vb + v_at + kk * 2048 + ((n2 * 32 + v_col) ^ swz), bf[2 * n2][0], bf[2 * n2][1],
+                      bf[2 * n2 + 1][0], bf[2 * n2 + 1][1]);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const int r = mt * 16 + (lane & 15), c = kk * 2 + (lane >> 4);
-        const uint32_t at = sbase + C::OFF_P + r * TILE * 2 + ((c ^ (r & 7)) << 4);
+        const uint32_t at = sbase + C::OFF_P + (mt * 16 + a_row) * TILE * 2 + ((kk * 32 + a_col) ^ swz);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
           uint32_t a[4];
@@ -569,27 +668,33 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
       }
     }
 
-    if (d.last) {
+    const bool last = ds.last;
+    const int sb = ds.b, sh = ds.h, n_tiles = ds.n_tiles;
+    const int64_t seg_start = ds.seg_start;
+    // the tile is read: hand it back (zeroed rows are ordinary stores, which the TMA must not overtake)
+    if (!full_tile) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    __syncwarp();
+    if (lane == 0) bar_arrive(empty + 8 * slot);
+
+    if (last) {
       // ---- the rows' sums over the four warps
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = l[mt][e];
+          float x = failed ? NAN : l[mt][e];
           x += __shfl_xor_sync(0xffffffffu, x, 1);
           x += __shfl_xor_sync(0xffffffffu, x, 2);
           if ((lane & 3) == 0) ssum[warp * ROWS + mt * 16 + e * 8 + lane / 4] = x;
         }
-      __syncthreads();
-      const int64_t at = g0 + i;                            // flat index of this tile
-      const bool begins = g0 <= d.seg_start;                // the segment's first tile is ours
-      const bool whole = begins && at == d.seg_start + d.n_tiles - 1;
-      const int64_t slot_o = (int64_t)blockIdx.x * 2 + (d.seg_start > g0 ? 1 : 0);
+      consumer_sync();
+      const bool whole = g0 <= seg_start && g0 + i == seg_start + n_tiles - 1;
+      const int64_t slot_o = (int64_t)blockIdx.x * 2 + (seg_start > g0 ? 1 : 0);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = mt * 16 + e * 8 + lane / 4, R = d.rt * ROWS + r;
+          const int r = mt * 16 + e * 8 + lane / 4, R = rt * ROWS + r;
           if (R >= p.R) continue;
           float sum = 0.f;
 #pragma unroll
@@ -598,7 +703,7 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
           if (whole) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const int t = R / p.G, g = R - t * p.G;
-            const int64_t row = ((int64_t)d.b * p.HQ + d.h * p.G + g) * p.T + t;
+            const int64_t row = ((int64_t)sb * p.HQ + sh * p.G + g) * p.T + t;
 #pragma unroll
             for (int n = 0; n < C::DT; ++n)
               *reinterpret_cast<uint32_t*>(p.out + row * D + col + n * 8) =
@@ -606,83 +711,125 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const __grid_consta
             if (warp == 0 && (lane & 3) == 0) {
               const float lse2 = sum == 0.f ? -INFINITY : finite_or_zero(m[mt][e]) + log2f(sum);
               if (p.lse) p.lse[row] = lse2 * 0.6931471805599453f;
-              if (p.row_lse2) p.row_lse2[(int64_t)(d.b * p.HKV + d.h) * p.R + R] = lse2;
+              if (p.row_lse2) p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + R] = lse2;
             }
           } else {
-            float* po = p.part_o + (slot_o * part_rows + r) * D + col;
+            float* po = p.part_o + (slot_o * ROWS + r) * D + col;
 #pragma unroll
             for (int n = 0; n < C::DT; ++n)
               *reinterpret_cast<float2*>(po + n * 8) = make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
             if (warp == 0 && (lane & 3) == 0)
-              *reinterpret_cast<float2*>(p.part_ml + (slot_o * part_rows + r) * 2) = make_float2(m[mt][e], sum);
+              *reinterpret_cast<float2*>(p.part_ml + (slot_o * ROWS + r) * 2) = make_float2(m[mt][e], sum);
           }
         }
       if (!whole) {
-        // ---- join: the last of the segment's CTAs to arrive adds the parts
-        // up in the order of the CTAs
-        const int64_t c0 = ((d.seg_start + 1) * ctas - 1) / total;
-        const int64_t c1 = ((d.seg_start + d.n_tiles) * ctas - 1) / total;
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          const int seen = atomicAdd(p.counters + c0, 1);
-          s_last = seen == (int)(c1 - c0);
-          if (s_last) p.counters[c0] = 0;
-        }
-        __syncthreads();
-        if (s_last) {
-          __threadfence();
-          const int n = (int)(c1 - c0) + 1;
-          // part k of the segment: CTA c0 + k; its second slot when it began with another segment
-          const int64_t first_slot = c0 * 2 + (total * c0 / ctas < d.seg_start ? 1 : 0);
-          auto slot_of = [&](int k) { return k == 0 ? first_slot : (c0 + k) * 2; };
-          for (int r = warp; r < ROWS; r += kWarps) {
-            if (d.rt * ROWS + r >= p.R) break;
-            float mm = -INFINITY;
-            for (int k = lane; k < n; k += 32) mm = fmaxf(mm, __ldcg(p.part_ml + (slot_of(k) * part_rows + r) * 2));
-#pragma unroll
-            for (int off = 16; off; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+        // ---- join.  The CTAs c0..c1 of the segment arrive in groups of
+        // kGroup; a group's last adds its parts up into the group's first
+        // part, the last group's last adds the groups up and writes the
+        // rows: two rounds of a few independent loads instead of one long
+        // chain.  The order of the sums is the CTAs', whoever does them.
+        const int64_t c0 = ((seg_start + 1) * ctas - 1) / total;
+        const int64_t c1 = ((seg_start + n_tiles) * ctas - 1) / total;
+        const int n = (int)(c1 - c0) + 1, groups = (n + kGroup - 1) / kGroup;
+        // part k of the segment: CTA c0 + k; CTA c0's second part when it began with another segment
+        const int64_t first_slot = c0 * 2 + (total * c0 / ctas < seg_start ? 1 : 0);
+        auto slot_of = [&](int k) { return k == 0 ? first_slot : (c0 + k) * 2; };
+        float* w_s = reinterpret_cast<float*>(smem + C::OFF_P);     // [ROWS][2][20]: maxima, then weights; sums
+        float* sum_s = ssum;                                       // [ROWS] sums, [ROWS] maxima behind them
+        const int n_rows = min(ROWS, p.R - rt * ROWS);
+        // parts k0, k0 + step, ... (cnt of them) -> final rows, or part k0
+        auto join = [&](int k0, int step, int cnt, bool final) {
+          for (int x = tid; x < n_rows * cnt; x += kConsumers) {
+            const int r = x / cnt, k = x - r * cnt;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot_of(k0 + k * step) * ROWS + r) * 2));
+            w_s[r * 40 + k] = ml.x;
+            w_s[r * 40 + 20 + k] = ml.y;
+          }
+          consumer_sync();
+          if (tid < n_rows) {
+            float mm = -INFINITY, sum = 0.f;
+            for (int k = 0; k < cnt; ++k) mm = fmaxf(mm, w_s[tid * 40 + k]);
             const float mu = finite_or_zero(mm);
-            float sum = 0.f;
-            for (int k = lane; k < n; k += 32) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot_of(k) * part_rows + r) * 2));
-              sum += ml.y * fast_exp2(ml.x - mu);
+            for (int k = 0; k < cnt; ++k) {
+              const float w = fast_exp2(w_s[tid * 40 + k] - mu);
+              sum += w * w_s[tid * 40 + 20 + k];
+              w_s[tid * 40 + k] = w;
+            }
+            sum_s[tid] = sum;
+            sum_s[ROWS + tid] = mm;
+          }
+          consumer_sync();
+          // a warp owns D/4 columns, 4 to a lane; its lanes' quarters (eighths) take every 4th (8th) part
+          constexpr int LC = C::DW / 4, LP = 32 / LC;   // lanes across the columns, parts side by side
+          const int col = warp * C::DW + (lane % LC) * 4, kp = lane / LC;
+#pragma unroll 2
+          for (int r = 0; r < n_rows; ++r) {
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 5
+            for (int k = kp; k < cnt; k += LP) {
+              const float w = w_s[r * 40 + k];
+              const float4 f =
+                  __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot_of(k0 + k * step) * ROWS + r) * D + col));
+              acc.x += w * f.x; acc.y += w * f.y; acc.z += w * f.z; acc.w += w * f.w;
             }
 #pragma unroll
-            for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            float acc[D / 32];
-#pragma unroll
-            for (int x = 0; x < D / 32; ++x) acc[x] = 0.f;
-#pragma unroll 8
-            for (int k = 0; k < n; ++k) {
-              const float w = fast_exp2(__ldcg(p.part_ml + (slot_of(k) * part_rows + r) * 2) - mu);
-              const float* src = p.part_o + (slot_of(k) * part_rows + r) * D + lane * (D / 32);
-              if constexpr (D == 128) {
-                const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
-                acc[0] += w * f.x; acc[1] += w * f.y; acc[2] += w * f.z; acc[3] += w * f.w;
-              } else {
-                const float2 f = __ldcg(reinterpret_cast<const float2*>(src));
-                acc[0] += w * f.x; acc[1] += w * f.y;
-              }
+            for (int off = LC; off < 32; off <<= 1) {
+              acc.x += __shfl_xor_sync(0xffffffffu, acc.x, off);
+              acc.y += __shfl_xor_sync(0xffffffffu, acc.y, off);
+              acc.z += __shfl_xor_sync(0xffffffffu, acc.z, off);
+              acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
+            }
+            const float sum = sum_s[r], mm = sum_s[ROWS + r];
+            if (kp != 0) continue;
+            if (!final) {
+              // (these columns of part k0 were read by this lane alone)
+              *reinterpret_cast<float4*>(p.part_o + (slot_of(k0) * ROWS + r) * D + col) = acc;
+              if (warp == 0 && lane == 0)
+                *reinterpret_cast<float2*>(p.part_ml + (slot_of(k0) * ROWS + r) * 2) = make_float2(mm, sum);
+              continue;
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            const int R = d.rt * ROWS + r, t = R / p.G, g = R - t * p.G;
-            const int64_t row = ((int64_t)d.b * p.HQ + d.h * p.G + g) * p.T + t;
-            uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * D + lane * (D / 32));
-#pragma unroll
-            for (int x = 0; x < D / 64; ++x) dst[x] = pack2<HALF>(acc[2 * x] * inv, acc[2 * x + 1] * inv);
-            if (lane == 0) {
-              const float lse2 = sum == 0.f ? -INFINITY : mu + log2f(sum);
+            const int R = rt * ROWS + r, t = R / p.G, g = R - t * p.G;
+            const int64_t row = ((int64_t)sb * p.HQ + sh * p.G + g) * p.T + t;
+            *reinterpret_cast<uint2*>(p.out + row * D + col) =
+                make_uint2(pack2<HALF>(acc.x * inv, acc.y * inv), pack2<HALF>(acc.z * inv, acc.w * inv));
+            if (warp == 0 && lane == 0) {
+              const float lse2 = sum == 0.f ? -INFINITY : finite_or_zero(mm) + log2f(sum);
               if (p.lse) p.lse[row] = lse2 * 0.6931471805599453f;
-              if (p.row_lse2) p.row_lse2[(int64_t)(d.b * p.HKV + d.h) * p.R + R] = lse2;
+              if (p.row_lse2) p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + R] = lse2;
             }
           }
+          consumer_sync();
+        };
+        // arrive at a counter that `of` CTAs share; true for the last one, which zeroes it
+        auto arrive = [&](int* counter, int of) {
+          __threadfence();
+          consumer_sync();
+          if (tid == 0) {
+            const int is_last = atomicAdd(counter, 1) == of - 1;
+            if (is_last) *counter = 0;
+            *s_last = is_last;
+          }
+          consumer_sync();
+          const bool is_last = *s_last != 0;
+          if (is_last) __threadfence();
+          return is_last;
+        };
+        const int grp = (int)(blockIdx.x - c0) / kGroup;
+        const int in_group = min(kGroup, n - grp * kGroup);
+        // (a group of one needs no counter; its CTA may begin the next segment, whose first group counts there)
+        if (in_group == 1 || arrive(p.counters + p.ctas + c0 + grp * kGroup, in_group)) {
+          if (groups == 1) {
+            join(0, 1, n, true);
+          } else {
+            if (in_group > 1) join(grp * kGroup, 1, in_group, false);
+            if (arrive(p.counters + c0, groups)) join(0, kGroup, groups, true);
+          }
         }
+        consumer_sync();   // s_last, the statistics and P are free again
       }
     }
-    finish(ahead, slot, (i + S) & (C::DESCS - 1));
   }
-  cp_async_wait<0>();
 }
 
 // token_weights[b, j] += sum over the heads and new tokens of 2^(x - lse2).
@@ -781,7 +928,8 @@ static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
   p.mt = R <= 16 ? 1 : R <= 32 ? 2 : 4;
   p.row_tiles = (p.R + 16 * p.mt - 1) / (16 * p.mt);
   const int64_t tiles = std::max<int64_t>(1, (cap + tile - 1) / tile) * a->batch * a->kv_heads * p.row_tiles;
-  p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, 2 * num_sms_of(a->num_sms)));
+  // two CTAs per SM; a join takes kGroup^2 parts and some
+  p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, std::min(2 * num_sms_of(a->num_sms), kGroup * 20)));
   p.score_stride = std::max<int64_t>(128, (cap + 127) / 128 * 128);
   const size_t rows = (size_t)16 * p.mt * 2 * p.ctas;
   p.part_o = rows * a->head_dim * sizeof(float);
@@ -793,10 +941,52 @@ static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
   return KVR_OK;
 }
 
-template <bool HALF, int D, int MT>
-static int launch(const Params& p, cudaStream_t s) {
+// Tensor maps of the pages: [page number][head][row][element] with the
+// caller's strides, boxes of `box` rows x 64 elements, 128-byte swizzle.
+// False where the pages do not fit one (an axis with stride 0, say).
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+static bool page_map(CUtensorMap* map, const void* base, bool half, int D, int page, int heads, int pages,
+                     int64_t row_stride, int64_t head_stride, int64_t page_stride, int box) {
+  EncodeFn fn = encode_fn();
+  if (!fn || pages <= 0) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)heads, (cuuint64_t)pages};
+  const int64_t given[3] = {row_stride, head_stride, page_stride};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) {
+    // an axis of one element is never stepped along: any valid stride does
+    strides[i] = 2 * (cuuint64_t)(dims[i + 1] == 1 ? D : given[i]);
+    if (dims[i + 1] > 1 && given[i] <= 0) return false;
+    if (strides[i] >= (1ull << 40)) return false;
+  }
+  const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
+  return fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base),
+            dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Maps {
+  CUtensorMap k, v;
+};
+
+template <bool HALF, int D, int MT, bool TMA>
+static int launch(const Params& p, const Maps& maps, cudaStream_t s) {
   using C = Cfg<D, MT>;
-  auto kern = attention_kernel<HALF, D, MT>;
+  auto kern = attention_kernel<HALF, D, MT, TMA>;
   static bool ready[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
@@ -806,16 +996,20 @@ static int launch(const Params& p, cudaStream_t s) {
     if (e != cudaSuccess) { set_last_cuda_error(e); return KVR_ERR_CUDA; }
     ready[dev & 63] = true;
   }
-  cudaError_t e = pdl_launch(kern, dim3(p.ctas), dim3(kThreads), C::SMEM, s, 1, p);
+  cudaError_t e = pdl_launch(kern, dim3(p.ctas), dim3(kThreads), C::SMEM, s, 1, p, maps.k, maps.v);
   if (e != cudaSuccess) { set_last_cuda_error(e); return KVR_ERR_CUDA; }
   return KVR_OK;
 }
 
+template <bool HALF, int D, bool TMA>
+static int launch_mt(int mt, const Params& p, const Maps& maps, cudaStream_t s) {
+  if (mt == 1) return launch<HALF, D, 1, TMA>(p, maps, s);
+  if (mt == 2) return launch<HALF, D, 2, TMA>(p, maps, s);
+  return launch<HALF, D, 4, TMA>(p, maps, s);
+}
 template <bool HALF, int D>
-static int launch_mt(int mt, const Params& p, cudaStream_t s) {
-  if (mt == 1) return launch<HALF, D, 1>(p, s);
-  if (mt == 2) return launch<HALF, D, 2>(p, s);
-  return launch<HALF, D, 4>(p, s);
+static int launch_tma(bool tma, int mt, const Params& p, const Maps& maps, cudaStream_t s) {
+  return tma ? launch_mt<HALF, D, true>(mt, p, maps, s) : launch_mt<HALF, D, false>(mt, p, maps, s);
 }
 
 }  // namespace paged
@@ -829,7 +1023,7 @@ extern "C" int kvr_paged_attention_plan(const kvr_paged_attention_args* a, size_
   const int st = paged::plan_of(a, &p);
   if (st != KVR_OK) return st;
   if (workspace_bytes) *workspace_bytes = p.part_o + p.part_ml;
-  if (counter_count) *counter_count = (size_t)p.ctas;
+  if (counter_count) *counter_count = 2 * (size_t)p.ctas;
   if (scores_bytes) *scores_bytes = p.lse2 + p.scores;
   return KVR_OK;
 }
@@ -878,8 +1072,23 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   p.counters = a->counters;
   cudaStream_t s = as_stream(stream);
   const bool half = a->dtype == 1;
-  if (a->head_dim == 64) st = half ? paged::launch_mt<true, 64>(pl.mt, p, s) : paged::launch_mt<false, 64>(pl.mt, p, s);
-  else st = half ? paged::launch_mt<true, 128>(pl.mt, p, s) : paged::launch_mt<false, 128>(pl.mt, p, s);
+  // TMA boxes: the largest number of tokens that divides both a page and a
+  // tile; below 8 rows (one swizzle pattern) the rows are copied one by one.
+  const int tile = a->head_dim == 64 ? 128 : 64;
+  int box = tile;
+  while (a->page_size % box) box /= 2;
+  p.box = box;
+  paged::Maps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  const bool tma = box >= 8 &&
+                   paged::page_map(&maps.k, a->key_pages, half, a->head_dim, a->page_size, a->kv_heads, a->num_pages,
+                                   a->key_row_stride, a->key_head_stride, a->key_page_stride, box) &&
+                   paged::page_map(&maps.v, a->value_pages, half, a->head_dim, a->page_size, a->kv_heads, a->num_pages,
+                                   a->value_row_stride, a->value_head_stride, a->value_page_stride, box);
+  if (a->head_dim == 64)
+    st = half ? paged::launch_tma<true, 64>(tma, pl.mt, p, maps, s) : paged::launch_tma<false, 64>(tma, pl.mt, p, maps, s);
+  else
+    st = half ? paged::launch_tma<true, 128>(tma, pl.mt, p, maps, s) : paged::launch_tma<false, 128>(tma, pl.mt, p, maps, s);
   if (st != KVR_OK || !a->token_weights || pl.cap == 0) return st;
   const int rows = p.HKV * p.R;
   const dim3 grid((pl.cap + 255) / 256, p.B);
