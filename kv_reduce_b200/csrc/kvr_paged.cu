@@ -39,7 +39,7 @@ constexpr int kWarps = 4;                     // consumers
 constexpr int kConsumers = 32 * kWarps;
 constexpr int kThreads = kConsumers + 32;     // and the producer warp
 constexpr int kGroup = 16;                    // CTAs a join takes at a time
-constexpr long long kWaitLimitNs = 2000000000ll;
+constexpr long long kWaitClocks = 2000000000ll;   // about a second
 
 // Rows that no mask leaves anything to keep m = -inf; 0 stands in for it
 // wherever it would be subtracted.
@@ -73,7 +73,7 @@ __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r
 }
 
 // ---- mbarriers.  A wait that runs out (which no input causes) is given up
-// after kWaitLimitNs: every later wait of the thread returns at once, the
+// after kWaitClocks: every later wait of the thread returns at once, the
 // loops end, and the outputs are NaN.
 __device__ __forceinline__ void bar_init(uint32_t bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
@@ -93,14 +93,9 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, int parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ long long now_ns() {
-  long long t;
-  asm volatile("mov.u64 %0, %globaltimer;\n" : "=l"(t));
-  return t;
-}
 __device__ __noinline__ bool bar_wait_long(uint32_t bar, int parity) {
-  const long long begin = now_ns();
-  while (now_ns() - begin < kWaitLimitNs)
+  const long long begin = clock64();
+  while (clock64() - begin < kWaitClocks)
     for (int i = 0; i < 64; ++i)
       if (bar_try(bar, parity)) return true;
   return false;
@@ -140,8 +135,8 @@ struct Params {
   int B, HQ, HKV, T, G, R, row_tiles, window, sinks, cap;
   float scale2;     // scale * log2(e)
   int ctas, min_tiles;
-  float* part_o;    // [2 * ctas][ROWS][D]
-  float* part_ml;   // [2 * ctas][ROWS][2]
+  float* part_o;    // [3 * ctas][ROWS][D]: two parts of each CTA, group sums
+  float* part_ml;   // [3 * ctas][ROWS][2]
   int* counters;    // [2 * ctas], zero on entry and on exit
   int box;          // tokens of a TMA box
 };
@@ -165,19 +160,27 @@ struct Cfg {
   static constexpr int OFF_Q = STAGES * STAGE;
   static constexpr int OFF_P = MT <= 2 ? OFF_Q : OFF_Q + Q_BYTES;
   static constexpr int OFF_DESC = OFF_Q + (MT <= 2 ? (Q_BYTES > P_BYTES ? Q_BYTES : P_BYTES) : Q_BYTES + P_BYTES);
-  static constexpr int OFF_MAX = OFF_DESC + STAGES * 80;
+  static constexpr int OFF_MAX = OFF_DESC + STAGES * 64;
   static constexpr int OFF_SUM = OFF_MAX + kWarps * ROWS * 4;
   static constexpr int OFF_BAR = OFF_SUM + kWarps * ROWS * 4;
-  static constexpr int OFF_MISC = OFF_BAR + 2 * STAGES * 8 + 16;
-  static constexpr int SMEM = OFF_MISC + 96 + 1024;   // 1 KB to align the ring
+  static constexpr int OFF_MISC = OFF_BAR + 3 * STAGES * 8;
+  static constexpr int SMEM = OFF_MISC + 64 + 1024;   // 1 KB to align the ring
 };
 
 struct Desc {
   int b, h, rt, token0, len, first, last, n_tiles;
-  int64_t seg_start;
+  int seg_start;
   uint32_t bad[4];   // tokens on pages outside the pool, a bit each
 };
-static_assert(sizeof(Desc) <= 80, "");
+static_assert(sizeof(Desc) <= 64, "");
+
+// `total` tiles cut into `n` ranges of equal size, the first ones a tile longer.
+struct Cut {
+  int q, r;
+  __device__ __forceinline__ Cut(int total, int n) : q(total / n), r(total % n) {}
+  __device__ __forceinline__ int begin(int c) const { return c * q + min(c, r); }
+  __device__ __forceinline__ int owner(int g) const { return g < r * (q + 1) ? g / (q + 1) : r + (g - r * (q + 1)) / q; }
+};
 
 // The tiles a sequence's queries look at: with a window, `ns` tiles that hold
 // the sinks, then the tiles from `lo_tile` on.
@@ -210,15 +213,17 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
   Desc* descs = reinterpret_cast<Desc*>(smem + C::OFF_DESC);
   float* smax = reinterpret_cast<float*>(smem + C::OFF_MAX);
   float* ssum = reinterpret_cast<float*>(smem + C::OFF_SUM);
-  const uint32_t full = sbase + C::OFF_BAR, empty = full + S * 8;
-  int64_t* s_start = reinterpret_cast<int64_t*>(smem + C::OFF_MISC);   // [3]
-  int64_t* s_scan = s_start + 3;                                       // [kThreads / 32]
-  int* s_last = reinterpret_cast<int*>(s_scan + kThreads / 32);
+  // a slot's data is there / is read / its descriptor is there (before the data)
+  const uint32_t full = sbase + C::OFF_BAR, empty = full + S * 8, ready = empty + S * 8;
+  int* s_start = reinterpret_cast<int*>(smem + C::OFF_MISC);   // [3]
+  int* s_scan = s_start + 4;                                   // [kThreads / 32]
+  int* s_last = s_scan + kThreads / 32;
 
   if (tid == 0) {
     for (int i = 0; i < S; ++i) {
       bar_init(full + 8 * i, TMA ? 1 : 33);
       bar_init(empty + 8 * i, kWarps);
+      bar_init(ready + 8 * i, 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
@@ -226,63 +231,63 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
 
   // ---- this CTA's range of the flat tile list
   const int HR = p.HKV * p.row_tiles;
-  int64_t total, g0, g1;
+  int total, ctas, g0, count;   // tiles in all, CTAs that take part, this one's first tile and how many
   {
     const int per = (p.B + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
-    int64_t mine = 0;
+    int mine = 0;
     for (int b = b0; b < b1; ++b) mine += span_of<TILE>(p, length_of(p, b)).n;
-    int64_t incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += x;
     }
     if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
-    int64_t base = 0;
+    int before = incl - mine;
     total = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) base += s_scan[w];
+      if (w < warp) before += s_scan[w];
       total += s_scan[w];
     }
     total *= HR;
-    const int64_t want = max((int64_t)1, total / p.min_tiles);
-    const int64_t n = min((int64_t)p.ctas, want);
-    if ((int64_t)blockIdx.x >= n) return;
-    g0 = total * blockIdx.x / n;
-    g1 = total * (blockIdx.x + 1) / n;
+    ctas = min(p.ctas, max(1, total / p.min_tiles));
+    const int me = blockIdx.x;
+    if (me >= ctas) return;
+    const Cut cut(total, ctas);
+    g0 = cut.begin(me);
+    count = cut.begin(me + 1) - g0;
     // the thread whose sequences hold tile g0 finds the sequence
-    int64_t before = base + incl - mine;
     if (mine > 0 && before * HR <= g0 && g0 < (before + mine) * HR) {
       int b = b0;
-      for (;; ++b) {
-        const int64_t nb = span_of<TILE>(p, length_of(p, b)).n;
-        if (g0 < (before + nb) * HR) break;
-        before += nb;
-      }
+      if (per > 1)
+        for (;; ++b) {
+          const int nb = span_of<TILE>(p, length_of(p, b)).n;
+          if (g0 < (before + nb) * HR) break;
+          before += nb;
+        }
       s_start[0] = b;
       s_start[1] = before;
-      s_start[2] = n;
+      s_start[2] = p.lengths[b];
     }
     __syncthreads();
   }
-  const int count = (int)(g1 - g0);
   bool failed = false;
 
   if (warp == kWarps) {
     // ------------------------------------------------------------ producer
-    int ld_b = (int)s_start[0], ld_left = count, ld_hr, ld_tile;
-    int ld_len = length_of(p, ld_b);
-    bool ld_over = p.lengths[ld_b] > p.cap;
+    int ld_b = s_start[0], ld_left = count, ld_hr, ld_tile;
+    int ld_len = min(max(s_start[2], 0), p.cap);
+    bool ld_over = s_start[2] > p.cap;
     Span ld_span = span_of<TILE>(p, ld_len);
-    int64_t ld_seg = s_start[1] * HR;
+    int ld_seg = s_start[1] * HR;
     {
-      const int64_t off = g0 - ld_seg;
-      ld_hr = (int)(off / ld_span.n);
-      ld_tile = (int)(off - (int64_t)ld_hr * ld_span.n);
-      ld_seg += (int64_t)ld_hr * ld_span.n;
+      const int off = g0 - ld_seg;
+      ld_hr = off / ld_span.n;
+      ld_tile = off - ld_hr * ld_span.n;
+      ld_seg += ld_hr * ld_span.n;
     }
     int next_raw = ld_b + 1 < p.B ? p.lengths[ld_b + 1] : 0;
     bool ld_first = true;
@@ -356,6 +361,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
             u.d.bad[w] = __ballot_sync(0xffffffffu, (bad >> ((w * 32 + lane) / p.box)) & 1);
         if (lane == 0) {
           descs[slot] = u.d;
+          bar_arrive(ready + 8 * slot);
           bar_arrive_tx(full + 8 * slot, __popc(good) * p.box * 128 * C::HALVES * 2);
         }
         __syncwarp();
@@ -378,7 +384,10 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
           ko[x] = !ok ? -1 : (int64_t)u.id[x] * p.k_page + (int64_t)u.d.h * p.k_head + (int64_t)u.row[x] * p.k_row;
           vo[x] = !ok ? -1 : (int64_t)u.id[x] * p.v_page + (int64_t)u.d.h * p.v_head + (int64_t)u.row[x] * p.v_row;
         }
-        if (lane == 0) descs[slot] = u.d;
+        if (lane == 0) {
+          descs[slot] = u.d;
+          bar_arrive(ready + 8 * slot);
+        }
         constexpr int RPI = 32 / C::PIECES;   // rows per step
         const int c = lane % C::PIECES, sub = lane / C::PIECES;
 #pragma unroll
@@ -405,7 +414,6 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
   }
 
   // -------------------------------------------------------------- consumers
-  const int64_t ctas = s_start[2];
   uint32_t qf[MT <= 2 ? MT : 1][D / 16][4];   // query fragments (MT = 4 reads them from shared memory)
   float o[MT][C::DT][4];
   float m[MT][2], l[MT][2];
@@ -420,12 +428,12 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
 
   for (int i = 0; i < count; ++i) {
     const int slot = i % S;
-    bar_wait(full + 8 * slot, (i / S) & 1, failed);
+    bar_wait(ready + 8 * slot, (i / S) & 1, failed);
     const Desc& ds = descs[slot];
     const int len = ds.len, token0 = ds.token0, rt = ds.rt;
 
     if (ds.first) {
-      // query rows of this segment: row r = t * G + g
+      // query rows of this segment, while its first tile is on the way: row r = t * G + g
       for (int x = tid; x < ROWS * C::PIECES; x += kConsumers) {
         const int r = x / C::PIECES, c = x % C::PIECES;
         const int R = rt * ROWS + r;
@@ -461,6 +469,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
                     qf[mt][kk][1], qf[mt][kk][2], qf[mt][kk][3]);
       }
     }
+
+    bar_wait(full + 8 * slot, (i / S) & 1, failed);
 
     // ---- scores: this warp's TILE/4 tokens x all rows
     const uint32_t kb = sbase + slot * C::STAGE, vb = kb + C::KV_BYTES;
@@ -670,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
 
     const bool last = ds.last;
     const int sb = ds.b, sh = ds.h, n_tiles = ds.n_tiles;
-    const int64_t seg_start = ds.seg_start;
+    const int seg_start = ds.seg_start;
     // the tile is read: hand it back (zeroed rows are ordinary stores, which the TMA must not overtake)
     if (!full_tile) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     __syncwarp();
@@ -689,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
         }
       consumer_sync();
       const bool whole = g0 <= seg_start && g0 + i == seg_start + n_tiles - 1;
-      const int64_t slot_o = (int64_t)blockIdx.x * 2 + (seg_start > g0 ? 1 : 0);
+      const int64_t slot_o = blockIdx.x * 2 + (seg_start > g0 ? 1 : 0);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -724,68 +734,60 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
         }
       if (!whole) {
         // ---- join.  The CTAs c0..c1 of the segment arrive in groups of
-        // kGroup; a group's last adds its parts up into the group's first
-        // part, the last group's last adds the groups up and writes the
-        // rows: two rounds of a few independent loads instead of one long
-        // chain.  The order of the sums is the CTAs', whoever does them.
-        const int64_t c0 = ((seg_start + 1) * ctas - 1) / total;
-        const int64_t c1 = ((seg_start + n_tiles) * ctas - 1) / total;
-        const int n = (int)(c1 - c0) + 1, groups = (n + kGroup - 1) / kGroup;
-        // part k of the segment: CTA c0 + k; CTA c0's second part when it began with another segment
-        const int64_t first_slot = c0 * 2 + (total * c0 / ctas < seg_start ? 1 : 0);
-        auto slot_of = [&](int k) { return k == 0 ? first_slot : (c0 + k) * 2; };
-        float* w_s = reinterpret_cast<float*>(smem + C::OFF_P);     // [ROWS][2][20]: maxima, then weights; sums
-        float* sum_s = ssum;                                       // [ROWS] sums, [ROWS] maxima behind them
+        // kGroup; a group's last adds its parts up, the last group's last
+        // adds the groups up and writes the rows: two rounds of a few
+        // independent loads instead of one long chain.  The order of the
+        // sums is the CTAs', whoever does them.
+        const Cut cut(total, ctas);
+        const int c0 = cut.owner(seg_start), c1 = cut.owner(seg_start + n_tiles - 1);
+        const int n = c1 - c0 + 1, groups = (n + kGroup - 1) / kGroup;
         const int n_rows = min(ROWS, p.R - rt * ROWS);
-        // parts k0, k0 + step, ... (cnt of them) -> final rows, or part k0
-        auto join = [&](int k0, int step, int cnt, bool final) {
-          for (int x = tid; x < n_rows * cnt; x += kConsumers) {
-            const int r = x / cnt, k = x - r * cnt;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot_of(k0 + k * step) * ROWS + r) * 2));
-            w_s[r * 40 + k] = ml.x;
-            w_s[r * 40 + 20 + k] = ml.y;
-          }
-          consumer_sync();
-          if (tid < n_rows) {
+        // part k of the segment: CTA c0 + k; CTA c0's second part when it began with another segment.
+        // A group's sum: behind all parts, by its first CTA.
+        const int first_slot = c0 * 2 + (cut.begin(c0) < seg_start ? 1 : 0);
+        // parts [k0, k0 + cnt) of the segment, or its group sums, -> the rows, or group sum `to`
+        auto join = [&](int k0, int cnt, bool of_groups, int to) {
+          auto slot_of = [&](int k) {
+            if (!of_groups) return k0 + k == 0 ? first_slot : (c0 + k0 + k) * 2;
+            return k * kGroup + 1 == n ? c1 * 2 : 2 * p.ctas + c0 + k * kGroup;   // a group of one is its part
+          };
+#pragma unroll 1
+          for (int x = tid; x < n_rows * (D / 4); x += kConsumers) {
+            const int r = x / (D / 4), col = x % (D / 4) * 4;
             float mm = -INFINITY, sum = 0.f;
-            for (int k = 0; k < cnt; ++k) mm = fmaxf(mm, w_s[tid * 40 + k]);
-            const float mu = finite_or_zero(mm);
-            for (int k = 0; k < cnt; ++k) {
-              const float w = fast_exp2(w_s[tid * 40 + k] - mu);
-              sum += w * w_s[tid * 40 + 20 + k];
-              w_s[tid * 40 + k] = w;
-            }
-            sum_s[tid] = sum;
-            sum_s[ROWS + tid] = mm;
-          }
-          consumer_sync();
-          // a warp owns D/4 columns, 4 to a lane; its lanes' quarters (eighths) take every 4th (8th) part
-          constexpr int LC = C::DW / 4, LP = 32 / LC;   // lanes across the columns, parts side by side
-          const int col = warp * C::DW + (lane % LC) * 4, kp = lane / LC;
-#pragma unroll 2
-          for (int r = 0; r < n_rows; ++r) {
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 5
-            for (int k = kp; k < cnt; k += LP) {
-              const float w = w_s[r * 40 + k];
-              const float4 f =
-                  __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot_of(k0 + k * step) * ROWS + r) * D + col));
-              acc.x += w * f.x; acc.y += w * f.y; acc.z += w * f.z; acc.w += w * f.w;
-            }
+#pragma unroll 1
+            for (int kb = 0; kb < cnt; kb += 8) {
+              float2 ml[8];
+              float4 f[8];
 #pragma unroll
-            for (int off = LC; off < 32; off <<= 1) {
-              acc.x += __shfl_xor_sync(0xffffffffu, acc.x, off);
-              acc.y += __shfl_xor_sync(0xffffffffu, acc.y, off);
-              acc.z += __shfl_xor_sync(0xffffffffu, acc.z, off);
-              acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
+              for (int y = 0; y < 8; ++y) {
+                ml[y] = make_float2(-INFINITY, 0.f);
+                f[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (kb + y < cnt) {
+                  const int64_t at = (int64_t)slot_of(kb + y) * ROWS + r;
+                  ml[y] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
+                  f[y] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + col));
+                }
+              }
+              float mn = mm;
+#pragma unroll
+              for (int y = 0; y < 8; ++y) mn = fmaxf(mn, ml[y].x);
+              const float mu = finite_or_zero(mn), alpha = fast_exp2(mm - mu);
+              mm = mn;
+              sum *= alpha;
+              acc.x *= alpha; acc.y *= alpha; acc.z *= alpha; acc.w *= alpha;
+#pragma unroll
+              for (int y = 0; y < 8; ++y) {
+                const float w = fast_exp2(ml[y].x - mu);
+                sum += w * ml[y].y;
+                acc.x += w * f[y].x; acc.y += w * f[y].y; acc.z += w * f[y].z; acc.w += w * f[y].w;
+              }
             }
-            const float sum = sum_s[r], mm = sum_s[ROWS + r];
-            if (kp != 0) continue;
-            if (!final) {
-              // (these columns of part k0 were read by this lane alone)
-              *reinterpret_cast<float4*>(p.part_o + (slot_of(k0) * ROWS + r) * D + col) = acc;
-              if (warp == 0 && lane == 0)
-                *reinterpret_cast<float2*>(p.part_ml + (slot_of(k0) * ROWS + r) * 2) = make_float2(mm, sum);
+            if (to >= 0) {
+              const int64_t at = (int64_t)(2 * p.ctas + to) * ROWS + r;
+              *reinterpret_cast<float4*>(p.part_o + at * D + col) = acc;
+              if (col == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, sum);
               continue;
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -793,40 +795,37 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
             const int64_t row = ((int64_t)sb * p.HQ + sh * p.G + g) * p.T + t;
             *reinterpret_cast<uint2*>(p.out + row * D + col) =
                 make_uint2(pack2<HALF>(acc.x * inv, acc.y * inv), pack2<HALF>(acc.z * inv, acc.w * inv));
-            if (warp == 0 && lane == 0) {
+            if (col == 0) {
               const float lse2 = sum == 0.f ? -INFINITY : finite_or_zero(mm) + log2f(sum);
               if (p.lse) p.lse[row] = lse2 * 0.6931471805599453f;
               if (p.row_lse2) p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + R] = lse2;
             }
           }
-          consumer_sync();
         };
         // arrive at a counter that `of` CTAs share; true for the last one, which zeroes it
         auto arrive = [&](int* counter, int of) {
-          __threadfence();
           consumer_sync();
           if (tid == 0) {
+            __threadfence();   // the whole CTA's stores, which the barrier put in front of it
             const int is_last = atomicAdd(counter, 1) == of - 1;
-            if (is_last) *counter = 0;
+            if (is_last) {
+              *counter = 0;
+              __threadfence();
+            }
             *s_last = is_last;
           }
           consumer_sync();
-          const bool is_last = *s_last != 0;
-          if (is_last) __threadfence();
-          return is_last;
+          return *s_last != 0;
         };
-        const int grp = (int)(blockIdx.x - c0) / kGroup;
+        const int grp = (blockIdx.x - c0) / kGroup;
         const int in_group = min(kGroup, n - grp * kGroup);
-        // (a group of one needs no counter; its CTA may begin the next segment, whose first group counts there)
+        // (a group of one needs no counter and no sum; its CTA may begin the next segment, whose first group
+        // has them there)
         if (in_group == 1 || arrive(p.counters + p.ctas + c0 + grp * kGroup, in_group)) {
-          if (groups == 1) {
-            join(0, 1, n, true);
-          } else {
-            if (in_group > 1) join(grp * kGroup, 1, in_group, false);
-            if (arrive(p.counters + c0, groups)) join(0, kGroup, groups, true);
-          }
+          if (groups > 1 && in_group > 1) join(grp * kGroup, in_group, false, c0 + grp * kGroup);
+          if (groups == 1 || arrive(p.counters + c0, groups)) join(0, groups == 1 ? n : groups, groups > 1, -1);
         }
-        consumer_sync();   // s_last, the statistics and P are free again
+        consumer_sync();   // s_last and the statistics are free again
       }
     }
   }
@@ -927,11 +926,12 @@ static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
   p.cap = (int)cap;
   p.mt = R <= 16 ? 1 : R <= 32 ? 2 : 4;
   p.row_tiles = (p.R + 16 * p.mt - 1) / (16 * p.mt);
-  const int64_t tiles = std::max<int64_t>(1, (cap + tile - 1) / tile) * a->batch * a->kv_heads * p.row_tiles;
+  const int64_t tiles = std::max<int64_t>(1, (cap + tile - 1) / tile + 1) * a->batch * a->kv_heads * p.row_tiles;
+  if (tiles > (1ll << 31) - 1) return KVR_ERR_UNSUPPORTED;
   // two CTAs per SM; a join takes kGroup^2 parts and some
   p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, std::min(2 * num_sms_of(a->num_sms), kGroup * 20)));
   p.score_stride = std::max<int64_t>(128, (cap + 127) / 128 * 128);
-  const size_t rows = (size_t)16 * p.mt * 2 * p.ctas;
+  const size_t rows = (size_t)16 * p.mt * 3 * p.ctas;
   p.part_o = rows * a->head_dim * sizeof(float);
   p.part_ml = rows * 2 * sizeof(float);
   const size_t all_rows = (size_t)a->batch * a->kv_heads * p.R;
