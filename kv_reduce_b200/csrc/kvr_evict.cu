@@ -28,19 +28,49 @@ constexpr int kBins = 2048;
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
 }
-// Word of another CTA's shared memory.
+// A word of another CTA's shared memory.
 __device__ __forceinline__ uint32_t peer_word(const void* p, int rank) {
   uint32_t a, v;
   asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
+// 16 bytes at `p` from N CTAs, ranks r0 on.  One statement, so that the loads
+// are all on their way before the first is used (left to itself the compiler
+// adds each up as it arrives, a round trip apiece).
+template <int N>
+__device__ __forceinline__ void peer_vectors(const void* p, int r0, uint4 (&v)[N]) {
+  static_assert(N == 2 || N == 4, "");
+  const uint32_t a = smem_u32(p);
+  if constexpr (N == 2) {
+    asm volatile(
+        "{\n.reg .u32 a0, a1;\n"
+        "mapa.shared::cluster.u32 a0, %8, %9;\nmapa.shared::cluster.u32 a1, %8, %10;\n"
+        "ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [a0];\nld.shared::cluster.v4.u32 {%4, %5, %6, %7}, [a1];\n}\n"
+        : "=&r"(v[0].x), "=&r"(v[0].y), "=&r"(v[0].z), "=&r"(v[0].w), "=&r"(v[1].x), "=&r"(v[1].y), "=&r"(v[1].z),
+          "=&r"(v[1].w)
+        : "r"(a), "r"(r0), "r"(r0 + 1)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n.reg .u32 a0, a1, a2, a3;\n"
+        "mapa.shared::cluster.u32 a0, %16, %17;\nmapa.shared::cluster.u32 a1, %16, %18;\n"
+        "mapa.shared::cluster.u32 a2, %16, %19;\nmapa.shared::cluster.u32 a3, %16, %20;\n"
+        "ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [a0];\nld.shared::cluster.v4.u32 {%4, %5, %6, %7}, [a1];\n"
+        "ld.shared::cluster.v4.u32 {%8, %9, %10, %11}, [a2];\nld.shared::cluster.v4.u32 {%12, %13, %14, %15}, [a3];\n"
+        "}\n"
+        : "=&r"(v[0].x), "=&r"(v[0].y), "=&r"(v[0].z), "=&r"(v[0].w), "=&r"(v[1].x), "=&r"(v[1].y), "=&r"(v[1].z),
+          "=&r"(v[1].w), "=&r"(v[2].x), "=&r"(v[2].y), "=&r"(v[2].z), "=&r"(v[2].w), "=&r"(v[3].x), "=&r"(v[3].y),
+          "=&r"(v[3].z), "=&r"(v[3].w)
+        : "r"(a), "r"(r0), "r"(r0 + 1), "r"(r0 + 2), "r"(r0 + 3)
+        : "memory");
+  }
+}
 
 // Weights as integers in the same order (-0 as 0; NaN above all others).
 __device__ __forceinline__ uint32_t ordered(float w) {
-  if (w != w) return 0xffffffffu;
   const uint32_t u = __float_as_uint(w + 0.f);
-  return (u >> 31) ? ~u : u | 0x80000000u;
+  return w != w ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
 // Exclusive sum over the block; *total the whole.
@@ -72,17 +102,23 @@ struct Params {
   int* kept;            // [B, keep]
   int* new_lengths;     // [B]
   float* new_weights;   // [B, keep]
-  int cap, keep, recent, first, slice, cluster;
+  int cap, keep, recent, first, slice;
 };
 
+// CL: CTAs of the cluster, one sequence.  Its slices are contiguous, and so
+// are the threads' runs within a slice (of an odd number of words, so that 32
+// runs are read without bank conflicts), so that one sum over the block gives
+// every thread its place.
+template <int CL>
 __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ Params p) {
-  extern __shared__ uint32_t keys[];   // [slice]
-  __shared__ uint32_t hist[2][kBins];
+  extern __shared__ float slice[];     // [p.slice]
+  __shared__ __align__(16) uint32_t hist[2][kBins];
   __shared__ int buf[kThreads / 32];
-  __shared__ uint32_t s_counts[2];     // tokens kept for certain, ties
+  __shared__ uint32_t s_counts;        // tokens kept for certain | ties << 16
   __shared__ int s_digit[2];
-  pdl_wait();
-  const int tid = threadIdx.x, rank = blockIdx.x % p.cluster, b = blockIdx.x / p.cluster;
+  const int tid = threadIdx.x, rank = CL == 1 ? 0 : blockIdx.x % CL, b = blockIdx.x / CL;
+  for (int i = tid; i < 2 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
+  pdl_enter();
   const int len = min(max(p.lengths[b], 0), p.cap);
   const float* w = p.weights + (int64_t)b * p.weights_b;
   int* kept = p.kept + (int64_t)b * p.keep;
@@ -90,110 +126,110 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   const int n_new = min(len, p.keep);
   if (rank == 0 && tid == 0) p.new_lengths[b] = n_new;
   // slots behind the last kept token
-  for (int i = n_new + rank * kThreads + tid; i < p.keep; i += p.cluster * kThreads) {
+  for (int i = n_new + rank * kThreads + tid; i < p.keep; i += CL * kThreads) {
     kept[i] = -1;
     new_w[i] = 0.f;
   }
   if (len <= p.keep) {   // all of them (the whole cluster takes this way out)
-    for (int i = rank * kThreads + tid; i < len; i += p.cluster * kThreads) {
+    for (int i = rank * kThreads + tid; i < len; i += CL * kThreads) {
       kept[i] = i;
       new_w[i] = w[i];
     }
     return;
   }
   // candidates: [first, len - recent); this CTA's slice of the sequence
-  const int c0 = p.first, c1 = len - p.recent;
-  const int part = (len + p.cluster - 1) / p.cluster;   // <= slice
+  const int part = (len + CL - 1) / CL;   // <= p.slice
   const int s0 = min(rank * part, len), n = min(part, len - s0);
-  for (int i = tid; i < n; i += kThreads) keys[i] = ordered(w[s0 + i]);
-  const int lo = max(c0 - s0, 0), hi = min(c1 - s0, n);   // candidates of the slice
-  int need = p.keep - p.first - p.recent;                 // heaviest candidates to keep
-  uint32_t prefix = 0;                                    // digits of the need-th heaviest found so far
-  int shift = 32;
-  if (need > 0) {
+#pragma unroll 4
+  for (int i = tid; i < n; i += kThreads) slice[i] = __ldg(w + s0 + i);
+  const int lo = max(p.first - s0, 0), hi = min(len - p.recent - s0, n);   // candidates of the slice
+  int need = p.keep - p.first - p.recent;                                  // heaviest candidates to keep
+  const bool any = need > 0;
+  uint32_t prefix = 0;                                                     // digits of the need-th heaviest so far
+  __syncthreads();
+  if (any) {
+#pragma unroll
     for (int round = 0; round < 3; ++round) {
-      const int bits = round == 2 ? 10 : 11, bins = 1 << bits;
+      // bits 31-21, 20-10, 9-0 (the last round on 1024 bins)
+      const int down = round == 0 ? 21 : round == 1 ? 10 : 0, up = round == 1 ? 21 : 10;
+      const int bins = round == 2 ? 1024 : 2048;
       uint32_t* h = hist[round & 1];
-      for (int i = tid; i < bins; i += kThreads) h[i] = 0;
-      __syncthreads();
-      const int down = shift - bits;
       for (int i = lo + tid; i < hi; i += kThreads) {
-        const uint32_t k = keys[i];
-        if (round == 0 || (k >> shift) == prefix) atomicAdd(&h[(k >> down) & (bins - 1)], 1u);
+        const uint32_t k = ordered(slice[i]);
+        if (round == 0 || (k >> up) == prefix) atomicAdd(&h[(k >> down) & (bins - 1)], 1u);
       }
-      if (p.cluster > 1) cluster_sync();
+      if (CL > 1) cluster_sync();
       else __syncthreads();
-      // thread t adds up 4 (2 in the last round) bins, the highest first
-      const int per = bins / kThreads, top = bins - 1 - tid * per;
-      uint32_t c[4];
-      int mine = 0;
-      for (int j = 0; j < per; ++j) {
-        c[j] = 0;
-        if (p.cluster == 1) c[j] = h[top - j];
-        else
-          for (int r = 0; r < p.cluster; ++r) c[j] += peer_word(&h[top - j], r);
-        mine += (int)c[j];
-      }
-      int total;
-      int before = block_scan(mine, buf, &total);
-      if (before < need && need <= before + mine) {
-        for (int j = 0; j < per; ++j) {
-          if (need <= before + (int)c[j]) {
-            s_digit[0] = top - j;
-            s_digit[1] = need - before;
-            break;
+      // thread t adds up 4 bins over the cluster, the highest first (in the last round half the threads do)
+      const int at = bins - 4 - tid * 4;   // its lowest bin
+      uint32_t c[4] = {0, 0, 0, 0};
+      if (at >= 0) {
+        auto add = [&](const uint4& x) {
+          c[0] += x.x; c[1] += x.y; c[2] += x.z; c[3] += x.w;
+        };
+        if constexpr (CL == 1) {
+          add(*reinterpret_cast<const uint4*>(&h[at]));
+        } else {
+          constexpr int N = CL < 4 ? CL : 4;
+#pragma unroll
+          for (int r = 0; r < CL; r += N) {
+            uint4 v[N];
+            peer_vectors<N>(&h[at], r, v);
+#pragma unroll
+            for (int y = 0; y < N; ++y) add(v[y]);
           }
-          before += (int)c[j];
         }
       }
+      int total;
+      int before = block_scan((int)(c[0] + c[1] + c[2] + c[3]), buf, &total);
+#pragma unroll
+      for (int j = 3; j >= 0; --j) {
+        if (before < need && need <= before + (int)c[j]) {
+          s_digit[0] = at + j;
+          s_digit[1] = need - before;
+        }
+        before += (int)c[j];
+      }
+      // round 2 counts where round 0 did: every peer has read that by now (it is past round 1's cluster barrier)
+      if (round == 1)
+        for (int i = tid; i < kBins; i += kThreads) hist[0][i] = 0;
       __syncthreads();
-      prefix = round == 0 ? (uint32_t)s_digit[0] : (prefix << bits) | (uint32_t)s_digit[0];
+      prefix = round == 0 ? (uint32_t)s_digit[0] : (prefix << (round == 1 ? 11 : 10)) | (uint32_t)s_digit[0];
       need = s_digit[1];   // of the tokens that share these digits, the heaviest `need`
-      shift = down;
     }
-  } else {
-    __syncthreads();
   }
   // prefix is the key of the last token to be kept; `need` of its ties are, the first ones
-  const bool any = p.keep - p.first - p.recent > 0;
-  int sure = 0, ties = 0;
-  for (int i = tid; i < n; i += kThreads) {
+  const int run = ((n + kThreads - 1) / kThreads) | 1, r0 = min(tid * run, n), r1 = min(r0 + run, n);
+  int mine = 0;
+  for (int i = r0; i < r1; ++i) {
+    const uint32_t k = ordered(slice[i]);
     const bool cand = i >= lo && i < hi;
-    sure += !cand || (any && keys[i] > prefix);
-    ties += cand && any && keys[i] == prefix;
+    mine += !cand || (any && k > prefix) ? 1 : any && k == prefix ? 1 << 16 : 0;
   }
-  int all_sure, all_ties;
-  block_scan(sure, buf, &all_sure);
-  block_scan(ties, buf, &all_ties);
-  if (tid == 0) {
-    s_counts[0] = (uint32_t)all_sure;
-    s_counts[1] = (uint32_t)all_ties;
-  }
-  int at = 0, ties_before = 0;
-  if (p.cluster > 1) {
+  int total;
+  const int before = block_scan(mine, buf, &total);
+  int sure = before & 0xffff, ties = (int)((uint32_t)before >> 16);
+  if (CL > 1) {
+    if (tid == 0) s_counts = (uint32_t)total;
     cluster_sync();
-    for (int r = 0; r < rank; ++r) {
-      at += (int)peer_word(&s_counts[0], r);
-      ties_before += (int)peer_word(&s_counts[1], r);
-    }
+    // lane r asks CTA r
+    const int lane = tid & 31;
+    const uint32_t x = lane < rank ? peer_word(&s_counts, lane) : 0u;
+    sure += __reduce_add_sync(~0u, (int)(x & 0xffff));
+    ties += __reduce_add_sync(~0u, (int)(x >> 16));
   }
-  at += min(ties_before, need);
-  for (int base = 0; base < n; base += kThreads) {
-    const int i = base + tid;
-    const bool cand = i >= lo && i < hi, live = i < n;
-    const bool tie = live && cand && any && keys[i] == prefix;
-    int n_ties, n_kept;
-    const int tie_rank = ties_before + block_scan(tie, buf, &n_ties);
-    const bool keep = live && (!cand || (any && keys[i] > prefix) || (tie && tie_rank < need));
-    const int pos = at + block_scan(keep, buf, &n_kept);
-    if (keep) {
+  for (int i = r0; i < r1; ++i) {
+    const uint32_t k = ordered(slice[i]);
+    const bool cand = i >= lo && i < hi, in = !cand || (any && k > prefix), tie = !in && any && k == prefix;
+    if (in || (tie && ties < need)) {
+      const int pos = sure + min(ties, need);
       kept[pos] = s0 + i;
-      new_w[pos] = w[s0 + i];
+      new_w[pos] = slice[i];
     }
-    at += n_kept;
-    ties_before += n_ties;
+    sure += in;
+    ties += tie;
   }
-  if (p.cluster > 1) cluster_sync();   // peers may still read this CTA's counts
+  if (CL > 1) cluster_sync();   // peers may still read this CTA's counts
 }
 
 constexpr int kCopyTokens = 32, kCopyThreads = 256;
@@ -240,8 +276,23 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
   }
 }
 
-// Slices of at most 40,000 weights (160 KB of shared memory), clusters of at most 8.
+// Slices of at most 40,000 weights: 160 KB of shared memory, counts of 16 bits.
 constexpr int kMaxSlice = 40000;
+
+template <int CL>
+static cudaError_t launch_select(const Params& p, int batch, cudaStream_t s) {
+  static bool ready[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  if (!ready[dev & 63]) {   // a benign race sets the same value
+    const cudaError_t e = cudaFuncSetAttribute(select_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kMaxSlice * (int)sizeof(float));
+    if (e != cudaSuccess) return e;
+    ready[dev & 63] = true;
+  }
+  return pdl_launch(select_kernel<CL>, dim3((unsigned)(batch * CL)), dim3(kThreads), (size_t)p.slice * sizeof(float), s,
+                    CL, p);
+}
 
 }  // namespace evict
 }  // namespace kvr
@@ -273,24 +324,18 @@ extern "C" int kvr_paged_evict(const kvr_paged_evict_args* a, kvr_stream_t strea
   p.weights = a->token_weights; p.weights_b = a->weights_b_stride;
   p.lengths = a->lengths; p.kept = a->kept; p.new_lengths = a->new_lengths; p.new_weights = a->new_weights;
   p.cap = (int)cap; p.keep = a->keep; p.recent = a->recent; p.first = a->first;
-  // CTAs per sequence: as many as fit the GPU beside the batch, of 1024 weights or more
-  p.cluster = 1;
-  while (p.cluster < 8 && (cap > (int64_t)p.cluster * evict::kMaxSlice ||
-                           (cap > 1024ll * p.cluster && (int64_t)a->batch * p.cluster * 2 <= 148)))
-    p.cluster *= 2;
-  p.slice = (int)std::max<int64_t>(1, (cap + p.cluster - 1) / p.cluster);
-  const size_t smem = (size_t)p.slice * sizeof(uint32_t);
-  static bool ready[64] = {false};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
-  if (!ready[dev & 63]) {   // a benign race sets the same value
-    const cudaError_t e = cudaFuncSetAttribute(evict::select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               evict::kMaxSlice * (int)sizeof(uint32_t));
-    if (e != cudaSuccess) { set_last_cuda_error(e); return KVR_ERR_CUDA; }
-    ready[dev & 63] = true;
-  }
-  cudaError_t e = pdl_launch(evict::select_kernel, dim3((unsigned)(a->batch * p.cluster)), dim3(evict::kThreads), smem,
-                             s, p.cluster, p);
+  // CTAs per sequence, while they fit the GPU beside the batch: a CTA takes 4096 weights about as fast as a
+  // cluster shares them (5K weights: 10.5, 10.9, 12.0, 15.1 us for the whole call with 1, 2, 4, 8 CTAs; 32 times
+  // 4K to 16K: 114, 109, 107, 118 us), and a cluster of 8 takes 3 us longer than one of 4.
+  int cluster = 1;
+  while (cluster < 8 && (cap > (int64_t)cluster * evict::kMaxSlice ||
+                         (cap > (cluster < 4 ? 4096ll : 8192ll) * cluster && (int64_t)a->batch * cluster * 2 <= 148)))
+    cluster *= 2;
+  p.slice = (int)std::max<int64_t>(1, (cap + cluster - 1) / cluster);
+  cudaError_t e = cluster == 8   ? evict::launch_select<8>(p, a->batch, s)
+                  : cluster == 4 ? evict::launch_select<4>(p, a->batch, s)
+                  : cluster == 2 ? evict::launch_select<2>(p, a->batch, s)
+                                 : evict::launch_select<1>(p, a->batch, s);
   const int64_t rows = std::min<int64_t>(a->keep, cap);
   if (e == cudaSuccess && rows > 0)
     e = pdl_launch(evict::copy_kernel,

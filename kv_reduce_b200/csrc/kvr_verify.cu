@@ -12,12 +12,13 @@
 // more pass over one row, in any order, with a maximum at its end.
 //
 // What bounds it: the logits' bytes, 2 K rows (up to the first refusal) of
-// 2*V bytes and one race row per sequence.  Every row is cut into chunks, a
-// CTA takes the same chunk of p_k and q_k and keeps it in registers: one read
-// for maximum and sum.  CTAs run through the positions in order, and one that
-// finds its sequence already refused earlier leaves its rows unread: that
-// changes the work, never the result, since no row behind the first refusal
-// is used.
+// 2*V bytes and one race row per sequence, with one exponential per logit
+// close behind (16 per clock and SM).  Every row is cut into chunks, a CTA
+// takes the same chunk of p_k and q_k and keeps it in registers: one read for
+// maximum and sum.  CTAs run through the positions in order, and in a large
+// batch one that finds its sequence already refused earlier leaves its rows
+// unread: that changes the work, never the result, since no row behind the
+// first refusal is used.
 #include "kvr_common.cuh"
 
 #include <algorithm>
@@ -47,13 +48,14 @@ struct Params {
   int B, K, V, chunks;     // chunks of a row in the first pass
   int race_chunks;
   float c;                 // log2(e) / temperature
+  bool skip;               // look for earlier refusals before reading
   // zero on entry and on exit
   unsigned long long* best;   // greedy [B, K + 1], else [B]
   int* arrived;               // [B, K + 1]
   int* done;                  // [B]
   int* refused;               // [B]: K + 1 - (first refused position), 0 while none is known
   // scratch
-  float4* part;               // [B, K, chunks]: (max, sum) of the target's and the draft's chunk
+  float4* part;               // [B, K, chunks]: (max * c, sum) of the target's and the draft's chunk
   float4* stats;              // [B, K]: the same of the rows
 };
 
@@ -69,6 +71,11 @@ struct Vec<__nv_bfloat16> {
     f[4] = bf16lo(w.z); f[5] = bf16hi(w.z); f[6] = bf16lo(w.w); f[7] = bf16hi(w.w);
   }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {   // of two pairs; a NaN gives way
+    asm("max.bf16x2 %0, %0, %1;\n" : "+r"(a) : "r"(b));
+    return a;
+  }
+  static __device__ __forceinline__ float top(uint32_t w) { return fmaxf(bf16lo(w), bf16hi(w)); }
   static constexpr uint32_t kLowest = 0xff80ff80u;   // -inf, -inf
 };
 template <>
@@ -84,6 +91,14 @@ struct Vec<__half> {
     }
   }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    asm("max.f16x2 %0, %0, %1;\n" : "+r"(a) : "r"(b));
+    return a;
+  }
+  static __device__ __forceinline__ float top(uint32_t w) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return fmaxf(v.x, v.y);
+  }
   static constexpr uint32_t kLowest = 0xfc00fc00u;
 };
 template <>
@@ -93,6 +108,10 @@ struct Vec<float> {
     f[0] = __uint_as_float(w.x); f[1] = __uint_as_float(w.y); f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
   }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float top(uint32_t w) { return __uint_as_float(w); }
   static constexpr uint32_t kLowest = 0xff800000u;
 };
 
@@ -133,39 +152,37 @@ struct Row {
 template <typename T>
 __device__ __forceinline__ int blocks_of(int V) { return (V + Vec<T>::N - 1) / Vec<T>::N; }
 
-__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float c) {
+// Maxima are kept times c, rounded once: m in 2^(x c - m) is one number for
+// the whole row and its rounding falls out of every ratio.
+__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
   const float mm = fmaxf(m, m2), mu = zero_if_none(mm);
-  s = s * fast_exp2((m - mu) * c) + s2 * fast_exp2((m2 - mu) * c);
+  s = s * fast_exp2(m - mu) + s2 * fast_exp2(m2 - mu);
   m = mm;
 }
 
-// (max, sum of 2^((x - max) c)) of the thread's UN blocks
+// (max c, sum of 2^(x c - max c)) of the thread's UN blocks
 template <typename T, int UN>
 __device__ __forceinline__ void chunk_stats(const uint4 (&w)[UN], float c, float& m, float& s) {
-  m = -INFINITY;
+  uint32_t top = Vec<T>::kLowest;
+#pragma unroll
+  for (int i = 0; i < UN; ++i)
+    top = Vec<T>::max2(top, Vec<T>::max2(Vec<T>::max2(w[i].x, w[i].y), Vec<T>::max2(w[i].z, w[i].w)));
+  m = Vec<T>::top(top) * c;
+  const float mu = zero_if_none(m);
+  float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < UN; ++i) {
     float f[Vec<T>::N];
     Vec<T>::get(w[i], f);
 #pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j) m = fmaxf(m, f[j]);
+    for (int j = 0; j < Vec<T>::N; ++j) part[j & 3] += fast_exp2(__fmaf_rn(f[j], c, -mu));
   }
-  const float mu = zero_if_none(m);   // x - max is exact or nearly so: the product with c is the one rounding
-  s = 0.f;
-#pragma unroll
-  for (int i = 0; i < UN; ++i) {
-    float f[Vec<T>::N];
-    Vec<T>::get(w[i], f);
-    float t = 0.f;
-#pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j) t += fast_exp2((f[j] - mu) * c);
-    s += t;
-  }
+  s = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-__device__ __forceinline__ void warp_merge(float& m, float& s, float c, float2* buf) {
+__device__ __forceinline__ void warp_merge(float& m, float& s, float2* buf) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) merge(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), c);
+  for (int o = 16; o; o >>= 1) merge(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o));
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = make_float2(m, s);
 }
 
@@ -185,9 +202,11 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const __grid_constant__
   const int k = blockIdx.x / per_k, b = (blockIdx.x - k * per_k) / p.chunks, ch = blockIdx.x % p.chunks;
   const int n_draft = drafted(p, b);
   if (k >= n_draft) return;
-  if (threadIdx.x == 0) s_flag = refused_at(p, b) < k;
-  __syncthreads();
-  if (s_flag) return;   // an earlier position of this sequence is refused already
+  if (p.skip && k > 0) {
+    if (threadIdx.x == 0) s_flag = refused_at(p, b) < k;
+    __syncthreads();
+    if (s_flag) return;   // an earlier position of this sequence is refused already
+  }
   const T* trow = static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)k * p.t_k;
   const T* drow = static_cast<const T*>(p.draft) + (int64_t)b * p.d_b + (int64_t)k * p.d_k;
   const Row<T> rt(trow), rd(drow);
@@ -201,15 +220,15 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const __grid_constant__
   float mt, st, md, sd;
   chunk_stats<T, UN>(wt, p.c, mt, st);
   chunk_stats<T, UN>(wd, p.c, md, sd);
-  warp_merge(mt, st, p.c, buf[0]);
-  warp_merge(md, sd, p.c, buf[1]);
+  warp_merge(mt, st, buf[0]);
+  warp_merge(md, sd, buf[1]);
   __syncthreads();
   const int row = b * p.K + k;
   if (threadIdx.x == 0) {
     mt = buf[0][0].x; st = buf[0][0].y; md = buf[1][0].x; sd = buf[1][0].y;
     for (int w = 1; w < kThreads / 32; ++w) {
-      merge(mt, st, buf[0][w].x, buf[0][w].y, p.c);
-      merge(md, sd, buf[1][w].x, buf[1][w].y, p.c);
+      merge(mt, st, buf[0][w].x, buf[0][w].y);
+      merge(md, sd, buf[1][w].x, buf[1][w].y);
     }
     p.part[(int64_t)row * p.chunks + ch] = make_float4(mt, st, md, sd);
     __threadfence();
@@ -223,13 +242,13 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const __grid_constant__
   st = sd = 0.f;
   for (int i = threadIdx.x; i < p.chunks; i += 32) {
     const float4 q = __ldcg(p.part + (int64_t)row * p.chunks + i);
-    merge(mt, st, q.x, q.y, p.c);
-    merge(md, sd, q.z, q.w, p.c);
+    merge(mt, st, q.x, q.y);
+    merge(md, sd, q.z, q.w);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    merge(mt, st, __shfl_xor_sync(~0u, mt, o), __shfl_xor_sync(~0u, st, o), p.c);
-    merge(md, sd, __shfl_xor_sync(~0u, md, o), __shfl_xor_sync(~0u, sd, o), p.c);
+    merge(mt, st, __shfl_xor_sync(~0u, mt, o), __shfl_xor_sync(~0u, st, o));
+    merge(md, sd, __shfl_xor_sync(~0u, md, o), __shfl_xor_sync(~0u, sd, o));
   }
   if (threadIdx.x == 0) {
     p.stats[row] = make_float4(mt, st, md, sd);
@@ -237,7 +256,7 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(const __grid_constant__
     float a = 0.f;   // a token outside the vocabulary is refused
     if (x >= 0 && x < p.V) {
       const float lt = Vec<T>::one(trow + x), ld = Vec<T>::one(drow + x);
-      const float r = exp2f(((lt - zero_if_none(mt)) - (ld - zero_if_none(md))) * p.c) * (sd / st);
+      const float r = exp2f(__fmaf_rn(lt, p.c, -zero_if_none(mt)) - __fmaf_rn(ld, p.c, -zero_if_none(md))) * (sd / st);
       a = r >= 1.f ? 1.f : r > 0.f ? r : 0.f;   // 0 / 0: not in the target's support
     }
     p.accept_prob[row] = a;
@@ -295,30 +314,24 @@ __device__ __forceinline__ void load_noise(const float* p, int e, int V, float (
   }
 }
 
-// weight / e over blocks [begin, end) of one row, in logarithms: x c - log2 e
-// has the same order and needs neither the row's maximum nor its sum.
+// weight / e over one block, in logarithms: x c - log2 e has the same order
+// and needs neither the row's maximum nor its sum.
 template <typename T>
-__device__ __forceinline__ unsigned long long race_target(const Params& p, const Row<T>& row, const float* noise,
-                                                          int begin, int end) {
-  constexpr int N = Vec<T>::N;
-  float top = -INFINITY;
-  int where = -1;
-#pragma unroll 2
-  for (int g = begin + threadIdx.x; g < end; g += kThreads) {
-    float f[N], e[N];
-    Vec<T>::get(row.load(g, p.V), f);
-    load_noise(noise, g * N, p.V, e);
+__device__ __forceinline__ void race_target(const uint4& w, const float (&e)[Vec<T>::N], float c, int at, float& top,
+                                            int& where) {
+  float f[Vec<T>::N];
+  Vec<T>::get(w, f);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float key = f[j] * p.c - __log2f(e[j]);
-      if (key > top) {
-        top = key;
-        where = g * N + j;
-      }
+  for (int j = 0; j < Vec<T>::N; ++j) {
+    const float key = f[j] * c - __log2f(e[j]);
+    if (key > top) {
+      top = key;
+      where = at + j;
     }
   }
-  return where < 0 ? 0ull : race_key(top, where);
 }
+
+constexpr int kRaceBlocks = 2;   // blocks of a thread: all its loads are issued at once
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) race_kernel(const __grid_constant__ Params p) {
@@ -327,52 +340,69 @@ __global__ void __launch_bounds__(kThreads) race_kernel(const __grid_constant__ 
   pdl_wait();
   const int b = blockIdx.x / p.race_chunks, ch = blockIdx.x % p.race_chunks;
   const int n_draft = drafted(p, b), at = min(refused_at(p, b), n_draft);
-  const T* trow = static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)at * p.t_k;
   const float* noise = p.noise + (int64_t)b * p.n_b;
   constexpr int N = Vec<T>::N;
-  const Row<T> rt(trow);
-  const int blocks = blocks_of<T>(p.V), per = (blocks + p.race_chunks - 1) / p.race_chunks;
-  const int begin = ch * per, end = min(begin + per, blocks);
-  unsigned long long best = 0;
+  const Row<T> rt(static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)at * p.t_k);
+  const int blocks = blocks_of<T>(p.V), g0 = ch * kRaceBlocks * kThreads + threadIdx.x;
+  const uint4 none = make_uint4(Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest);
+  uint4 wt[kRaceBlocks], wd[kRaceBlocks];
+  float e[kRaceBlocks][N];
+#pragma unroll
+  for (int i = 0; i < kRaceBlocks; ++i) {
+    const int g = g0 + i * kThreads;
+    wt[i] = g < blocks ? rt.load(g, p.V) : none;
+    if (g < blocks) load_noise(noise, g * N, p.V, e[i]);
+    else
+      for (int j = 0; j < N; ++j) e[i][j] = 1.f;
+  }
+  float top = -INFINITY;
+  int where = -1;
   if (at < n_draft) {
     const Row<T> rd(static_cast<const T*>(p.draft) + (int64_t)b * p.d_b + (int64_t)at * p.d_k);
+#pragma unroll
+    for (int i = 0; i < kRaceBlocks; ++i) wd[i] = g0 + i * kThreads < blocks ? rd.load(g0 + i * kThreads, p.V) : none;
     const float4 st = p.stats[b * p.K + at];
     const float mt = zero_if_none(st.x), md = zero_if_none(st.z);
     const float it = st.y > 0.f ? 1.f / st.y : 0.f, id = st.w > 0.f ? 1.f / st.w : 0.f;
-    float top = 0.f;
-    int where = -1;
-#pragma unroll 2
-    for (int g = begin + threadIdx.x; g < end; g += kThreads) {
-      float f[N], d[N], e[N];
-      Vec<T>::get(rt.load(g, p.V), f);
-      Vec<T>::get(rd.load(g, p.V), d);
-      load_noise(noise, g * N, p.V, e);
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRaceBlocks; ++i) {
+      float f[N], d[N];
+      Vec<T>::get(wt[i], f);
+      Vec<T>::get(wd[i], d);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float w = fast_exp2((f[j] - mt) * p.c) * it - fast_exp2((d[j] - md) * p.c) * id;
-        const float score = __fdividef(w, e[j]);
+        const float w = fast_exp2(__fmaf_rn(f[j], p.c, -mt)) * it - fast_exp2(__fmaf_rn(d[j], p.c, -md)) * id;
+        const float score = __fdividef(w, e[i][j]);
         if (score > top) {
           top = score;
-          where = g * N + j;
+          where = (g0 + i * kThreads) * N + j;
         }
       }
     }
-    best = where < 0 ? 0ull : race_key(top, where);
   } else {
-    best = race_target<T>(p, rt, noise, begin, end);
+#pragma unroll
+    for (int i = 0; i < kRaceBlocks; ++i) race_target<T>(wt[i], e[i], p.c, (g0 + i * kThreads) * N, top, where);
   }
-  best = block_best(best, buf);
+  unsigned long long best = block_best(where < 0 ? 0ull : race_key(top, where), buf);
   if (threadIdx.x == 0) {
     if (best) atomicMax(p.best + b, best);
     __threadfence();
     s_last = atomicAdd(p.done + b, 1) == p.race_chunks - 1;
+    if (s_last) __threadfence();
   }
   __syncthreads();
   if (!s_last) return;
-  __threadfence();
   best = *reinterpret_cast<volatile unsigned long long*>(p.best + b);
-  // p = q up to rounding leaves nothing to draw from: draw from p
-  if (best == 0 && at < n_draft) best = block_best(race_target<T>(p, rt, noise, 0, blocks), buf);
+  if (best == 0 && at < n_draft) {   // p = q up to rounding leaves nothing to draw from: draw from p
+    top = -INFINITY;
+    where = -1;
+    for (int g = threadIdx.x; g < blocks; g += kThreads) {
+      load_noise(noise, g * N, p.V, e[0]);
+      race_target<T>(rt.load(g, p.V), e[0], p.c, g * N, top, where);
+    }
+    best = block_best(where < 0 ? 0ull : race_key(top, where), buf);
+  }
   __syncthreads();
   write_out(p, b, at, best == 0 ? -1 : (int64_t)(0xffffffffu - (uint32_t)best), 1);
 }
@@ -382,15 +412,19 @@ __global__ void __launch_bounds__(kThreads) race_kernel(const __grid_constant__ 
 template <typename T, int UN>
 __global__ void __launch_bounds__(kThreads) greedy_kernel(const __grid_constant__ Params p) {
   __shared__ unsigned long long buf[kThreads / 32];
-  __shared__ int s_flag;
+  __shared__ int s_flag, s_at;
   pdl_wait();
   const int per_k = p.B * p.chunks;
   const int k = blockIdx.x / per_k, b = (blockIdx.x - k * per_k) / p.chunks, ch = blockIdx.x % p.chunks;
   const int n_draft = drafted(p, b);
-  if (threadIdx.x == 0) s_flag = k > n_draft || refused_at(p, b) < k;
-  __syncthreads();
-  const bool skip = s_flag;
-  __syncthreads();
+  bool skip = k > n_draft;
+  if (p.skip && k > 0) {
+    if (threadIdx.x == 0) s_flag = refused_at(p, b) < k;
+    __syncthreads();
+    skip |= s_flag != 0;
+    __syncthreads();
+  }
+  unsigned long long best = 0;
   if (!skip) {
     const Row<T> rt(static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)k * p.t_k);
     const int g0 = ch * UN * kThreads + threadIdx.x, blocks = blocks_of<T>(p.V);
@@ -412,29 +446,35 @@ __global__ void __launch_bounds__(kThreads) greedy_kernel(const __grid_constant_
           where = e + j;
         }
     }
-    const unsigned long long best = block_best(where < 0 ? 0ull : race_key(top, where), buf);
-    if (threadIdx.x == 0) {
-      unsigned long long* slot = p.best + (int64_t)b * (p.K + 1) + k;
-      if (best) atomicMax(slot, best);
-      __threadfence();
-      if (atomicAdd(p.arrived + b * (p.K + 1) + k, 1) == p.chunks - 1 && k < n_draft) {
-        __threadfence();
-        const unsigned long long x = *reinterpret_cast<volatile unsigned long long*>(slot);
-        const bool same = x != 0 && (int64_t)(0xffffffffu - (uint32_t)x) == p.tokens[(int64_t)b * p.tok_b + k];
-        p.accept_prob[b * p.K + k] = same ? 1.f : 0.f;
-        if (!same) atomicMax(p.refused + b, p.K + 1 - k);
-      }
-    }
+    best = block_best(where < 0 ? 0ull : race_key(top, where), buf);
   }
   if (threadIdx.x == 0) {
+    unsigned long long* slot = p.best + (int64_t)b * (p.K + 1) + k;
+    if (best) atomicMax(slot, best);
     __threadfence();
+    if (p.skip && !skip && k < n_draft && atomicAdd(p.arrived + b * (p.K + 1) + k, 1) == p.chunks - 1) {
+      __threadfence();
+      const unsigned long long x = *reinterpret_cast<volatile unsigned long long*>(slot);
+      if (x == 0 || (int64_t)(0xffffffffu - (uint32_t)x) != p.tokens[(int64_t)b * p.tok_b + k])
+        atomicMax(p.refused + b, p.K + 1 - k);
+    }
     s_flag = atomicAdd(p.done + b, 1) == (p.K + 1) * p.chunks - 1;
+    if (s_flag) __threadfence();
+    s_at = n_draft;
   }
   __syncthreads();
   if (!s_flag) return;
-  __threadfence();
-  const int at = min(refused_at(p, b), n_draft);
-  const unsigned long long x = *reinterpret_cast<volatile unsigned long long*>(p.best + (int64_t)b * (p.K + 1) + at);
+  // the sequence's last CTA: the first token that is not its row's argmax (rows behind it may be unread)
+  const volatile unsigned long long* rows = p.best + (int64_t)b * (p.K + 1);
+  for (int i = threadIdx.x; i < n_draft; i += kThreads) {
+    const unsigned long long x = rows[i];
+    if (x == 0 || (int64_t)(0xffffffffu - (uint32_t)x) != p.tokens[(int64_t)b * p.tok_b + i]) atomicMin(&s_at, i);
+  }
+  __syncthreads();
+  const int at = s_at;
+  for (int i = threadIdx.x; i < at; i += kThreads) p.accept_prob[b * p.K + i] = 1.f;
+  if (threadIdx.x == 0 && at < n_draft) p.accept_prob[b * p.K + at] = 0.f;
+  const unsigned long long x = rows[at];
   __syncthreads();
   write_out(p, b, at, x == 0 ? -1 : (int64_t)(0xffffffffu - (uint32_t)x), p.K + 1);
 }
@@ -442,6 +482,7 @@ __global__ void __launch_bounds__(kThreads) greedy_kernel(const __grid_constant_
 // ------------------------------------------------------------------- host
 struct Plan {
   int un, chunks, race_chunks;
+  bool skip;
   size_t zeroed, scratch;
 };
 
@@ -456,14 +497,17 @@ static int plan_of(const kvr_verify_args* a, Plan* out) {
   const int64_t blocks = (a->vocab + n - 1) / n;
   const int64_t rows = std::max<int64_t>(1, (int64_t)a->batch * (a->draft_tokens + (a->temperature > 0.f ? 0 : 1)));
   Plan p;
-  p.un = 8;
+  // 4 blocks of a row to a thread keep the registers at 64 (four CTAs per SM); fewer where that fills the GPU
+  p.un = 4;
   for (; p.un > 1; p.un /= 2)
     if (rows * ((blocks + p.un * kThreads - 1) / (p.un * kThreads)) >= 296) break;
   p.chunks = (int)((blocks + p.un * kThreads - 1) / (p.un * kThreads));
   if (rows * p.chunks > (1ll << 31) - 1) return KVR_ERR_UNSUPPORTED;
-  // the race: about 4 CTAs per SM over the batch, at least 1024 tokens each
-  p.race_chunks = (int)std::max<int64_t>(
-      1, std::min<int64_t>((a->vocab + 1023) / 1024, (592 + std::max(a->batch, 1) - 1) / std::max(a->batch, 1)));
+  // Looking for an earlier refusal costs every CTA a round trip to L2 and saves reading: not for logits that
+  // 5 us read anyway.
+  p.skip = rows * a->vocab * (a->dtype == 2 ? 4 : 2) > (32 << 20);
+  p.race_chunks = (int)((blocks + kRaceBlocks * kThreads - 1) / (kRaceBlocks * kThreads));
+  if ((int64_t)a->batch * p.race_chunks > (1ll << 31) - 1) return KVR_ERR_UNSUPPORTED;
   const size_t B = a->batch, K1 = a->draft_tokens + 1;
   p.zeroed = B * K1 * 8 + B * K1 * 4 + 2 * B * 4;
   p.scratch = B * (K1 - 1) * ((size_t)p.chunks + 1) * sizeof(float4);
@@ -475,13 +519,11 @@ template <typename T>
 static cudaError_t launch(const Params& p, const Plan& pl, bool greedy, cudaStream_t s) {
   auto grid = [&](int rows) { return dim3((unsigned)((int64_t)rows * p.B * pl.chunks)); };
   if (greedy) {
-    auto kern = pl.un == 8 ? greedy_kernel<T, 8> : pl.un == 4 ? greedy_kernel<T, 4> : pl.un == 2 ? greedy_kernel<T, 2>
-                                                                                              : greedy_kernel<T, 1>;
+    auto kern = pl.un == 4 ? greedy_kernel<T, 4> : pl.un == 2 ? greedy_kernel<T, 2> : greedy_kernel<T, 1>;
     return pdl_launch(kern, grid(p.K + 1), dim3(kThreads), 0, s, 1, p);
   }
   if (p.K > 0) {
-    auto kern = pl.un == 8 ? stats_kernel<T, 8> : pl.un == 4 ? stats_kernel<T, 4> : pl.un == 2 ? stats_kernel<T, 2>
-                                                                                            : stats_kernel<T, 1>;
+    auto kern = pl.un == 4 ? stats_kernel<T, 4> : pl.un == 2 ? stats_kernel<T, 2> : stats_kernel<T, 1>;
     cudaError_t e = pdl_launch(kern, grid(p.K), dim3(kThreads), 0, s, 1, p);
     if (e != cudaSuccess) return e;
   }
@@ -523,6 +565,7 @@ extern "C" int kvr_verify(const kvr_verify_args* a, kvr_stream_t stream) {
   p.draft_lengths = a->draft_lengths;
   p.out_tokens = a->out_tokens; p.accepted = a->accepted; p.accept_prob = a->accept_prob;
   p.B = a->batch; p.K = K; p.V = a->vocab; p.chunks = pl.chunks; p.race_chunks = pl.race_chunks;
+  p.skip = pl.skip;
   p.c = greedy ? 1.f : 1.4426950408889634f / a->temperature;
   const size_t rows = (size_t)p.B * (K + 1);
   p.best = static_cast<unsigned long long*>(a->zeroed);
