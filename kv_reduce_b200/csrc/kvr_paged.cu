@@ -25,7 +25,7 @@
 //    complete in the CTA: nothing is merged between warps.
 //  * A sequence that several CTAs share is joined by the last of them to
 //    arrive, in the order of the CTAs: the result does not depend on timing.
-#include "kvr_common.cuh"
+#include "kvr_ring.cuh"
 
 #include <cuda.h>
 
@@ -35,11 +35,12 @@
 namespace kvr {
 namespace paged {
 
+using namespace ring;
+
 constexpr int kWarps = 4;                     // consumers
 constexpr int kConsumers = 32 * kWarps;
 constexpr int kThreads = kConsumers + 32;     // and the producer warp
 constexpr int kGroup = 16;                    // CTAs a join takes at a time
-constexpr long long kWaitClocks = 2000000000ll;   // about a second
 
 // Rows that no mask leaves anything to keep m = -inf; 0 stands in for it
 // wherever it would be subtracted.
@@ -72,38 +73,6 @@ __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r
                : "r"(addr));
 }
 
-// ---- mbarriers.  A wait that runs out (which no input causes) is given up
-// after kWaitClocks: every later wait of the thread returns at once, the
-// loops end, and the outputs are NaN.
-__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void bar_arrive_tx(uint32_t bar, int bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, int parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __noinline__ bool bar_wait_long(uint32_t bar, int parity) {
-  const long long begin = clock64();
-  while (clock64() - begin < kWaitClocks)
-    for (int i = 0; i < 64; ++i)
-      if (bar_try(bar, parity)) return true;
-  return false;
-}
-__device__ __forceinline__ void bar_wait(uint32_t bar, int parity, bool& failed) {
-  if (bar_try(bar, parity) || failed) return;
-  failed = !bar_wait_long(bar, parity);
-}
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); }
 
 // A box of `rows` tokens x 64 elements of one head of one page.
@@ -225,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
       bar_init(empty + 8 * i, kWarps);
       bar_init(ready + 8 * i, 1);
     }
-    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    bar_init_fence();
   }
   pdl_wait();
 

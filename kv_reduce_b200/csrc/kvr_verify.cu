@@ -13,10 +13,12 @@
 //
 // What bounds it: the logits' bytes, 2 K rows (up to the first refusal) of
 // 2*V bytes and one race row per sequence, with one exponential per logit
-// close behind (16 per clock and SM).  Every row is cut into chunks, a CTA
-// takes the same chunk of p_k and q_k and keeps it in registers: one read for
-// maximum and sum.  CTAs run through the positions in order, and in a large
-// batch one that finds its sequence already refused earlier leaves its rows
+// close behind (16 per clock and SM).  Rows are cut into segments, one to a
+// warp, and the warps have nothing to do with one another: no barrier holds
+// a warp back, so that the loads, the exponentials and the round trips at a
+// segment's end of 32 and more warps per SM overlap.  A row pair's last
+// segment decides its position.  The segments come position by position, and
+// in a large batch one whose sequence is already refused earlier is left
 // unread: that changes the work, never the result, since no row behind the
 // first refusal is used.
 #include "kvr_common.cuh"
@@ -28,7 +30,9 @@
 namespace kvr {
 namespace verify {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnroll = 4;      // blocks a lane has in hand, and as many on their way
 
 struct Params {
   const void* target;
@@ -45,8 +49,9 @@ struct Params {
   int64_t* out_tokens;
   int* accepted;
   float* accept_prob;
-  int B, K, V, chunks;     // chunks of a row in the first pass
-  int race_chunks;
+  int B, K, V;
+  int segments, seg_blocks;            // of a row in the first pass: how many, and blocks of 16 bytes in one
+  int race_segments, race_blocks;
   float c;                 // log2(e) / temperature
   bool skip;               // look for earlier refusals before reading
   // zero on entry and on exit
@@ -55,8 +60,8 @@ struct Params {
   int* done;                  // [B]
   int* refused;               // [B]: K + 1 - (first refused position), 0 while none is known
   // scratch
-  float4* part;               // [B, K, chunks]: (max * c, sum) of the target's and the draft's chunk
-  float4* stats;              // [B, K]: the same of the rows
+  float2* part;               // [B, K, 2, segments]: (max, sum) of the target's and the draft's segments
+  float4* stats;              // [B, K]: the same of the rows, target then draft
 };
 
 __device__ __forceinline__ float zero_if_none(float m) { return m == -INFINITY ? 0.f : m; }
@@ -152,38 +157,69 @@ struct Row {
 template <typename T>
 __device__ __forceinline__ int blocks_of(int V) { return (V + Vec<T>::N - 1) / Vec<T>::N; }
 
-// Maxima are kept times c, rounded once: m in 2^(x c - m) is one number for
-// the whole row and its rounding falls out of every ratio.
-__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2) {
+// 2^((x - m) c): x - m is exact or nearly so, the product the one rounding,
+// and the largest gives 1 whatever c is.
+__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float c) {
   const float mm = fmaxf(m, m2), mu = zero_if_none(mm);
-  s = s * fast_exp2(m - mu) + s2 * fast_exp2(m2 - mu);
+  s = s * fast_exp2((m - mu) * c) + s2 * fast_exp2((m2 - mu) * c);
+  m = mm;
+}
+// The same over the warp's lanes, one exponential a lane.
+__device__ __forceinline__ void lanes_merge(float& m, float& s, float c) {
+  float mm = m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(~0u, mm, o));
+  s *= fast_exp2((m - zero_if_none(mm)) * c);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   m = mm;
 }
 
-// (max c, sum of 2^(x c - max c)) of the thread's UN blocks
+// Two fp32 operations to an instruction.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void halves(uint64_t x, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(lo), "=f"(hi) : "l"(x));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Takes UN blocks into a running (max, sum of 2^((x - max) c)).
 template <typename T, int UN>
-__device__ __forceinline__ void chunk_stats(const uint4 (&w)[UN], float c, float& m, float& s) {
+__device__ __forceinline__ void take(const uint4 (&w)[UN], float c, float& m, float& s) {
   uint32_t top = Vec<T>::kLowest;
 #pragma unroll
   for (int i = 0; i < UN; ++i)
     top = Vec<T>::max2(top, Vec<T>::max2(Vec<T>::max2(w[i].x, w[i].y), Vec<T>::max2(w[i].z, w[i].w)));
-  m = Vec<T>::top(top) * c;
-  const float mu = zero_if_none(m);
-  float part[4] = {0.f, 0.f, 0.f, 0.f};
+  const float mm = fmaxf(m, Vec<T>::top(top)), mu = zero_if_none(mm);
+  const uint64_t mu2 = pair(-mu, -mu), c2 = pair(c, c);
+  uint64_t sum[2] = {pair(s * fast_exp2((m - mu) * c), 0.f), pair(0.f, 0.f)};
+  m = mm;
 #pragma unroll
   for (int i = 0; i < UN; ++i) {
     float f[Vec<T>::N];
     Vec<T>::get(w[i], f);
 #pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j) part[j & 3] += fast_exp2(__fmaf_rn(f[j], c, -mu));
+    for (int j = 0; j < Vec<T>::N; j += 2) {
+      float a, b;
+      halves(mul2(add2(pair(f[j], f[j + 1]), mu2), c2), a, b);
+      sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pair(fast_exp2(a), fast_exp2(b)));
+    }
   }
-  s = (part[0] + part[1]) + (part[2] + part[3]);
-}
-
-__device__ __forceinline__ void warp_merge(float& m, float& s, float2* buf) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) merge(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o));
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = make_float2(m, s);
+  float a, b;
+  halves(add2(sum[0], sum[1]), a, b);
+  s = a + b;
 }
 
 __device__ __forceinline__ int drafted(const Params& p, int b) {
@@ -193,106 +229,106 @@ __device__ __forceinline__ int refused_at(const Params& p, int b) {   // K + 1: 
   return p.K + 1 - *reinterpret_cast<volatile int*>(p.refused + b);
 }
 
-template <typename T, int UN>
-__global__ void __launch_bounds__(kThreads) stats_kernel(const __grid_constant__ Params p) {
-  __shared__ float2 buf[2][kThreads / 32];
-  __shared__ int s_flag;
-  pdl_wait();
-  const int per_k = p.B * p.chunks;
-  const int k = blockIdx.x / per_k, b = (blockIdx.x - k * per_k) / p.chunks, ch = blockIdx.x % p.chunks;
-  const int n_draft = drafted(p, b);
-  if (k >= n_draft) return;
-  if (p.skip && k > 0) {
-    if (threadIdx.x == 0) s_flag = refused_at(p, b) < k;
-    __syncthreads();
-    if (s_flag) return;   // an earlier position of this sequence is refused already
-  }
-  const T* trow = static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)k * p.t_k;
-  const T* drow = static_cast<const T*>(p.draft) + (int64_t)b * p.d_b + (int64_t)k * p.d_k;
-  const Row<T> rt(trow), rd(drow);
-  const int g0 = ch * UN * kThreads + threadIdx.x, blocks = blocks_of<T>(p.V);
-  uint4 wt[UN], wd[UN];
-  const uint4 none = make_uint4(Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest);
-#pragma unroll
-  for (int i = 0; i < UN; ++i) wt[i] = g0 + i * kThreads < blocks ? rt.load(g0 + i * kThreads, p.V) : none;
-#pragma unroll
-  for (int i = 0; i < UN; ++i) wd[i] = g0 + i * kThreads < blocks ? rd.load(g0 + i * kThreads, p.V) : none;
-  float mt, st, md, sd;
-  chunk_stats<T, UN>(wt, p.c, mt, st);
-  chunk_stats<T, UN>(wd, p.c, md, sd);
-  warp_merge(mt, st, buf[0]);
-  warp_merge(md, sd, buf[1]);
-  __syncthreads();
-  const int row = b * p.K + k;
-  if (threadIdx.x == 0) {
-    mt = buf[0][0].x; st = buf[0][0].y; md = buf[1][0].x; sd = buf[1][0].y;
-    for (int w = 1; w < kThreads / 32; ++w) {
-      merge(mt, st, buf[0][w].x, buf[0][w].y);
-      merge(md, sd, buf[1][w].x, buf[1][w].y);
-    }
-    p.part[(int64_t)row * p.chunks + ch] = make_float4(mt, st, md, sd);
-    __threadfence();
-    s_flag = atomicAdd(p.arrived + b * (p.K + 1) + k, 1) == p.chunks - 1;
-  }
-  __syncthreads();
-  if (!s_flag || threadIdx.x >= 32) return;
-  // ---- the row's last chunk: join them in order and decide
-  __threadfence();
-  mt = md = -INFINITY;
-  st = sd = 0.f;
-  for (int i = threadIdx.x; i < p.chunks; i += 32) {
-    const float4 q = __ldcg(p.part + (int64_t)row * p.chunks + i);
-    merge(mt, st, q.x, q.y);
-    merge(md, sd, q.z, q.w);
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    merge(mt, st, __shfl_xor_sync(~0u, mt, o), __shfl_xor_sync(~0u, st, o));
-    merge(md, sd, __shfl_xor_sync(~0u, md, o), __shfl_xor_sync(~0u, sd, o));
-  }
-  if (threadIdx.x == 0) {
-    p.stats[row] = make_float4(mt, st, md, sd);
-    const int64_t x = p.tokens[(int64_t)b * p.tok_b + k];
-    float a = 0.f;   // a token outside the vocabulary is refused
-    if (x >= 0 && x < p.V) {
-      const float lt = Vec<T>::one(trow + x), ld = Vec<T>::one(drow + x);
-      const float r = exp2f(__fmaf_rn(lt, p.c, -zero_if_none(mt)) - __fmaf_rn(ld, p.c, -zero_if_none(md))) * (sd / st);
-      a = r >= 1.f ? 1.f : r > 0.f ? r : 0.f;   // 0 / 0: not in the target's support
-    }
-    p.accept_prob[row] = a;
-    if (!(p.uniforms[(int64_t)b * p.u_b + k] < a)) atomicMax(p.refused + b, p.K + 1 - k);
-  }
-}
-
 // Larger is better; equal weights: the lowest index.
 __device__ __forceinline__ unsigned long long race_key(float score, int index) {
   uint32_t u = __float_as_uint(score + 0.f);
   u = (u >> 31) ? ~u : u | 0x80000000u;
   return ((unsigned long long)u << 32) | (0xffffffffu - (uint32_t)index);
 }
-__device__ __forceinline__ unsigned long long block_best(unsigned long long best, unsigned long long* buf) {
+__device__ __forceinline__ int64_t race_index(unsigned long long key) {
+  return key == 0 ? -1 : (int64_t)(0xffffffffu - (uint32_t)key);
+}
+__device__ __forceinline__ unsigned long long lanes_best(unsigned long long best) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     const unsigned long long x = __shfl_xor_sync(~0u, best, o);
     best = x > best ? x : best;
   }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = best;
-  __syncthreads();
-  for (int w = 0; w < kThreads / 32; ++w) best = buf[w] > best ? buf[w] : best;
   return best;
 }
 
-// The sequence's outputs, and its zeros for the next call.
+// One segment of a row through `use(blocks in hand, first block)`, the next
+// blocks on their way.  Lane l has blocks first + 32 i + l.
+template <typename T, typename Use>
+__device__ __forceinline__ void stream(const Row<T>& row, int begin, int end, int V, Use use) {
+  const int lane = threadIdx.x & 31;
+  const uint4 none = make_uint4(Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest);
+  uint4 w[kUnroll], next[kUnroll];
+  auto load = [&](int g, uint4 (&x)[kUnroll]) {
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) x[i] = g + 32 * i + lane < end ? row.load(g + 32 * i + lane, V) : none;
+  };
+  load(begin, w);
+  for (int g = begin; g < end; g += 32 * kUnroll) {
+    if (g + 32 * kUnroll < end) load(g + 32 * kUnroll, next);
+    use(w, g);
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) w[i] = next[i];
+  }
+}
+
+// Rows in the order of their positions: (k, b, target | draft, segment).
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 8) stats_kernel(const __grid_constant__ Params p) {
+  const int lane = threadIdx.x & 31;
+  const int unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int seg = unit % p.segments, row = unit / p.segments;   // row = (k * B + b) * 2 + (draft)
+  const int side = row & 1, k = (row >> 1) / p.B, b = (row >> 1) - k * p.B;
+  if (k >= p.K) return;
+  pdl_wait();
+  const int n_draft = drafted(p, b);
+  if (k >= n_draft) return;
+  if (p.skip && k > 0 && refused_at(p, b) < k) return;   // an earlier position of this sequence is refused already
+  const T* trow = static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)k * p.t_k;
+  const T* drow = static_cast<const T*>(p.draft) + (int64_t)b * p.d_b + (int64_t)k * p.d_k;
+  float m = -INFINITY, s = 0.f;
+  const int begin = seg * p.seg_blocks, end = min(begin + p.seg_blocks, blocks_of<T>(p.V));
+  stream<T>(Row<T>(side ? drow : trow), begin, end, p.V,
+            [&](const uint4(&w)[kUnroll], int) { take<T, kUnroll>(w, p.c, m, s); });
+  lanes_merge(m, s, p.c);
+  const int at = b * p.K + k;
+  float2* part = p.part + (int64_t)at * 2 * p.segments;   // [2][segments]
+  int last = 0;
+  if (lane == 0) {
+    part[side * p.segments + seg] = make_float2(m, s);
+    __threadfence();
+    last = atomicAdd(p.arrived + b * (p.K + 1) + k, 1) == 2 * p.segments - 1;
+    if (last) __threadfence();
+  }
+  if (!__shfl_sync(~0u, last, 0)) return;
+  // ---- the position's last segment: join them in order and decide
+  float mt = -INFINITY, st = 0.f, md = -INFINITY, sd = 0.f;
+  for (int i = lane; i < p.segments; i += 32) {
+    const float2 x = __ldcg(part + i), y = __ldcg(part + p.segments + i);
+    merge(mt, st, x.x, x.y, p.c);
+    merge(md, sd, y.x, y.y, p.c);
+  }
+  lanes_merge(mt, st, p.c);
+  lanes_merge(md, sd, p.c);
+  if (lane == 0) {
+    p.stats[at] = make_float4(mt, st, md, sd);
+    const int64_t x = p.tokens[(int64_t)b * p.tok_b + k];
+    float a = 0.f;   // a token outside the vocabulary is refused
+    if (x >= 0 && x < p.V) {
+      const float lt = Vec<T>::one(trow + x), ld = Vec<T>::one(drow + x);
+      const float r = exp2f(((lt - zero_if_none(mt)) - (ld - zero_if_none(md))) * p.c) * (sd / st);
+      a = r >= 1.f ? 1.f : r > 0.f ? r : 0.f;   // 0 / 0: not in the target's support
+    }
+    p.accept_prob[at] = a;
+    if (!(p.uniforms[(int64_t)b * p.u_b + k] < a)) atomicMax(p.refused + b, p.K + 1 - k);
+  }
+}
+
+// The sequence's outputs, and its zeros for the next call, by one warp.
 __device__ __forceinline__ void write_out(const Params& p, int b, int at, int64_t token, int best_rows) {
-  for (int k = threadIdx.x; k <= p.K; k += kThreads) {
-    p.out_tokens[(int64_t)b * (p.K + 1) + k] =
-        k < at ? p.tokens[(int64_t)b * p.tok_b + k] : k == at ? token : -1;
-    if (k < p.K && (k > at || k >= drafted(p, b))) p.accept_prob[b * p.K + k] = 0.f;
+  const int n_draft = drafted(p, b), lane = threadIdx.x & 31;
+  for (int k = lane; k <= p.K; k += 32) {
+    p.out_tokens[(int64_t)b * (p.K + 1) + k] = k < at ? p.tokens[(int64_t)b * p.tok_b + k] : k == at ? token : -1;
+    if (k < p.K && (k > at || k >= n_draft)) p.accept_prob[b * p.K + k] = 0.f;
     p.arrived[b * (p.K + 1) + k] = 0;
     if (k < best_rows) p.best[(int64_t)b * best_rows + k] = 0;
   }
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
     p.accepted[b] = at;
     p.done[b] = 0;
     p.refused[b] = 0;
@@ -331,157 +367,164 @@ __device__ __forceinline__ void race_target(const uint4& w, const float (&e)[Vec
   }
 }
 
-constexpr int kRaceBlocks = 2;   // blocks of a thread: all its loads are issued at once
+constexpr int kRaceUnroll = 2;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) race_kernel(const __grid_constant__ Params p) {
-  __shared__ unsigned long long buf[kThreads / 32];
-  __shared__ int s_last;
-  pdl_wait();
-  const int b = blockIdx.x / p.race_chunks, ch = blockIdx.x % p.race_chunks;
-  const int n_draft = drafted(p, b), at = min(refused_at(p, b), n_draft);
-  const float* noise = p.noise + (int64_t)b * p.n_b;
+__global__ void __launch_bounds__(kThreads, 8) race_kernel(const __grid_constant__ Params p) {
   constexpr int N = Vec<T>::N;
+  const int lane = threadIdx.x & 31;
+  const int unit = blockIdx.x * kWarps + (threadIdx.x >> 5), b = unit / p.race_segments;
+  if (b >= p.B) return;
+  const int begin = (unit - b * p.race_segments) * p.race_blocks, end = min(begin + p.race_blocks, blocks_of<T>(p.V));
+  pdl_wait();
+  const int n_draft = drafted(p, b), at = min(refused_at(p, b), n_draft);
+  const bool residual = at < n_draft;
+  const float* noise = p.noise + (int64_t)b * p.n_b;
   const Row<T> rt(static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)at * p.t_k);
-  const int blocks = blocks_of<T>(p.V), g0 = ch * kRaceBlocks * kThreads + threadIdx.x;
-  const uint4 none = make_uint4(Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest);
-  uint4 wt[kRaceBlocks], wd[kRaceBlocks];
-  float e[kRaceBlocks][N];
-#pragma unroll
-  for (int i = 0; i < kRaceBlocks; ++i) {
-    const int g = g0 + i * kThreads;
-    wt[i] = g < blocks ? rt.load(g, p.V) : none;
-    if (g < blocks) load_noise(noise, g * N, p.V, e[i]);
-    else
-      for (int j = 0; j < N; ++j) e[i][j] = 1.f;
-  }
-  float top = -INFINITY;
+  float mt = 0.f, md = 0.f, it = 0.f, id = 0.f, top = -INFINITY;
   int where = -1;
-  if (at < n_draft) {
+  if (residual) {
     const Row<T> rd(static_cast<const T*>(p.draft) + (int64_t)b * p.d_b + (int64_t)at * p.d_k);
-#pragma unroll
-    for (int i = 0; i < kRaceBlocks; ++i) wd[i] = g0 + i * kThreads < blocks ? rd.load(g0 + i * kThreads, p.V) : none;
     const float4 st = p.stats[b * p.K + at];
-    const float mt = zero_if_none(st.x), md = zero_if_none(st.z);
-    const float it = st.y > 0.f ? 1.f / st.y : 0.f, id = st.w > 0.f ? 1.f / st.w : 0.f;
+    mt = zero_if_none(st.x);
+    md = zero_if_none(st.z);
+    it = st.y > 0.f ? 1.f / st.y : 0.f;
+    id = st.w > 0.f ? 1.f / st.w : 0.f;
     top = 0.f;
-#pragma unroll
-    for (int i = 0; i < kRaceBlocks; ++i) {
-      float f[N], d[N];
-      Vec<T>::get(wt[i], f);
-      Vec<T>::get(wd[i], d);
+#pragma unroll kRaceUnroll
+    for (int g = begin + lane; g < end; g += 32) {
+      float f[N], d[N], e[N];
+      Vec<T>::get(rt.load(g, p.V), f);
+      Vec<T>::get(rd.load(g, p.V), d);
+      load_noise(noise, g * N, p.V, e);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float w = fast_exp2(__fmaf_rn(f[j], p.c, -mt)) * it - fast_exp2(__fmaf_rn(d[j], p.c, -md)) * id;
-        const float score = __fdividef(w, e[i][j]);
+        const float x = fast_exp2((f[j] - mt) * p.c) * it - fast_exp2((d[j] - md) * p.c) * id;
+        const float score = __fdividef(x, e[j]);
         if (score > top) {
           top = score;
-          where = (g0 + i * kThreads) * N + j;
+          where = g * N + j;
         }
       }
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < kRaceBlocks; ++i) race_target<T>(wt[i], e[i], p.c, (g0 + i * kThreads) * N, top, where);
+#pragma unroll kRaceUnroll
+    for (int g = begin + lane; g < end; g += 32) {
+      float e[N];
+      const uint4 w = rt.load(g, p.V);
+      load_noise(noise, g * N, p.V, e);
+      race_target<T>(w, e, p.c, g * N, top, where);
+    }
   }
-  unsigned long long best = block_best(where < 0 ? 0ull : race_key(top, where), buf);
-  if (threadIdx.x == 0) {
+  unsigned long long best = lanes_best(where < 0 ? 0ull : race_key(top, where));
+  int last = 0;
+  if (lane == 0) {
     if (best) atomicMax(p.best + b, best);
     __threadfence();
-    s_last = atomicAdd(p.done + b, 1) == p.race_chunks - 1;
-    if (s_last) __threadfence();
+    last = atomicAdd(p.done + b, 1) == p.race_segments - 1;
+    if (last) __threadfence();
   }
-  __syncthreads();
-  if (!s_last) return;
+  if (!__shfl_sync(~0u, last, 0)) return;
   best = *reinterpret_cast<volatile unsigned long long*>(p.best + b);
-  if (best == 0 && at < n_draft) {   // p = q up to rounding leaves nothing to draw from: draw from p
+  if (best == 0 && residual) {   // p = q up to rounding leaves nothing to draw from: draw from p
     top = -INFINITY;
     where = -1;
-    for (int g = threadIdx.x; g < blocks; g += kThreads) {
-      load_noise(noise, g * N, p.V, e[0]);
-      race_target<T>(rt.load(g, p.V), e[0], p.c, g * N, top, where);
+    for (int g = lane; g < blocks_of<T>(p.V); g += 32) {
+      float e[N];
+      const uint4 w = rt.load(g, p.V);
+      load_noise(noise, g * N, p.V, e);
+      race_target<T>(w, e, p.c, g * N, top, where);
     }
-    best = block_best(where < 0 ? 0ull : race_key(top, where), buf);
+    best = lanes_best(where < 0 ? 0ull : race_key(top, where));
   }
-  __syncthreads();
-  write_out(p, b, at, best == 0 ? -1 : (int64_t)(0xffffffffu - (uint32_t)best), 1);
+  write_out(p, b, at, race_index(best), 1);
 }
 
 // t = 0: x_k is accepted while it is the argmax of target_k (the lowest index
-// of the largest logit; NaN is never the largest).
-template <typename T, int UN>
-__global__ void __launch_bounds__(kThreads) greedy_kernel(const __grid_constant__ Params p) {
-  __shared__ unsigned long long buf[kThreads / 32];
-  __shared__ int s_flag, s_at;
+// of the largest logit; NaN is never the largest).  A CTA's warps take
+// neighbouring segments of a row and count as one: with a maximum in place of
+// the exponentials the warps are done together, and the counts are what takes
+// time in a small batch.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 8) greedy_kernel(const __grid_constant__ Params p) {
+  constexpr int N = Vec<T>::N;
+  const int lane = threadIdx.x & 31;
+  const int chunks = (p.segments + kWarps - 1) / kWarps;   // CTAs of a row
+  const int row = blockIdx.x / chunks, k = row / p.B, b = row - k * p.B;
+  const int seg = (blockIdx.x - row * chunks) * kWarps + (threadIdx.x >> 5);
+  __shared__ unsigned long long buf[kWarps];
+  __shared__ int s_unread;
   pdl_wait();
-  const int per_k = p.B * p.chunks;
-  const int k = blockIdx.x / per_k, b = (blockIdx.x - k * per_k) / p.chunks, ch = blockIdx.x % p.chunks;
   const int n_draft = drafted(p, b);
-  bool skip = k > n_draft;
-  if (p.skip && k > 0) {
-    if (threadIdx.x == 0) s_flag = refused_at(p, b) < k;
+  bool unread = k > n_draft;
+  if (p.skip && k > 0) {   // one look for the whole CTA
+    if (threadIdx.x == 0) s_unread = refused_at(p, b) < k;
     __syncthreads();
-    skip |= s_flag != 0;
-    __syncthreads();
+    unread |= s_unread != 0;
   }
   unsigned long long best = 0;
-  if (!skip) {
-    const Row<T> rt(static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)k * p.t_k);
-    const int g0 = ch * UN * kThreads + threadIdx.x, blocks = blocks_of<T>(p.V);
-    uint4 w[UN];
-    const uint4 none = make_uint4(Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest, Vec<T>::kLowest);
-#pragma unroll
-    for (int i = 0; i < UN; ++i) w[i] = g0 + i * kThreads < blocks ? rt.load(g0 + i * kThreads, p.V) : none;
+  if (!unread) {
     float top = -INFINITY;
     int where = -1;
+    const int begin = seg * p.seg_blocks, end = min(begin + p.seg_blocks, blocks_of<T>(p.V));
+    stream<T>(Row<T>(static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)k * p.t_k), begin, end, p.V,
+              [&](const uint4(&w)[kUnroll], int g) {
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      float f[Vec<T>::N];
-      Vec<T>::get(w[i], f);
-      const int e = (g0 + i * kThreads) * Vec<T>::N;
+                for (int i = 0; i < kUnroll; ++i) {
+                  // most blocks hold nothing new: their largest pair tells
+                  const uint32_t high = Vec<T>::max2(Vec<T>::max2(w[i].x, w[i].y), Vec<T>::max2(w[i].z, w[i].w));
+                  if (!(Vec<T>::top(high) > top || where < 0)) continue;
+                  float f[N];
+                  Vec<T>::get(w[i], f);
+                  const int e = (g + 32 * i + lane) * N;
 #pragma unroll
-      for (int j = 0; j < Vec<T>::N; ++j)
-        if (e + j < p.V && (f[j] > top || (where < 0 && f[j] == top))) {
-          top = f[j];
-          where = e + j;
-        }
-    }
-    best = block_best(where < 0 ? 0ull : race_key(top, where), buf);
+                  for (int j = 0; j < N; ++j)
+                    if (f[j] > top || (where < 0 && f[j] == top && e + j < p.V)) {
+                      top = f[j];
+                      where = e + j;
+                    }
+                }
+              });
+    best = lanes_best(where < 0 ? 0ull : race_key(top, where));
   }
-  if (threadIdx.x == 0) {
+  if (lane == 0) buf[threadIdx.x >> 5] = best;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  int last = 0;
+  if (lane == 0) {
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) best = buf[w] > best ? buf[w] : best;
     unsigned long long* slot = p.best + (int64_t)b * (p.K + 1) + k;
     if (best) atomicMax(slot, best);
     __threadfence();
-    if (p.skip && !skip && k < n_draft && atomicAdd(p.arrived + b * (p.K + 1) + k, 1) == p.chunks - 1) {
+    if (p.skip && !unread && k < n_draft && atomicAdd(p.arrived + b * (p.K + 1) + k, 1) == chunks - 1) {
       __threadfence();
-      const unsigned long long x = *reinterpret_cast<volatile unsigned long long*>(slot);
-      if (x == 0 || (int64_t)(0xffffffffu - (uint32_t)x) != p.tokens[(int64_t)b * p.tok_b + k])
+      if (race_index(*reinterpret_cast<volatile unsigned long long*>(slot)) != p.tokens[(int64_t)b * p.tok_b + k])
         atomicMax(p.refused + b, p.K + 1 - k);
+      __threadfence();
     }
-    s_flag = atomicAdd(p.done + b, 1) == (p.K + 1) * p.chunks - 1;
-    if (s_flag) __threadfence();
-    s_at = n_draft;
+    last = atomicAdd(p.done + b, 1) == (p.K + 1) * chunks - 1;
+    if (last) __threadfence();
   }
-  __syncthreads();
-  if (!s_flag) return;
+  if (!__shfl_sync(~0u, last, 0)) return;
   // the sequence's last CTA: the first token that is not its row's argmax (rows behind it may be unread)
   const volatile unsigned long long* rows = p.best + (int64_t)b * (p.K + 1);
-  for (int i = threadIdx.x; i < n_draft; i += kThreads) {
-    const unsigned long long x = rows[i];
-    if (x == 0 || (int64_t)(0xffffffffu - (uint32_t)x) != p.tokens[(int64_t)b * p.tok_b + i]) atomicMin(&s_at, i);
+  int at = n_draft;
+  for (int i = lane; i < n_draft; i += 32) {
+    const int64_t x = race_index(rows[i]);
+    if (x < 0 || x != p.tokens[(int64_t)b * p.tok_b + i]) at = min(at, i);
   }
-  __syncthreads();
-  const int at = s_at;
-  for (int i = threadIdx.x; i < at; i += kThreads) p.accept_prob[b * p.K + i] = 1.f;
-  if (threadIdx.x == 0 && at < n_draft) p.accept_prob[b * p.K + at] = 0.f;
-  const unsigned long long x = rows[at];
-  __syncthreads();
-  write_out(p, b, at, x == 0 ? -1 : (int64_t)(0xffffffffu - (uint32_t)x), p.K + 1);
+  at = __reduce_min_sync(~0u, at);
+  for (int i = lane; i < at; i += 32) p.accept_prob[b * p.K + i] = 1.f;
+  if (lane == 0 && at < n_draft) p.accept_prob[b * p.K + at] = 0.f;
+  const int64_t token = race_index(rows[at]);
+  __syncwarp();
+  write_out(p, b, at, token, p.K + 1);
 }
 
 // ------------------------------------------------------------------- host
 struct Plan {
-  int un, chunks, race_chunks;
+  int segments, seg_blocks, race_segments, race_blocks;
   bool skip;
   size_t zeroed, scratch;
 };
@@ -492,42 +535,47 @@ static int plan_of(const kvr_verify_args* a, Plan* out) {
     return KVR_ERR_INVALID_ARGUMENT;
   if (a->dtype < 0 || a->dtype > 2) return KVR_ERR_UNSUPPORTED;
   if (a->temperature > 0.f && a->temperature < FLT_MIN) return KVR_ERR_UNSUPPORTED;   // its reciprocal may overflow
-  if (a->draft_tokens > 4095 || (int64_t)a->batch * (a->draft_tokens + 1) > (1 << 24)) return KVR_ERR_UNSUPPORTED;
+  if (a->vocab > (1 << 30) || a->draft_tokens > 4095 || (int64_t)a->batch * (a->draft_tokens + 1) > (1 << 24))
+    return KVR_ERR_UNSUPPORTED;
   const int n = a->dtype == 2 ? 4 : 8;
   const int64_t blocks = (a->vocab + n - 1) / n;
-  const int64_t rows = std::max<int64_t>(1, (int64_t)a->batch * (a->draft_tokens + (a->temperature > 0.f ? 0 : 1)));
+  const bool greedy = a->temperature == 0.f;
+  const int64_t rows = std::max<int64_t>(1, (int64_t)a->batch * (greedy ? a->draft_tokens + 1 : 2 * a->draft_tokens));
   Plan p;
-  // 4 blocks of a row to a thread keep the registers at 64 (four CTAs per SM); fewer where that fills the GPU
-  p.un = 4;
-  for (; p.un > 1; p.un /= 2)
-    if (rows * ((blocks + p.un * kThreads - 1) / (p.un * kThreads)) >= 296) break;
-  p.chunks = (int)((blocks + p.un * kThreads - 1) / (p.un * kThreads));
-  if (rows * p.chunks > (1ll << 31) - 1) return KVR_ERR_UNSUPPORTED;
-  // Looking for an earlier refusal costs every CTA a round trip to L2 and saves reading: not for logits that
+  // A warp's segment: at most 4 steps of kUnroll blocks a lane (longer ones are under way when their sequence is
+  // refused, shorter ones spend more of their time on the count: 64 x 5 of 128K took 51, 48, 45.5, 46, 52 us with 2,
+  // 3, 4, 8, 16), fewer while they leave warps out (32 on each of 148 SMs).
+  p.seg_blocks = 4 * 32 * kUnroll;
+  while (p.seg_blocks > 32 * kUnroll && rows * ((blocks + p.seg_blocks - 1) / p.seg_blocks) < 148 * 32) p.seg_blocks /= 2;
+  p.segments = (int)((blocks + p.seg_blocks - 1) / p.seg_blocks);
+  p.race_blocks = 8 * 32;   // 8 blocks a lane: 2, 4, 16, 32 took 7, 2, 4 and 16 us longer on the same
+  while (p.race_blocks > 32 * kRaceUnroll &&
+         (int64_t)a->batch * ((blocks + p.race_blocks - 1) / p.race_blocks) < 148 * 32)
+    p.race_blocks /= 2;
+  p.race_segments = (int)((blocks + p.race_blocks - 1) / p.race_blocks);
+  if (rows * p.segments > (1ll << 31) - 1 || (int64_t)a->batch * p.race_segments > (1ll << 31) - 1)
+    return KVR_ERR_UNSUPPORTED;
+  // Looking for an earlier refusal costs every warp a round trip to L2 and saves reading: not for logits that
   // 5 us read anyway.
   p.skip = rows * a->vocab * (a->dtype == 2 ? 4 : 2) > (32 << 20);
-  p.race_chunks = (int)((blocks + kRaceBlocks * kThreads - 1) / (kRaceBlocks * kThreads));
-  if ((int64_t)a->batch * p.race_chunks > (1ll << 31) - 1) return KVR_ERR_UNSUPPORTED;
   const size_t B = a->batch, K1 = a->draft_tokens + 1;
   p.zeroed = B * K1 * 8 + B * K1 * 4 + 2 * B * 4;
-  p.scratch = B * (K1 - 1) * ((size_t)p.chunks + 1) * sizeof(float4);
+  p.scratch = greedy ? 0 : B * (K1 - 1) * (sizeof(float4) + 2 * (size_t)p.segments * sizeof(float2));
   *out = p;
   return KVR_OK;
 }
 
 template <typename T>
-static cudaError_t launch(const Params& p, const Plan& pl, bool greedy, cudaStream_t s) {
-  auto grid = [&](int rows) { return dim3((unsigned)((int64_t)rows * p.B * pl.chunks)); };
-  if (greedy) {
-    auto kern = pl.un == 4 ? greedy_kernel<T, 4> : pl.un == 2 ? greedy_kernel<T, 2> : greedy_kernel<T, 1>;
-    return pdl_launch(kern, grid(p.K + 1), dim3(kThreads), 0, s, 1, p);
-  }
+static cudaError_t launch(const Params& p, bool greedy, cudaStream_t s) {
+  auto grid = [](int64_t warps) { return dim3((unsigned)((warps + kWarps - 1) / kWarps)); };
+  if (greedy)
+    return pdl_launch(greedy_kernel<T>, dim3((unsigned)((int64_t)p.B * (p.K + 1) * ((p.segments + kWarps - 1) / kWarps))),
+                      dim3(kThreads), 0, s, 1, p);
   if (p.K > 0) {
-    auto kern = pl.un == 4 ? stats_kernel<T, 4> : pl.un == 2 ? stats_kernel<T, 2> : stats_kernel<T, 1>;
-    cudaError_t e = pdl_launch(kern, grid(p.K), dim3(kThreads), 0, s, 1, p);
+    const cudaError_t e = pdl_launch(stats_kernel<T>, grid(2ll * p.B * p.K * p.segments), dim3(kThreads), 0, s, 1, p);
     if (e != cudaSuccess) return e;
   }
-  return pdl_launch(race_kernel<T>, dim3((unsigned)((int64_t)p.B * pl.race_chunks)), dim3(kThreads), 0, s, 1, p);
+  return pdl_launch(race_kernel<T>, grid((int64_t)p.B * p.race_segments), dim3(kThreads), 0, s, 1, p);
 }
 
 }  // namespace verify
@@ -564,7 +612,9 @@ extern "C" int kvr_verify(const kvr_verify_args* a, kvr_stream_t stream) {
   p.noise = a->noise; p.n_b = a->noise_b_stride;
   p.draft_lengths = a->draft_lengths;
   p.out_tokens = a->out_tokens; p.accepted = a->accepted; p.accept_prob = a->accept_prob;
-  p.B = a->batch; p.K = K; p.V = a->vocab; p.chunks = pl.chunks; p.race_chunks = pl.race_chunks;
+  p.B = a->batch; p.K = K; p.V = a->vocab; 
+  p.segments = pl.segments; p.seg_blocks = pl.seg_blocks;
+  p.race_segments = pl.race_segments; p.race_blocks = pl.race_blocks;
   p.skip = pl.skip;
   p.c = greedy ? 1.f : 1.4426950408889634f / a->temperature;
   const size_t rows = (size_t)p.B * (K + 1);
@@ -573,11 +623,11 @@ extern "C" int kvr_verify(const kvr_verify_args* a, kvr_stream_t stream) {
   p.done = p.arrived + rows;
   p.refused = p.done + p.B;
   p.stats = static_cast<float4*>(a->workspace);
-  p.part = p.stats + (size_t)p.B * K;
+  p.part = reinterpret_cast<float2*>(p.stats + (size_t)p.B * K);
   cudaStream_t s = as_stream(stream);
-  const cudaError_t e = a->dtype == 0   ? verify::launch<__nv_bfloat16>(p, pl, greedy, s)
-                        : a->dtype == 1 ? verify::launch<__half>(p, pl, greedy, s)
-                                        : verify::launch<float>(p, pl, greedy, s);
+  const cudaError_t e = a->dtype == 0   ? verify::launch<__nv_bfloat16>(p, greedy, s)
+                        : a->dtype == 1 ? verify::launch<__half>(p, greedy, s)
+                                        : verify::launch<float>(p, greedy, s);
   if (e != cudaSuccess) { set_last_cuda_error(e); return KVR_ERR_CUDA; }
   return KVR_OK;
 }
