@@ -21,6 +21,17 @@ CUDA graphs with the library kernels as opaque nodes.
         geom, key_scale_pairs=None) -> out
                               packed_review.py:23-31 + :78 on a streaming layer
     kvr::lse_merge(part_ml, part_o) -> out           (cross-GPU partial merge)
+    kvr::paged_append(key, value, key_pages, value_pages, block_table, lengths)
+    kvr::paged_attention(query, key_pages, value_pages, block_table, lengths,
+        scale=None, window=0, sinks=0, token_weights=None, return_lse=False)
+        -> (out, lse)
+    kvr::paged_evict(key_pages, value_pages, block_table, lengths,
+        token_weights, new_block_table, keep, recent, first)
+        -> (kept, new_lengths, new_weights)
+    kvr::verify_draft(target_logits, draft_logits, draft_tokens, uniforms,
+        noise, temperature=1.0, draft_lengths=None)
+        -> (tokens, accepted, accept_prob)   (the paged and the verification
+        operators have no reference counterpart)
 
 Import this module to register them.
 """
@@ -61,6 +72,33 @@ def _(query, k_new, v_new, key_payload, key_scale, key_offset, key_residual, val
 @torch.library.register_fake("kvr::lse_merge")
 def _(part_ml, part_o):
     return part_o.new_empty((int(part_o.shape[1]), int(part_o.shape[2])), dtype=torch.bfloat16)
+
+
+@torch.library.register_fake("kvr::paged_append")
+def _(key, value, key_pages, value_pages, block_table, lengths):
+    return None
+
+
+@torch.library.register_fake("kvr::paged_attention")
+def _(query, key_pages, value_pages, block_table, lengths, scale=None, window=0, sinks=0, token_weights=None,
+      return_lse=False):
+    lse = query.new_empty(query.shape[:3] if return_lse else (0,), dtype=torch.float32)
+    return query.new_empty(query.shape), lse
+
+
+@torch.library.register_fake("kvr::paged_evict")
+def _(key_pages, value_pages, block_table, lengths, token_weights, new_block_table, keep, recent, first):
+    batch = block_table.shape[0]
+    return (lengths.new_empty((batch, keep)), lengths.new_empty((batch,)),
+            token_weights.new_empty((batch, keep)))
+
+
+@torch.library.register_fake("kvr::verify_draft")
+def _(target_logits, draft_logits, draft_tokens, uniforms, noise, temperature=1.0, draft_lengths=None):
+    batch, draft = target_logits.shape[0], target_logits.shape[1] - 1
+    return (target_logits.new_empty((batch, draft + 1), dtype=torch.int64),
+            target_logits.new_empty((batch,), dtype=torch.int32),
+            target_logits.new_empty((batch, draft), dtype=torch.float32))
 
 
 @torch.library.custom_op("kvr::pack_per_token", mutates_args=())

@@ -18,7 +18,7 @@ captured in a CUDA graph.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple, Union
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -114,3 +114,132 @@ def paged_evict(
     if _evict_op is None:
         _bind_ops()
     return _evict_op(key_pages, value_pages, block_table, lengths, token_weights, new_block_table, keep, recent, first)
+
+
+class PagedKVCache:
+    """A model's key-value cache in pages: pools for every layer, one block
+    table and one set of lengths for all of them.
+
+    The host keeps the lengths too, to hand out and take back pages; a step is
+
+        cache.advance(T)                      # once: pages and lengths for T more tokens
+        cache.append(layer, k, v)             # every layer: [batch, kv_heads, T, head_dim]
+        out = cache.attention(layer, q)       # [batch, query_heads, T, head_dim]
+        cache.crop(lengths)                   # after a verification: each sequence to its own length
+
+    With ``track_weights`` the attention adds up what weight every token got
+    (per layer), and ``evict`` brings the sequences down to a budget by it.
+    """
+
+    def __init__(self, num_layers: int, batch: int, kv_heads: int, head_dim: int, *, num_pages: int,
+                 page_size: int = 16, max_pages: Optional[int] = None, dtype: torch.dtype = torch.bfloat16,
+                 device: torch.device | str = "cuda", track_weights: bool = False) -> None:
+        if min(num_layers, batch, kv_heads, head_dim, num_pages, page_size) <= 0:
+            raise ValueError("num_layers, batch, kv_heads, head_dim, num_pages and page_size must be positive.")
+        self.batch, self.page_size, self.num_pages = int(batch), int(page_size), int(num_pages)
+        # a sequence's share of the block table (default: all pages could be one sequence's)
+        self.max_pages = int(max_pages or num_pages)
+        self.device = torch.device(device)
+        shape = (self.num_pages, kv_heads, self.page_size, head_dim)
+        self.key_pages = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(num_layers)]
+        self.value_pages = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(num_layers)]
+        self.block_table = torch.full((self.batch, self.max_pages), -1, dtype=torch.int32, device=self.device)
+        self.lengths = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
+        self.token_weights: Optional[List[torch.Tensor]] = None
+        if track_weights:
+            self.token_weights = [torch.zeros(self.batch, self.max_pages * self.page_size, device=self.device)
+                                  for _ in range(num_layers)]
+        self._free = list(range(self.num_pages - 1, -1, -1))
+        self._pages: List[List[int]] = [[] for _ in range(self.batch)]
+        self._lengths = [0] * self.batch
+
+    # ------------------------------------------------------------- lengths
+    def get_seq_length(self) -> int:
+        """Tokens of the longest sequence."""
+        return max(self._lengths)
+
+    def seq_lengths(self) -> List[int]:
+        return list(self._lengths)
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _upload(self, table: bool) -> None:
+        if table:
+            rows = [p + [-1] * (self.max_pages - len(p)) for p in self._pages]
+            self.block_table.copy_(torch.tensor(rows, dtype=torch.int32))
+        self.lengths.copy_(torch.tensor(self._lengths, dtype=torch.int32))
+
+    def advance(self, tokens: Union[int, Sequence[int]]) -> None:
+        """Lengthen the sequences (by one number, or one each) and give them
+        pages; the rows are written by ``append``."""
+        more = [int(tokens)] * self.batch if isinstance(tokens, int) else [int(t) for t in tokens]
+        if len(more) != self.batch or min(more) < 0:
+            raise ValueError(f"advance needs a number of tokens >= 0 for each of {self.batch} sequences.")
+        need = [-(-(n + m) // self.page_size) - len(p) for n, m, p in zip(self._lengths, more, self._pages)]
+        if sum(max(n, 0) for n in need) > len(self._free):
+            raise ValueError("not enough free pages: crop, evict or make the cache with more.")
+        if any(len(p) + n > self.max_pages for p, n in zip(self._pages, need)):
+            raise ValueError("a sequence needs more than max_pages pages.")
+        for pages, n in zip(self._pages, need):
+            pages.extend(self._free.pop() for _ in range(n))
+        self._lengths = [n + m for n, m in zip(self._lengths, more)]
+        self._upload(any(n > 0 for n in need))
+
+    def crop(self, lengths: Union[int, Sequence[int]]) -> None:
+        """Roll every sequence back to its length; pages behind it are free again."""
+        to = [min(int(lengths), n) for n in self._lengths] if isinstance(lengths, int) else [int(n) for n in lengths]
+        if len(to) != self.batch or any(not 0 <= t <= n for t, n in zip(to, self._lengths)):
+            raise ValueError(f"crop needs a length within each of the {self.batch} sequences.")
+        freed = False
+        for b, t in enumerate(to):
+            keep = -(-t // self.page_size)
+            freed |= keep < len(self._pages[b])
+            self._free.extend(reversed(self._pages[b][keep:]))
+            del self._pages[b][keep:]
+            if self.token_weights is not None and t < self._lengths[b]:
+                for w in self.token_weights:
+                    w[b, t:self._lengths[b]] = 0
+        self._lengths = to
+        self._upload(freed)
+
+    # ---------------------------------------------------------- operations
+    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
+        """Write the tokens that ``advance`` made room for."""
+        paged_append(key, value, self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths)
+
+    def attention(self, layer: int, query: torch.Tensor, *, scale: Optional[float] = None, window: int = 0,
+                  sinks: int = 0) -> torch.Tensor:
+        weights = None if self.token_weights is None else self.token_weights[layer]
+        return paged_decode_attention(query, self.key_pages[layer], self.value_pages[layer], self.block_table,
+                                      self.lengths, scale=scale, window=window, sinks=sinks, token_weights=weights)
+
+    def evict(self, keep: int, *, recent: int = 0, first: int = 0) -> bool:
+        """Bring every sequence down to ``keep`` tokens (see ``paged_evict``),
+        each layer by its own weights; the rows move to fresh pages.  False,
+        and nothing done, while no sequence is longer."""
+        if self.token_weights is None:
+            raise ValueError("evict needs a cache made with track_weights=True.")
+        if keep <= 0 or recent < 0 or first < 0 or first + recent > keep:
+            raise ValueError("keep must be positive and hold first + recent tokens.")
+        if max(self._lengths) <= keep:
+            return False
+        left = [min(n, keep) for n in self._lengths]
+        need = [-(-n // self.page_size) for n in left]
+        if sum(need) > len(self._free):
+            raise ValueError("not enough free pages to evict into.")
+        fresh = [[self._free.pop() for _ in range(n)] for n in need]
+        width = -(-min(keep, self.max_pages * self.page_size) // self.page_size)
+        rows = [p + [-1] * (width - len(p)) for p in fresh]
+        new_table = torch.tensor(rows, dtype=torch.int32).to(self.device)
+        for layer, weights in enumerate(self.token_weights):
+            _, _, kept = paged_evict(self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths,
+                                     weights, new_table, keep=keep, recent=recent, first=first)
+            n = min(keep, weights.shape[1])
+            weights.zero_()
+            weights[:, :n].copy_(kept[:, :n])
+        for pages in self._pages:
+            self._free.extend(reversed(pages))
+        self._pages, self._lengths = fresh, left
+        self._upload(True)
+        return True
