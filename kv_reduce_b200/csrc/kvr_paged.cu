@@ -10,19 +10,24 @@
 //
 // What bounds it: the bytes of K and V.  A token of one KV head is 4*D bytes
 // and 4*D*R operations for the R = T*q_heads/kv_heads query rows that share
-// it, so R operations per byte, far below the tensor cores' rate for the few
-// rows of a decode step.  The kernel is therefore laid out around keeping
-// loads in flight and the instructions per tile few:
+// it, so R operations per byte, below what the tensor cores do; but the
+// softmax between the two products has to keep up as well, and the loads must
+// never pause.  So the threads do as little per tile as they can:
 //  * Work is a flat list of token tiles (sequence, KV head, row tile, tile),
 //    cut into equal ranges, one per CTA.  Lengths are read on the device, so
 //    a ragged batch is balanced to one tile without the host knowing it.
-//  * A producer warp looks up pages and fills a ring of tiles, on across
-//    sequence boundaries; four consumer warps compute.  Pages of a multiple
-//    of 8 tokens come by TMA, a box per page; others row by row (cp.async).
-//  * The consumers share each tile: for the scores a warp owns a quarter of
-//    the tokens, for the output a quarter of the head dimension, so every
-//    byte of K and V is read from shared memory once and the accumulator is
-//    complete in the CTA: nothing is merged between warps.
+//  * One warp looks up pages and fills a ring of K and V tiles, on across
+//    sequence boundaries.  Pages of a multiple of 8 tokens come by TMA, a box
+//    per page; others row by row (cp.async).
+//  * One thread issues the products (tcgen05).  Both are transposed: scores^T
+//    = K Q^T has a tile's 128 tokens in the 128 lanes of tensor memory and
+//    only as many columns as there are rows, and output^T = V^T P^T the head
+//    dimension; so no lane is spent on padding the few query rows to 128, K
+//    and V are read where the copies put them, and a thread of the four
+//    softmax warps has one token and every row: R exponentials a tile.
+//  * The next tile's scores are computed while this one's softmax runs.  The
+//    output stays in tensor memory; it is read back to be rescaled only in
+//    the tiles where a row's maximum moves.
 //  * A sequence that several CTAs share is joined by the last of them to
 //    arrive, in the order of the CTAs: the result does not depend on timing.
 #include "kvr_ring.cuh"
@@ -39,19 +44,13 @@ using namespace ring;
 
 constexpr int kWarps = 4;                     // consumers
 constexpr int kConsumers = 32 * kWarps;
-constexpr int kThreads = kConsumers + 32;     // and the producer warp
+constexpr int kLoadWarp = 4, kMmaWarp = 5;
+constexpr int kThreads = kConsumers + 64;
 constexpr int kGroup = 16;                    // CTAs a join takes at a time
 
 // Rows that no mask leaves anything to keep m = -inf; 0 stands in for it
 // wherever it would be subtracted.
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
-
-template <bool HALF>
-__device__ __forceinline__ void mma_e(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                      uint32_t b1) {
-  if constexpr (HALF) mma_f16(d, a0, a1, a2, a3, b0, b1);
-  else mma_bf16(d, a0, a1, a2, a3, b0, b1);
-}
 
 template <bool HALF>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -65,12 +64,6 @@ template <bool HALF>
 __device__ __forceinline__ float to_float(uint16_t w) {
   if constexpr (HALF) return __half2float(__ushort_as_half(w));
   else return bf16_bits_to_f32(w);
-}
-
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
 }
 
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;\n" ::: "memory"); }
@@ -103,47 +96,63 @@ struct Params {
   int64_t score_stride;
   int B, HQ, HKV, T, G, R, row_tiles, window, sinks, cap;
   float scale2;     // scale * log2(e)
-  int ctas, min_tiles;
+  int ctas;
   float* part_o;    // [3 * ctas][ROWS][D]: two parts of each CTA, group sums
   float* part_ml;   // [3 * ctas][ROWS][2]
   int* counters;    // [2 * ctas], zero on entry and on exit
   int box;          // tokens of a TMA box
 };
 
-template <int D, int MT>
+template <int D, int N>
 struct Cfg {
-  static constexpr int TILE = D == 64 ? 128 : 64;   // tokens: 16 KB of K and 16 KB of V either way
-  static constexpr int ROWS = 16 * MT;
+  static constexpr int TILE = 128;                   // tokens: the 128 lanes of a score tile
   static constexpr int HALVES = D / 64;
   static constexpr int PIECES = D / 8;
-  static constexpr int HALF_BYTES = TILE * 128;     // 64 elements of every token, 128-byte rows
-  static constexpr int KV_BYTES = HALVES * HALF_BYTES;
-  static constexpr int STAGE = 2 * KV_BYTES;
-  static constexpr int STAGES = MT == 4 ? 2 : 3;    // two CTAs per SM in every case
-  static constexpr int NT = TILE / kWarps / 8;      // 8-token score tiles of a warp
-  static constexpr int DW = D / kWarps;             // output columns of a warp
-  static constexpr int DT = DW / 8;
-  // shared memory: ring, Q (MT <= 2 keeps it in registers and lets P take its place), P, descriptors, row
-  // statistics, barriers
-  static constexpr int Q_BYTES = ROWS * D * 2, P_HALF = ROWS * TILE * 2, P_BYTES = 2 * P_HALF;
-  static constexpr int OFF_Q = STAGES * STAGE;
-  static constexpr int OFF_P = MT <= 2 ? OFF_Q : OFF_Q + Q_BYTES;
-  static constexpr int OFF_DESC = OFF_Q + (MT <= 2 ? (Q_BYTES > P_BYTES ? Q_BYTES : P_BYTES) : Q_BYTES + P_BYTES);
-  static constexpr int OFF_MAX = OFF_DESC + STAGES * 64;
-  static constexpr int OFF_SUM = OFF_MAX + kWarps * ROWS * 4;
-  static constexpr int OFF_BAR = OFF_SUM + kWarps * ROWS * 4;
-  static constexpr int OFF_MISC = OFF_BAR + 3 * STAGES * 8;
-  static constexpr int SMEM = OFF_MISC + 64 + 1024;   // 1 KB to align the ring
+  static constexpr int HALF_BYTES = TILE * 128;      // 64 elements of every token, 128-byte rows
+  static constexpr int UNIT = HALVES * HALF_BYTES;   // K or V of a tile
+  static constexpr int Q_BYTES = N * D * 2;
+  static constexpr int P_ROW = N == 16 ? 64 : 128;          // bytes of a token's weights (a swizzle row)
+  static constexpr int P_BYTES = TILE * 4 * N;
+  // Two CTAs per SM where the ring still holds three units or more; else one with a longer ring.
+  static constexpr int CTAS = N == 16 || (N == 32 && D == 64) ? 2 : 1;
+  static constexpr int UNITS = CTAS == 2 ? (D == 128 ? 3 : N == 16 ? 6 : 5) : (D == 128 ? (N == 32 ? 6 : 5) : 8);
+  static constexpr int DESCS = 8;
+  static constexpr int OFF_Q = UNITS * UNIT;
+  static constexpr int OFF_P = OFF_Q + Q_BYTES;
+  static constexpr int OFF_DESC = OFF_P + P_BYTES;
+  static constexpr int OFF_ROWS = OFF_DESC + DESCS * 64;   // float [12][N]: reference, alpha, position, row, 4 maxima, 4 sums
+  static constexpr int OFF_BAR = OFF_ROWS + 12 * N * 4;
+  static constexpr int BARS = 2 * UNITS + DESCS + 4 + 3;
+  static constexpr int OFF_MISC = OFF_BAR + BARS * 8;
+  static constexpr int SMEM = OFF_MISC + 80 + 1024;        // 1 KB to align the ring
+  static constexpr int TMEM = 4 * N;                       // columns: two score tiles, output and its rest
+
+  // Weight of (token t, row r), rounded (part 0) or its rest (part 1): token-major, the two parts side by side.
+  static __device__ __forceinline__ int p_at(int t, int r, int part) {
+    const int piece = (N == 64 ? 0 : part * (N / 8)) + (r >> 3);
+    return (N == 64 ? part * TILE * 128 : 0) + t * P_ROW + ((piece ^ (N == 16 ? (t >> 1) & 3 : t & 7)) << 4) + (r & 7) * 2;
+  }
 };
 
+// The reference of a row that no token has been seen by: far below any score.
+constexpr float kUnseen = -1e30f;
+
 struct Desc {
-  int b, h, rt, token0, len, first, last, n_tiles;
-  int seg_start;
+  int first, last, full, token0;   // full: every row sees every token
+  int b, h, rt, len;
+  int n_tiles, seg_start;          // of the segment: tiles, flat index of the first
+  int whole;                       // with `last`: all of the segment's tiles are this CTA's
   uint32_t bad[4];   // tokens on pages outside the pool, a bit each
 };
 static_assert(sizeof(Desc) <= 64, "");
 
-// `total` tiles cut into `n` ranges of equal size, the first ones a tile longer.
+// The flat list counts a segment as its tiles and kHead more in front: what it
+// costs beside its tiles (its queries, a first tile without a reference, its
+// output or part, the join), so that a CTA does not end up with many short
+// ones.
+constexpr int kHead = 2;
+
+// `total` units cut into `n` ranges of equal size, the first ones a unit longer.
 struct Cut {
   int q, r;
   __device__ __forceinline__ Cut(int total, int n) : q(total / n), r(total % n) {}
@@ -156,56 +165,176 @@ struct Cut {
 struct Span {
   int n, ns, lo_tile, lo;
 };
-template <int TILE>
+constexpr int kTile = 128;
 __device__ __forceinline__ Span span_of(const Params& p, int len) {
   Span s;
-  const int total = (len + TILE - 1) / TILE;
+  const int total = (len + kTile - 1) / kTile;
   s.lo = p.window > 0 ? max(0, max(len - p.T, 0) - p.window + 1) : 0;
-  s.lo_tile = min(s.lo / TILE, max(total - 1, 0));
-  s.ns = min((p.sinks + TILE - 1) / TILE, s.lo_tile);
+  s.lo_tile = min(s.lo / kTile, max(total - 1, 0));
+  s.ns = min((p.sinks + kTile - 1) / kTile, s.lo_tile);
   s.n = max(1, s.ns + total - s.lo_tile);   // an empty sequence gets one tile, to write its zero rows
   return s;
 }
 __device__ __forceinline__ int length_of(const Params& p, int b) { return min(max(p.lengths[b], 0), p.cap); }
 
-template <bool HALF, int D, int MT, bool TMA>
-__global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_constant__ Params p,
-                                                                const __grid_constant__ CUtensorMap kmap,
-                                                                const __grid_constant__ CUtensorMap vmap) {
-  using C = Cfg<D, MT>;
-  constexpr int TILE = C::TILE, ROWS = C::ROWS, S = C::STAGES;
+// ---- tensor memory and the 5th-generation tensor cores
+// Shared-memory operand in rows of 128 (or 64) bytes with the swizzle of that
+// width, patterns of 8 rows.  The rows are the operand's own (K-major) or its
+// depth (transposed); `next`: bytes to the next row's width of elements of a
+// transposed operand.
+template <int ROW = 128>
+__device__ __forceinline__ uint64_t operand(uint32_t addr, int next) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((next >> 4) & 0x3fff) << 16 | (uint64_t)(8 * ROW >> 4) << 32 |
+         1ull << 46 | (ROW == 128 ? 2ull : 4ull) << 61;
+}
+// bf16 or fp16 operands, fp32 accumulation, M x N, both operands transposed or neither.
+__device__ __forceinline__ constexpr uint32_t mma_kind(bool half, int m, int n, bool transposed) {
+  return 1u << 4 | (half ? 0u : 1u) << 7 | (half ? 0u : 1u) << 10 | (transposed ? 3u : 0u) << 15 |
+         (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool add) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(kind), "r"((uint32_t)add)
+      : "memory");
+}
+// The barrier is arrived at when all tensor-core work issued so far is done.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+// 16 columns of this warp's 32 lanes, a lane to a thread.
+__device__ __forceinline__ void tmem_load(uint32_t addr, float* x) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];\n"
+      : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]),
+        "=f"(x[9]), "=f"(x[10]), "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const float* x) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15};\n" ::"f"(x[0]),
+      "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]), "f"(x[8]), "f"(x[9]), "f"(x[10]),
+      "f"(x[11]), "f"(x[12]), "f"(x[13]), "f"(x[14]), "f"(x[15]), "r"(addr)
+      : "memory");
+}
+// (the registers are named so that nothing reads them before the wait)
+__device__ __forceinline__ void tmem_wait_load(float* x) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3]), "+f"(x[4]), "+f"(x[5]), "+f"(x[6]), "+f"(x[7]), "+f"(x[8]),
+                 "+f"(x[9]), "+f"(x[10]), "+f"(x[11]), "+f"(x[12]), "+f"(x[13]), "+f"(x[14]), "+f"(x[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+// Maxima or sums of NR rows over the warp's lanes, halving the rows a lane
+// deals with at every exchange: NR - 1 exchanges and a few instead of 5 NR.
+// Row r ends in lane r 32 / NR (NR = 64: rows 2 l and 2 l + 1 in lane l).
+template <int NR, int BIT, bool SUM>
+__device__ __forceinline__ void rows_join(float* v, int lane) {
+  if constexpr (BIT >= 1) {
+    if constexpr (NR > 1) {
+      const bool up = lane & BIT;
+#pragma unroll
+      for (int k = 0; k < NR / 2; ++k) {
+        const float mine = up ? v[k + NR / 2] : v[k], other = up ? v[k] : v[k + NR / 2];
+        const float got = __shfl_xor_sync(0xffffffffu, other, BIT);
+        v[k] = SUM ? mine + got : fmaxf(mine, got);
+      }
+      rows_join<NR / 2, BIT / 2, SUM>(v, lane);
+    } else {
+      const float got = __shfl_xor_sync(0xffffffffu, v[0], BIT);
+      v[0] = SUM ? v[0] + got : fmaxf(v[0], got);
+      rows_join<1, BIT / 2, SUM>(v, lane);
+    }
+  }
+}
+// ... written to `to` (v is used up).
+template <int NR, bool SUM>
+__device__ __forceinline__ void store_rows(float* v, float* to, int lane) {
+  rows_join<NR, 16, SUM>(v, lane);
+  if constexpr (NR >= 32) {
+#pragma unroll
+    for (int k = 0; k < NR / 32; ++k) to[lane * (NR / 32) + k] = v[k];
+  } else {
+    constexpr int SHIFT = NR == 16 ? 1 : 2;
+    if ((lane & ((1 << SHIFT) - 1)) == 0) to[lane >> SHIFT] = v[0];
+  }
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
+// Barrier of the consumers; true for all when it is for one.
+__device__ __forceinline__ bool consumer_any(bool x) {
+  int r;
+  asm volatile("{\n.reg .pred a, b;\nsetp.ne.s32 a, %1, 0;\nbar.red.or.pred b, 1, 128, a;\nselp.s32 %0, 1, 0, b;\n}\n"
+               : "=r"(r)
+               : "r"((int)x)
+               : "memory");
+  return r != 0;
+}
+
+template <bool HALF, int D, int N, bool TMA>
+__global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(const __grid_constant__ Params p,
+                                                                              const __grid_constant__ CUtensorMap kmap,
+                                                                              const __grid_constant__ CUtensorMap vmap) {
+  using C = Cfg<D, N>;
+  constexpr int TILE = C::TILE, U = C::UNITS, ROWS = N;
   extern __shared__ uint8_t raw_smem[];
   // the swizzle pattern of a tile follows address bits 7..9: align the ring to 1 KB
   uint8_t* smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
   const uint32_t sbase = smem_u32(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  Desc* descs = reinterpret_cast<Desc*>(smem + C::OFF_DESC);
-  float* smax = reinterpret_cast<float*>(smem + C::OFF_MAX);
-  float* ssum = reinterpret_cast<float*>(smem + C::OFF_SUM);
-  // a slot's data is there / is read / its descriptor is there (before the data)
-  const uint32_t full = sbase + C::OFF_BAR, empty = full + S * 8, ready = empty + S * 8;
-  int* s_start = reinterpret_cast<int*>(smem + C::OFF_MISC);   // [3]
-  int* s_scan = s_start + 4;                                   // [kThreads / 32]
+  auto desc_at = [&](int i) { return reinterpret_cast<Desc*>(smem + C::OFF_DESC + (i & (C::DESCS - 1)) * 64); };
+  float* mu_s = reinterpret_cast<float*>(smem + C::OFF_ROWS);   // references of the rows' exponents
+  float* alpha_s = mu_s + N;
+  int* pos_s = reinterpret_cast<int*>(alpha_s + N);
+  int* row_s = pos_s + N;          // the rows of the output
+  float* smax = alpha_s + 3 * N;   // [4][N]
+  float* ssum = smax + 4 * N;      // [4][N]
+  // A ring unit's data is there / is read; a tile's descriptor is there (before its data); score tile done / read;
+  // P written; the output up to a tile done; a segment's queries written.
+  const uint32_t full = sbase + C::OFF_BAR, empty = full + 8 * U, ready = empty + 8 * U, s_full = ready + 8 * C::DESCS,
+                 s_empty = s_full + 16, p_full = s_empty + 16, o_done = p_full + 8, q_full = o_done + 8;
+  int* s_start = reinterpret_cast<int*>(smem + C::OFF_MISC);   // [7]
+  int* s_scan = s_start + 8;                                   // [kThreads / 32]
   int* s_last = s_scan + kThreads / 32;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_last + 1);
+  int* s_add = s_last + 2;                                     // the output holds something before its first product
 
   if (tid == 0) {
-    for (int i = 0; i < S; ++i) {
-      bar_init(full + 8 * i, TMA ? 1 : 33);
-      bar_init(empty + 8 * i, kWarps);
-      bar_init(ready + 8 * i, 1);
+    for (int i = 0; i < U; ++i) {
+      bar_init(full + 8 * i, 1);
+      bar_init(empty + 8 * i, 1);
     }
+    for (int i = 0; i < C::DESCS; ++i) bar_init(ready + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(s_full + 8 * i, 1);
+      bar_init(s_empty + 8 * i, kWarps);
+    }
+    bar_init(p_full, kWarps);
+    bar_init(o_done, 1);
+    bar_init(q_full, 1);
     bar_init_fence();
   }
   pdl_wait();
 
   // ---- this CTA's range of the flat tile list
   const int HR = p.HKV * p.row_tiles;
-  int total, ctas, g0, count;   // tiles in all, CTAs that take part, this one's first tile and how many
+  int total, ctas, g0, count;   // units in all, CTAs that take part, this one's first unit, and its tiles
   {
     const int per = (p.B + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += span_of<TILE>(p, length_of(p, b)).n;
+    for (int b = b0; b < b1; ++b) mine += span_of(p, length_of(p, b)).n + kHead;
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -222,42 +351,116 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
       total += s_scan[w];
     }
     total *= HR;
-    ctas = min(p.ctas, max(1, total / p.min_tiles));
+    ctas = min(p.ctas, total);
     const int me = blockIdx.x;
     if (me >= ctas) return;
     const Cut cut(total, ctas);
     g0 = cut.begin(me);
-    count = cut.begin(me + 1) - g0;
-    // the thread whose sequences hold tile g0 finds the sequence
-    if (mine > 0 && before * HR <= g0 && g0 < (before + mine) * HR) {
-      int b = b0;
-      if (per > 1)
-        for (;; ++b) {
-          const int nb = span_of<TILE>(p, length_of(p, b)).n;
-          if (g0 < (before + nb) * HR) break;
-          before += nb;
+    const int g1 = cut.begin(me + 1);
+    // the threads whose sequences hold units g0 and g1 find the sequences
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const int g = which ? g1 : g0;
+      if (mine > 0 && before * HR <= g && g < (before + mine) * HR) {
+        int b = b0, at = before;
+        int raw = p.lengths[b];
+        int nb = span_of(p, min(max(raw, 0), p.cap)).n + kHead;
+        while (g >= (at + nb) * HR) {
+          at += nb;
+          raw = p.lengths[++b];
+          nb = span_of(p, min(max(raw, 0), p.cap)).n + kHead;
         }
-      s_start[0] = b;
-      s_start[1] = before;
-      s_start[2] = p.lengths[b];
+        const int off = g - at * HR, hr = off / nb, in_seg = off - hr * nb;
+        // tiles in front of unit g: those units less the heads in front
+        const int tiles = g - kHead * (b * HR + hr) - min(in_seg, kHead);
+        if (which) {
+          s_start[6] = tiles;
+        } else {
+          s_start[0] = b;
+          s_start[1] = raw;
+          s_start[2] = hr;
+          s_start[3] = max(in_seg - kHead, 0);
+          s_start[4] = tiles;
+        }
+      }
     }
+    if (tid == 0 && g1 == total) s_start[6] = total - kHead * p.B * HR;
     __syncthreads();
+    count = s_start[6] - s_start[4];
+    if (count == 0) return;   // nothing but heads
+    if (warp == kMmaWarp) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
+                   "r"(C::TMEM)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    }
+    tc_before_sync();
+    __syncthreads();
+    tc_after_sync();
   }
+  const uint32_t tmem = *s_tmem, tmem_o = tmem + 2 * N;
   bool failed = false;
 
-  if (warp == kWarps) {
-    // ------------------------------------------------------------ producer
-    int ld_b = s_start[0], ld_left = count, ld_hr, ld_tile;
-    int ld_len = min(max(s_start[2], 0), p.cap);
-    bool ld_over = s_start[2] > p.cap;
-    Span ld_span = span_of<TILE>(p, ld_len);
-    int ld_seg = s_start[1] * HR;
-    {
-      const int off = g0 - ld_seg;
-      ld_hr = off / ld_span.n;
-      ld_tile = off - ld_hr * ld_span.n;
-      ld_seg += ld_hr * ld_span.n;
+  if (warp == kMmaWarp) {
+    // ---------------------------------------- tensor cores: one thread issues
+    // (the warp stays together around it, so that the operands are made in uniform registers)
+    constexpr uint32_t s_kind = mma_kind(HALF, 128, N, false), o_kind = mma_kind(HALF, D, 2 * N, true);
+    const uint64_t q_op = operand(sbase + C::OFF_Q, 16);
+    const uint64_t p_op = operand<C::P_ROW>(sbase + C::OFF_P, TILE * 128);
+    int queries = 0;   // segments whose queries have been waited for
+    // scores^T of tile i: 128 tokens x N rows
+    auto scores = [&](int i, bool first) {
+      const int u = 2 * i, slot = u % U, sb = i & 1;
+      if (first) bar_wait(q_full, queries++ & 1, failed);
+      bar_wait(full + 8 * slot, (u / U) & 1, failed);
+      if (i >= 2) bar_wait(s_empty + 8 * sb, (i / 2 - 1) & 1, failed);
+      tc_after_sync();
+      __syncwarp();
+      const uint64_t k_op = operand(sbase + slot * C::UNIT, 16);
+      if (elect_one()) {
+        if (!failed)
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma(tmem + sb * N, k_op + (((kk >> 2) * C::HALF_BYTES + (kk & 3) * 32) >> 4),
+                q_op + (((kk >> 2) * N * 128 + (kk & 3) * 32) >> 4), s_kind, kk > 0);
+        mma_commit(empty + 8 * slot);
+        mma_commit(s_full + 8 * sb);
+      }
+      __syncwarp();
+    };
+    scores(0, true);
+    for (int i = 0; i < count; ++i) {
+      bar_wait(ready + 8 * (i & (C::DESCS - 1)), (i / C::DESCS) & 1, failed);
+      const bool first = desc_at(i)->first, last = desc_at(i)->last;
+      // the next tile's scores go first, unless its queries come after this segment's output
+      if (!last && i + 1 < count) scores(i + 1, false);
+      const int u = 2 * i + 1, slot = u % U;
+      bar_wait(full + 8 * slot, (u / U) & 1, failed);
+      bar_wait(p_full, i & 1, failed);
+      tc_after_sync();
+      const bool add = !first || *s_add;
+      __syncwarp();
+      const uint64_t v_op = operand(sbase + slot * C::UNIT, C::HALF_BYTES);
+      if (elect_one()) {
+        // output^T: D x 2N, V^T times the rounded weights and times their rests
+        if (!failed)
+#pragma unroll
+          for (int kk = 0; kk < TILE / 16; ++kk)
+            mma(tmem_o, v_op + (kk * 2048 >> 4), p_op + (kk * 16 * C::P_ROW >> 4), o_kind, add || kk > 0);
+        mma_commit(empty + 8 * slot);
+        mma_commit(o_done);
+      }
+      __syncwarp();
+      if (last && i + 1 < count) scores(i + 1, true);
     }
+  } else if (warp == kLoadWarp) {
+    // ------------------------------------------------------------ producer
+    int ld_b = s_start[0], ld_left = count, ld_hr = s_start[2], ld_tile = s_start[3], ld_from = ld_tile;
+    int ld_len = min(max(s_start[1], 0), p.cap);
+    bool ld_over = s_start[1] > p.cap;
+    Span ld_span = span_of(p, ld_len);
+    // (the segment's first tile: the units in front of this one's, less those of the segment itself)
+    int ld_seg = s_start[4] + kHead * (ld_b * HR + ld_hr + 1) - ld_tile;
     int next_raw = ld_b + 1 < p.B ? p.lengths[ld_b + 1] : 0;
     bool ld_first = true;
 
@@ -279,8 +482,12 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
       u.d.first = ld_first;
       u.d.n_tiles = ld_span.n;
       u.d.seg_start = ld_seg;
+      // positions run from len - T to len - 1
+      u.d.full = token0 + TILE <= ld_len - p.T + 1 &&
+                 (p.window == 0 || token0 > ld_len - 1 - p.window || token0 + TILE <= p.sinks);
       --ld_left;
       u.d.last = ld_left == 0 || ld_tile + 1 == ld_span.n;
+      u.d.whole = ld_from == 0 && ld_tile + 1 == ld_span.n;
       const int step = TMA ? p.box : 1;
 #pragma unroll
       for (int x = 0; x < LU; ++x) {
@@ -298,511 +505,493 @@ __global__ void __launch_bounds__(kThreads, 2) attention_kernel(const __grid_con
       ld_first = false;
       if (++ld_tile == ld_span.n && ld_left > 0) {
         ld_first = true;
-        ld_tile = 0;
-        ld_seg += ld_span.n;
+        ld_tile = ld_from = 0;
+        ld_seg += ld_span.n + kHead;
         if (++ld_hr == HR) {
           ld_hr = 0;
           ++ld_b;
           ld_len = min(max(next_raw, 0), p.cap);
           ld_over = next_raw > p.cap;
-          ld_span = span_of<TILE>(p, ld_len);
+          ld_span = span_of(p, ld_len);
           next_raw = ld_b + 1 < p.B ? p.lengths[ld_b + 1] : 0;
         }
       }
+    };
+    // a unit copied row by row is announced once its copies have landed, when the next one's are on their way
+    int pending = -1;
+    auto announce = [&]() {
+      if (pending < 0) return;
+      proxy_fence();
+      __syncwarp();
+      if (lane == 0) bar_arrive(full + 8 * pending);
+      pending = -1;
     };
     Lookup next;
     look(next);
     for (int i = 0; i < count; ++i) {
       Lookup u = next;
       look(next);
-      const int slot = i % S;
-      if (i >= S) bar_wait(empty + 8 * slot, (i / S - 1) & 1, failed);
-      const uint32_t kdst = sbase + slot * C::STAGE, vdst = kdst + C::KV_BYTES;
-      if constexpr (TMA) {
-        const bool ok = u.state[0] == 1 && u.id[0] >= 0 && u.id[0] < p.num_pages;
-        const uint32_t good = __ballot_sync(0xffffffffu, ok);
-        const uint32_t bad = __ballot_sync(0xffffffffu, u.state[0] != 0 && !ok);
+      bool ok[LU];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) u.d.bad[w] = 0;
+      for (int w = 0; w < 4; ++w) u.d.bad[w] = 0;
+      if constexpr (TMA) {
+        ok[0] = u.state[0] == 1 && u.id[0] >= 0 && u.id[0] < p.num_pages;
+        const uint32_t bad = __ballot_sync(0xffffffffu, u.state[0] != 0 && !ok[0]);
         if (bad)
 #pragma unroll
           for (int w = 0; w < TILE / 32; ++w)
             u.d.bad[w] = __ballot_sync(0xffffffffu, (bad >> ((w * 32 + lane) / p.box)) & 1);
-        if (lane == 0) {
-          descs[slot] = u.d;
-          bar_arrive(ready + 8 * slot);
-          bar_arrive_tx(full + 8 * slot, __popc(good) * p.box * 128 * C::HALVES * 2);
-        }
-        __syncwarp();
-        if (ok && !failed) {
-          const uint32_t at = lane * p.box * 128;
-#pragma unroll
-          for (int hf = 0; hf < C::HALVES; ++hf) {
-            tma_box(kdst + hf * C::HALF_BYTES + at, &kmap, full + 8 * slot, hf * 64, u.row[0], u.d.h, u.id[0]);
-            tma_box(vdst + hf * C::HALF_BYTES + at, &vmap, full + 8 * slot, hf * 64, u.row[0], u.d.h, u.id[0]);
-          }
-        }
       } else {
-        int64_t ko[LU], vo[LU];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) u.d.bad[w] = 0;
 #pragma unroll
         for (int x = 0; x < LU; ++x) {
-          const bool ok = u.state[x] == 1 && u.id[x] >= 0 && u.id[x] < p.num_pages;
-          u.d.bad[x] = __ballot_sync(0xffffffffu, u.state[x] != 0 && !ok);
-          ko[x] = !ok ? -1 : (int64_t)u.id[x] * p.k_page + (int64_t)u.d.h * p.k_head + (int64_t)u.row[x] * p.k_row;
-          vo[x] = !ok ? -1 : (int64_t)u.id[x] * p.v_page + (int64_t)u.d.h * p.v_head + (int64_t)u.row[x] * p.v_row;
+          ok[x] = u.state[x] == 1 && u.id[x] >= 0 && u.id[x] < p.num_pages;
+          u.d.bad[x] = __ballot_sync(0xffffffffu, u.state[x] != 0 && !ok[x]);
         }
-        if (lane == 0) {
-          descs[slot] = u.d;
-          bar_arrive(ready + 8 * slot);
+      }
+      for (int side = 0; side < 2; ++side) {   // K, V
+        const int un = 2 * i + side, slot = un % U;
+        if (un >= U) bar_wait(empty + 8 * slot, (un / U - 1) & 1, failed);
+        if (side == 0 && lane == 0) {
+          u.d.full = u.d.full && (u.d.bad[0] | u.d.bad[1] | u.d.bad[2] | u.d.bad[3]) == 0;
+          *desc_at(i) = u.d;
+          bar_arrive(ready + 8 * (i & (C::DESCS - 1)));
         }
-        constexpr int RPI = 32 / C::PIECES;   // rows per step
-        const int c = lane % C::PIECES, sub = lane / C::PIECES;
+        const uint32_t dst = sbase + slot * C::UNIT;
+        if constexpr (TMA) {
+          const uint32_t good = __ballot_sync(0xffffffffu, ok[0]);
+          if (lane == 0) bar_arrive_tx(full + 8 * slot, failed ? 0 : __popc(good) * p.box * 128 * C::HALVES);
+          __syncwarp();
+          if (ok[0] && !failed)
 #pragma unroll
-        for (int x = 0; x < LU; ++x)
+            for (int hf = 0; hf < C::HALVES; ++hf)
+              tma_box(dst + hf * C::HALF_BYTES + lane * p.box * 128, side ? &vmap : &kmap, full + 8 * slot, hf * 64,
+                      u.row[0], u.d.h, u.id[0]);
+        } else {
+          constexpr int RPI = 32 / C::PIECES;   // rows per step
+          const int c = lane % C::PIECES, sub = lane / C::PIECES;
+          const uint16_t* base = side ? p.v : p.k;
+#pragma unroll
+          for (int x = 0; x < LU; ++x) {
+            const int64_t mine = !ok[x] ? -1
+                                 : side ? (int64_t)u.id[x] * p.v_page + (int64_t)u.d.h * p.v_head + (int64_t)u.row[x] * p.v_row
+                                        : (int64_t)u.id[x] * p.k_page + (int64_t)u.d.h * p.k_head + (int64_t)u.row[x] * p.k_row;
 #pragma unroll 4
-          for (int r0 = 0; r0 < 32; r0 += RPI) {
-            const int64_t k_at = __shfl_sync(0xffffffffu, ko[x], r0 + sub), v_at = __shfl_sync(0xffffffffu, vo[x], r0 + sub);
-            const int r = x * 32 + r0 + sub;
-            const uint32_t at = (c >> 3) * C::HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-            if (k_at >= 0) {
-              cp_async16(kdst + at, p.k + k_at + c * 8);
-              cp_async16(vdst + at, p.v + v_at + c * 8);
+            for (int r0 = 0; r0 < 32; r0 += RPI) {
+              const int64_t from = __shfl_sync(0xffffffffu, mine, r0 + sub);
+              const int r = x * 32 + r0 + sub;
+              if (from >= 0)
+                cp_async16(dst + (c >> 3) * C::HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + from + c * 8);
             }
           }
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(full + 8 * slot) : "memory");
-        __syncwarp();
-        if (lane == 0) bar_arrive(full + 8 * slot);
+          cp_async_commit();
+          cp_async_wait<1>();
+          announce();
+          pending = slot;
+        }
       }
     }
-    // consumers wait for every tile; after a wait that ran out, see the copies in flight off
-    if (failed)
-      for (int i = max(0, count - S); i < count; ++i) bar_wait_long(full + 8 * (i % S), (i / S) & 1);
-    return;
-  }
-
-  // -------------------------------------------------------------- consumers
-  uint32_t qf[MT <= 2 ? MT : 1][D / 16][4];   // query fragments (MT = 4 reads them from shared memory)
-  float o[MT][C::DT][4];
-  float m[MT][2], l[MT][2];
-  int back[MT][2];                            // T - t of the thread's rows: position = len - back
-  // Fragment addresses: 128-byte rows, 16-byte piece c of row r at c ^ (r & 7); the rows of a thread's
-  // ldmatrix lanes all have r & 7 = lane & 7.
-  const uint32_t swz = (lane & 7) << 4;
-  const uint32_t k_row = (warp * (TILE / kWarps) + ((lane >> 4) << 3) + (lane & 7)) * 128, k_col = ((lane >> 3) & 1) << 4;
-  const uint32_t v_at = (lane & 15) * 128 + ((warp * C::DW) >> 6) * C::HALF_BYTES;
-  const uint32_t v_col = ((warp * C::DW) & 63) * 2 + ((lane >> 4) << 4);
-  const uint32_t a_row = lane & 15, a_col = (lane >> 4) << 4;   // Q and P operands
-
-  for (int i = 0; i < count; ++i) {
-    const int slot = i % S;
-    bar_wait(ready + 8 * slot, (i / S) & 1, failed);
-    const Desc& ds = descs[slot];
-    const int len = ds.len, token0 = ds.token0, rt = ds.rt;
-
-    if (ds.first) {
-      // query rows of this segment, while its first tile is on the way: row r = t * G + g
-      for (int x = tid; x < ROWS * C::PIECES; x += kConsumers) {
-        const int r = x / C::PIECES, c = x % C::PIECES;
-        const int R = rt * ROWS + r;
-        uint4 w = make_uint4(0, 0, 0, 0);
+    if constexpr (!TMA) {
+      cp_async_wait<0>();
+      announce();
+    }
+    // after a wait that ran out, see the copies in flight off
+    if (TMA && failed)
+      for (int un = max(0, 2 * count - U); un < 2 * count; ++un) bar_wait_long(full + 8 * (un % U), (un / U) & 1);
+  } else {
+    // ------------------------------------------------------------ consumers
+    const uint32_t my_lanes = (uint32_t)warp << 21;   // tensor-memory lanes 32 w ..
+    float l[N];                                       // this thread's tokens' share of the rows' sums
+    // A segment's query rows, row r = t * G + g; read while the segment before it is finished (N = 64: not, for
+    // the registers).
+    constexpr int QV = N * C::PIECES / kConsumers;
+    uint4 q[QV];
+    auto load_queries = [&](const Desc& d) {
+#pragma unroll
+      for (int y = 0; y < QV; ++y) {
+        const int r = (y * kConsumers + tid) / C::PIECES, c = tid % C::PIECES, R = d.rt * N + r;
+        q[y] = make_uint4(0, 0, 0, 0);
         if (R < p.R) {
           const int t = R / p.G, g = R - t * p.G;
-          w = *reinterpret_cast<const uint4*>(p.q + (int64_t)ds.b * p.q_b + (int64_t)(ds.h * p.G + g) * p.q_h +
-                                              (int64_t)t * p.q_t + c * 8);
+          q[y] = *reinterpret_cast<const uint4*>(p.q + (int64_t)d.b * p.q_b + (int64_t)(d.h * p.G + g) * p.q_h +
+                                                 (int64_t)t * p.q_t + c * 8);
         }
-        *reinterpret_cast<uint4*>(smem + C::OFF_Q + r * D * 2 + ((c ^ (r & 7)) << 4)) = w;
       }
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int R = rt * ROWS + mt * 16 + e * 8 + lane / 4;
-          back[mt][e] = p.T - min(R, p.R - 1) / p.G;
-          m[mt][e] = -INFINITY;
-          l[mt][e] = 0.f;
-        }
-#pragma unroll
-        for (int n = 0; n < C::DT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
-      }
-      consumer_sync();
-      if constexpr (MT <= 2) {
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            ldsm_x4(sbase + C::OFF_Q + (mt * 16 + a_row) * D * 2 + ((kk * 32 + a_col) ^ swz), qf[mt][kk][0],
-                    qf[mt][kk][1], qf[mt][kk][2], qf[mt][kk][3]);
-      }
-    }
+    };
+    constexpr bool kAhead = N <= 32;
+    for (int i = 0; i < count; ++i) {
+      bar_wait(ready + 8 * (i & (C::DESCS - 1)), (i / C::DESCS) & 1, failed);
+      const Desc& ds = *desc_at(i);
+      const int len = ds.len, token0 = ds.token0, rt = ds.rt;
+      const int n_rows = min(N, p.R - rt * N);
+      const int v_unit = 2 * i + 1, v_slot = v_unit % U;
+      uint8_t* vs = smem + v_slot * C::UNIT;
 
-    bar_wait(full + 8 * slot, (i / S) & 1, failed);
-
-    // ---- scores: this warp's TILE/4 tokens x all rows
-    const uint32_t kb = sbase + slot * C::STAGE, vb = kb + C::KV_BYTES;
-    float s[MT][C::NT][4];
+      if (ds.first) {
+        if (!kAhead || i == 0) load_queries(ds);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int n = 0; n < C::NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      uint32_t bf[C::NT][2];
-#pragma unroll
-      for (int n2 = 0; n2 < C::NT / 2; ++n2)
-        ldsm_x4(kb + k_row + n2 * 2048 + (kk >> 2) * C::HALF_BYTES + (((kk & 3) * 32 + k_col) ^ swz), bf[2 * n2][0],
-                bf[2 * n2][1], bf[2 * n2 + 1][0], bf[2 * n2 + 1][1]);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        uint32_t a[4];
-        if constexpr (MT <= 2) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) a[e] = qf[mt][kk][e];
-        } else {
-          ldsm_x4(sbase + C::OFF_Q + (mt * 16 + a_row) * D * 2 + ((kk * 32 + a_col) ^ swz), a[0], a[1], a[2], a[3]);
+        for (int y = 0; y < QV; ++y) {
+          const int r = (y * kConsumers + tid) / C::PIECES, c = tid % C::PIECES;
+          *reinterpret_cast<uint4*>(smem + C::OFF_Q + (c >> 3) * N * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = q[y];
         }
+        if (tid < N) {
+          const int R = min(rt * N + tid, p.R - 1), t = R / p.G;
+          mu_s[tid] = kUnseen;
+          pos_s[tid] = len - p.T + t;
+          row_s[tid] = (ds.b * p.HQ + ds.h * p.G + R - t * p.G) * p.T + t;
+        }
+        if (tid == 0) *s_add = 0;
 #pragma unroll
-        for (int n = 0; n < C::NT; ++n) mma_e<HALF>(s[mt][n], a[0], a[1], a[2], a[3], bf[n][0], bf[n][1]);
+        for (int r = 0; r < N; ++r) l[r] = 0.f;
+        proxy_fence();
+        consumer_sync();
+        if (tid == 0) bar_arrive(q_full);
       }
-    }
-    const int in_tile = warp * (TILE / kWarps) + (lane & 3) * 2;   // token of n-tile 0, element 0
-    const int tok = token0 + in_tile;
-    // every row sees every token of the tile: positions run from len - T to len - 1
-    const bool full_tile = token0 + TILE <= len - p.T + 1 &&
-                           (p.window == 0 || token0 > len - 1 - p.window || token0 + TILE <= p.sinks) &&
-                           (ds.bad[0] | ds.bad[1] | ds.bad[2] | ds.bad[3]) == 0;
-    float mx[MT][2];
+      const bool full_tile = ds.full;
+      const int lo = p.window > 0 ? max(0, max(len - p.T, 0) - p.window + 1) : 0;
+      if (!full_tile) {
+        // rows of V that no query sees hold whatever the page or an earlier
+        // tile left there, and 0 * NaN is NaN: zero them
+        bar_wait(full + 8 * v_slot, (v_unit / U) & 1, failed);
+        for (int x = tid; x < TILE * C::PIECES; x += kConsumers) {
+          const int r = x / C::PIECES, c = x % C::PIECES, j = token0 + r;
+          if (j < len && (j >= lo || j < p.sinks) && !((ds.bad[r >> 5] >> (r & 31)) & 1)) continue;
+          *reinterpret_cast<uint4*>(vs + (c >> 3) * C::HALF_BYTES + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+      }
+
+      // ---- scores: thread = token, registers = rows
+      bar_wait(s_full + 8 * (i & 1), (i >> 1) & 1, failed);
+      tc_after_sync();
+      const int j = token0 + tid;
+      // the scores of this thread's token, scaled (log2 units) where `factor` is 1: in a tile that some row does
+      // not see whole they are also masked, -inf, or NaN on a page outside the pool for the rows that see it
+      const float factor = full_tile ? p.scale2 : 1.f;
+      float x[N];
+      auto load_scores = [&]() {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      mx[mt][0] = mx[mt][1] = -INFINITY;
+        for (int c = 0; c < N; c += 16)
+          if (c < n_rows) tmem_load(tmem + (i & 1) * N + my_lanes + c, x + c);
 #pragma unroll
-      for (int n = 0; n < C::NT; ++n)
+        for (int c = 0; c < N; c += 16)
+          if (c < n_rows) tmem_wait_load(x + c);
+        if (!full_tile) {
+          const bool bad = (ds.bad[warp] >> lane) & 1;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = s[mt][n][e] * p.scale2;
-          if (!full_tile) {
-            const int at = in_tile + n * 8 + (e & 1), j = token0 + at, pos = len - back[mt][e >> 1];
+          for (int r = 0; r < N; ++r) {
+            if ((r & 3) == 0 && r >= n_rows) break;
+            const int pos = pos_s[r];
             const bool seen = j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks);
-            // a page outside the pool: the rows that see it say so
-            x = !seen ? -INFINITY : (ds.bad[at >> 5] >> (at & 31)) & 1 ? NAN : x;
-          }
-          s[mt][n][e] = x;
-          mx[mt][e >> 1] = fmaxf(mx[mt][e >> 1], x);
-        }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        mx[mt][e] = fmaxf(mx[mt][e], __shfl_xor_sync(0xffffffffu, mx[mt][e], 1));
-        mx[mt][e] = fmaxf(mx[mt][e], __shfl_xor_sync(0xffffffffu, mx[mt][e], 2));
-        if ((lane & 3) == 0) smax[warp * ROWS + mt * 16 + e * 8 + lane / 4] = mx[mt][e];
-      }
-    }
-    if (p.scores != nullptr) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int R = rt * ROWS + mt * 16 + e * 8 + lane / 4;
-          if (R < p.R) {
-            float* dst = p.scores + ((int64_t)(ds.b * p.HKV + ds.h) * p.R + R) * p.score_stride + tok;
-#pragma unroll
-            for (int n = 0; n < C::NT; ++n)
-              *reinterpret_cast<float2*>(dst + n * 8) = make_float2(s[mt][n][2 * e], s[mt][n][2 * e + 1]);
+            x[r] = !seen ? -INFINITY : bad ? NAN : x[r] * p.scale2;
           }
         }
-    }
-    if (!full_tile) {
-      // rows of V that no query sees hold whatever the page or an earlier
-      // tile left there, and 0 * NaN is NaN: zero them
-      const int lo = p.window > 0 ? max(0, max(len - p.T, 0) - p.window + 1) : 0;
-      for (int x = tid; x < TILE * C::PIECES; x += kConsumers) {
-        const int r = x / C::PIECES, c = x % C::PIECES, j = token0 + r;
-        if (j < len && (j >= lo || j < p.sinks) && !((ds.bad[r >> 5] >> (r & 31)) & 1)) continue;
-        *reinterpret_cast<uint4*>(smem + slot * C::STAGE + C::KV_BYTES + (c >> 3) * C::HALF_BYTES + r * 128 +
-                                  ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-      }
-    }
-    consumer_sync();
-
-    // ---- running maximum and sum; P to shared memory.  The tensor cores
-    // take it in the pages' type: as the rounded value and the rounded rest,
-    // two products, so that the output's own rounding stays the largest error
-    // (one rounded value alone doubles it).
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = mt * 16 + e * 8 + lane / 4;
-        float mn = m[mt][e];
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) mn = fmaxf(mn, smax[w * ROWS + r]);
-        const float mu = finite_or_zero(mn);
-        const float alpha = fast_exp2(m[mt][e] - mu);
-        m[mt][e] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int n = 0; n < C::NT; ++n) {
-          const float p0 = fast_exp2(s[mt][n][2 * e] - mu), p1 = fast_exp2(s[mt][n][2 * e + 1] - mu);
-          sum += p0 + p1;
-          const int c = warp * (TILE / kWarps / 8) + n;   // 8-token piece of the row
-          const uint32_t hi = pack2<HALF>(p0, p1);
-          const uint32_t lo = pack2<HALF>(p0 - to_float<HALF>((uint16_t)hi), p1 - to_float<HALF>((uint16_t)(hi >> 16)));
-          uint8_t* dst = smem + C::OFF_P + r * TILE * 2 + ((c ^ (r & 7)) << 4) + (lane & 3) * 4;
-          *reinterpret_cast<uint32_t*>(dst) = hi;
-          *reinterpret_cast<uint32_t*>(dst + C::P_HALF) = lo;
-        }
-        l[mt][e] = l[mt][e] * alpha + sum;
-#pragma unroll
-        for (int n = 0; n < C::DT; ++n) {
-          o[mt][n][2 * e] *= alpha;
-          o[mt][n][2 * e + 1] *= alpha;
-        }
-      }
-    consumer_sync();
-
-    // A token that some rows see and others do not has weight 0 in the
-    // others, and 0 * inf is NaN in the product below.  Such tokens exist for
-    // T > 1 only, T - 1 of them at either end of the span.  When one of them
-    // holds an infinity or NaN, they are added by hand to the rows that see
-    // them and then zeroed.
-    if (p.T > 1 && !full_tile) {
-      const int lo = p.window > 0 ? max(0, max(len - p.T, 0) - p.window + 1) : 0;
-      const int n_part = (p.window > 0 ? 2 : 1) * (p.T - 1);
-      // the n-th such token's row in the tile, or -1
-      auto part_row = [&](int n) {
-        const int j = n < p.T - 1 ? len - 1 - n : lo + n - (p.T - 1);
-        return j >= 0 && j < len && j >= token0 && j < token0 + TILE ? j - token0 : -1;
       };
-      uint8_t* vs = smem + slot * C::STAGE + C::KV_BYTES;
-      int odd = 0;
-      for (int x = tid; x < n_part * C::PIECES; x += kConsumers) {
-        const int r = part_row(x / C::PIECES), c = x % C::PIECES;
-        if (r < 0) continue;
-        const uint4 w = *reinterpret_cast<const uint4*>(vs + (c >> 3) * C::HALF_BYTES + r * 128 + ((c & 7) << 4));
-        const uint32_t ones = HALF ? 0x7c00u : 0x7f80u;
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+      // ---- exponents against the rows' references, each a maximum so far.
+      // Any reference does while 2^(score - reference) stays in range: it
+      // moves, and the output is rescaled, only when an exponent passes 8 or a
+      // row is seen for the first time (kUnseen makes its exponents huge).
+      auto exponents = [&]() {
+        float hot = -INFINITY;
 #pragma unroll
-        for (int y = 0; y < 4; ++y) odd |= (ws[y] & ones) == ones || ((ws[y] >> 16) & ones) == ones;
+        for (int r = 0; r < N; ++r) {
+          if ((r & 3) == 0 && r >= n_rows) break;
+          x[r] = __fmaf_rn(x[r], factor, -mu_s[r]);
+          if (r < n_rows) hot = fmaxf(hot, x[r]);
+        }
+        return hot > 8.f;
+      };
+      load_scores();
+      if (p.scores != nullptr) {
+        float* dst = p.scores + ((int64_t)(ds.b * p.HKV + ds.h) * p.R + rt * N) * p.score_stride + j;
+#pragma unroll
+        for (int r = 0; r < N; ++r)
+          if (r < n_rows) dst[r * p.score_stride] = x[r] * factor;
       }
-      int any;
-      asm volatile("{\n.reg .pred a, b;\nsetp.ne.s32 a, %1, 0;\nbar.red.or.pred b, 1, 128, a;\nselp.s32 %0, 1, 0, b;\n}\n"
-                   : "=r"(any)
-                   : "r"(odd)
-                   : "memory");
-      if (any) {
-        for (int n = 0; n < n_part; ++n) {
-          const int r = part_row(n), j = token0 + r;
-          if (r < 0 || (n >= p.T - 1 && j > len - p.T)) continue;   // both ends may name it: once
+      const bool moves = ds.first || consumer_any(exponents());
+      // the product before this one is done: its P may be overwritten, its output read
+      if (i > 0) bar_wait(o_done, (i - 1) & 1, failed);
+      tc_after_sync();
+      if (moves) {
+        if (!ds.first) load_scores();
+        {
+          float v[N];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int r = 0; r < N; ++r) v[r] = x[r] * factor;
+          if (N == 16 && n_rows <= 8) store_rows<8, false>(v, smax + warp * N, lane);
+          else store_rows<N, false>(v, smax + warp * N, lane);
+        }
+        consumer_sync();
+        if (tid < n_rows) {   // thread = row
+          const float before = mu_s[tid];
+          float mn = before;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int pos = len - back[mt][e], row = mt * 16 + e * 8 + lane / 4;
-              if (!(j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks))) continue;
-              const uint8_t* pw = smem + C::OFF_P + row * TILE * 2 + (((r >> 3) ^ (row & 7)) << 4) + (r & 7) * 2;
-              const float w = to_float<HALF>(*reinterpret_cast<const uint16_t*>(pw)) +
-                              to_float<HALF>(*reinterpret_cast<const uint16_t*>(pw + C::P_HALF));
+          for (int w = 0; w < kWarps; ++w) mn = fmaxf(mn, smax[w * N + tid]);
+          mu_s[tid] = mn;
+          alpha_s[tid] = fast_exp2(before - mn);
+        }
+        consumer_sync();
+        if (!ds.first) {
 #pragma unroll
-              for (int x = 0; x < C::DT; ++x) {
-                const int col = warp * C::DW + x * 8 + (lane & 3) * 2;
-                const uint32_t vv = *reinterpret_cast<const uint32_t*>(
-                    vs + (col >> 6) * C::HALF_BYTES + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4) + (col & 7) * 2);
-                o[mt][x][2 * e] += w * to_float<HALF>((uint16_t)vv);
-                o[mt][x][2 * e + 1] += w * to_float<HALF>((uint16_t)(vv >> 16));
+          for (int c = 0; c < N; c += 16)
+            if (c < n_rows) {
+#pragma unroll
+              for (int part = 0; part < 2; ++part) {
+                float o[16];
+                tmem_load(tmem_o + my_lanes + part * N + c, o);
+                tmem_wait_load(o);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[r] *= c + r < n_rows ? alpha_s[c + r] : 1.f;
+                tmem_store(tmem_o + my_lanes + part * N + c, o);
+              }
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+                if (c + r < n_rows) l[c + r] *= alpha_s[c + r];
+            }
+          tmem_wait_store();
+        }
+        exponents();
+      }
+      tc_before_sync();
+      __syncwarp();
+      if (lane == 0) bar_arrive(s_empty + 8 * (i & 1));
+      // ---- P.  The tensor cores take it in the pages' type: as the rounded
+      // value and the rounded rest, side by side, so that the output's own
+      // rounding stays the largest error (one rounded value alone doubles it).
+#pragma unroll
+      for (int r0 = 0; r0 < N; r0 += 8) {
+        if (r0 >= n_rows) break;
+        uint32_t hi[4], rest[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int r = r0 + 2 * y;
+          const float p0 = fast_exp2(x[r]), p1 = fast_exp2(x[r + 1]);
+          l[r] += p0;
+          l[r + 1] += p1;
+          hi[y] = pack2<HALF>(p0, p1);
+          rest[y] = pack2<HALF>(p0 - to_float<HALF>((uint16_t)hi[y]), p1 - to_float<HALF>((uint16_t)(hi[y] >> 16)));
+        }
+        *reinterpret_cast<uint4*>(smem + C::OFF_P + C::p_at(tid, r0, 0)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(smem + C::OFF_P + C::p_at(tid, r0, 1)) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+      }
+      // A token that some rows see and others do not has weight 0 in the
+      // others, and 0 * inf is NaN in the product.  Such tokens exist for
+      // T > 1 only, T - 1 of them at either end of the span.  When one of them
+      // holds an infinity or NaN, they are added by hand to the rows that see
+      // them and then zeroed.
+      if (p.T > 1 && !full_tile) {
+        const int n_part = (p.window > 0 ? 2 : 1) * (p.T - 1);
+        // the n-th such token's row in the tile, or -1
+        auto part_row = [&](int n) {
+          const int y = n < p.T - 1 ? len - 1 - n : lo + n - (p.T - 1);
+          return y >= 0 && y < len && y >= token0 && y < token0 + TILE ? y - token0 : -1;
+        };
+        bool odd = false;
+        for (int y = tid; y < n_part * C::PIECES; y += kConsumers) {
+          const int r = part_row(y / C::PIECES), c = y % C::PIECES;
+          if (r < 0) continue;
+          const uint4 w = *reinterpret_cast<const uint4*>(vs + (c >> 3) * C::HALF_BYTES + r * 128 + ((c & 7) << 4));
+          const uint32_t ones = HALF ? 0x7c00u : 0x7f80u;
+          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int z = 0; z < 4; ++z) odd |= (ws[z] & ones) == ones || ((ws[z] >> 16) & ones) == ones;
+        }
+        if (consumer_any(odd)) {
+          // thread = output element d of every row (D = 64: 16 of a warp's lanes)
+          const int d = D == 128 ? tid : warp * 16 + (lane & 15);
+#pragma unroll
+          for (int c = 0; c < N; c += 16) {
+            if (c >= n_rows) break;
+            float o[16];
+            tmem_load(tmem_o + my_lanes + c, o);
+            tmem_wait_load(o);
+            if (ds.first) {   // nothing there yet
+#pragma unroll
+              for (int r = 0; r < 16; ++r) o[r] = 0.f;
+              tmem_store(tmem_o + my_lanes + N + c, o);
+            }
+            for (int n = 0; n < n_part; ++n) {
+              const int tr = part_row(n), y = token0 + tr;
+              if (tr < 0 || (n >= p.T - 1 && y > len - p.T)) continue;   // both ends may name it: once
+              const float v = to_float<HALF>(*reinterpret_cast<const uint16_t*>(
+                  vs + (d >> 6) * C::HALF_BYTES + tr * 128 + ((((d & 63) >> 3) ^ (tr & 7)) << 4) + (d & 7) * 2));
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                if (c + r >= n_rows) break;
+                const int pos = pos_s[c + r];
+                if (!(y <= pos && (p.window == 0 || y > pos - p.window || y < p.sinks))) continue;
+                o[r] += v * (to_float<HALF>(*reinterpret_cast<const uint16_t*>(smem + C::OFF_P + C::p_at(tr, c + r, 0))) +
+                             to_float<HALF>(*reinterpret_cast<const uint16_t*>(smem + C::OFF_P + C::p_at(tr, c + r, 1))));
               }
             }
-        }
-        consumer_sync();
-        for (int x = tid; x < n_part * C::PIECES; x += kConsumers) {
-          const int r = part_row(x / C::PIECES), c = x % C::PIECES;
-          if (r >= 0)
-            *reinterpret_cast<uint4*>(vs + (c >> 3) * C::HALF_BYTES + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-        }
-        consumer_sync();
-      }
-    }
-
-    // ---- output: all tokens x this warp's D/4 columns
-#pragma unroll
-    for (int kk = 0; kk < TILE / 16; ++kk) {
-      uint32_t bf[C::DT][2];
-#pragma unroll
-      for (int n2 = 0; n2 < C::DT / 2; ++n2)
-        ldsm_x4_trans(vb + v_at + kk * 2048 + ((n2 * 32 + v_col) ^ swz), bf[2 * n2][0], bf[2 * n2][1],
-                      bf[2 * n2 + 1][0], bf[2 * n2 + 1][1]);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const uint32_t at = sbase + C::OFF_P + (mt * 16 + a_row) * TILE * 2 + ((kk * 32 + a_col) ^ swz);
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          uint32_t a[4];
-          ldsm_x4(at + part * C::P_HALF, a[0], a[1], a[2], a[3]);
-#pragma unroll
-          for (int n = 0; n < C::DT; ++n) mma_e<HALF>(o[mt][n], a[0], a[1], a[2], a[3], bf[n][0], bf[n][1]);
-        }
-      }
-    }
-
-    const bool last = ds.last;
-    const int sb = ds.b, sh = ds.h, n_tiles = ds.n_tiles;
-    const int seg_start = ds.seg_start;
-    // the tile is read: hand it back (zeroed rows are ordinary stores, which the TMA must not overtake)
-    if (!full_tile) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    __syncwarp();
-    if (lane == 0) bar_arrive(empty + 8 * slot);
-
-    if (last) {
-      // ---- the rows' sums over the four warps
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = failed ? NAN : l[mt][e];
-          x += __shfl_xor_sync(0xffffffffu, x, 1);
-          x += __shfl_xor_sync(0xffffffffu, x, 2);
-          if ((lane & 3) == 0) ssum[warp * ROWS + mt * 16 + e * 8 + lane / 4] = x;
-        }
-      consumer_sync();
-      const bool whole = g0 <= seg_start && g0 + i == seg_start + n_tiles - 1;
-      const int64_t slot_o = blockIdx.x * 2 + (seg_start > g0 ? 1 : 0);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = mt * 16 + e * 8 + lane / 4, R = rt * ROWS + r;
-          if (R >= p.R) continue;
-          float sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) sum += ssum[w * ROWS + r];
-          const int col = warp * C::DW + (lane & 3) * 2;
-          if (whole) {
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            const int t = R / p.G, g = R - t * p.G;
-            const int64_t row = ((int64_t)sb * p.HQ + sh * p.G + g) * p.T + t;
-#pragma unroll
-            for (int n = 0; n < C::DT; ++n)
-              *reinterpret_cast<uint32_t*>(p.out + row * D + col + n * 8) =
-                  pack2<HALF>(o[mt][n][2 * e] * inv, o[mt][n][2 * e + 1] * inv);
-            if (warp == 0 && (lane & 3) == 0) {
-              const float lse2 = sum == 0.f ? -INFINITY : finite_or_zero(m[mt][e]) + log2f(sum);
-              if (p.lse) p.lse[row] = lse2 * 0.6931471805599453f;
-              if (p.row_lse2) p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + R] = lse2;
-            }
-          } else {
-            float* po = p.part_o + (slot_o * ROWS + r) * D + col;
-#pragma unroll
-            for (int n = 0; n < C::DT; ++n)
-              *reinterpret_cast<float2*>(po + n * 8) = make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
-            if (warp == 0 && (lane & 3) == 0)
-              *reinterpret_cast<float2*>(p.part_ml + (slot_o * ROWS + r) * 2) = make_float2(m[mt][e], sum);
+            tmem_store(tmem_o + my_lanes + c, o);
+          }
+          tmem_wait_store();
+          consumer_sync();
+          if (tid == 0) *s_add = 1;
+          for (int y = tid; y < n_part * C::PIECES; y += kConsumers) {
+            const int r = part_row(y / C::PIECES), c = y % C::PIECES;
+            if (r >= 0)
+              *reinterpret_cast<uint4*>(vs + (c >> 3) * C::HALF_BYTES + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
           }
         }
-      if (!whole) {
-        // ---- join.  The CTAs c0..c1 of the segment arrive in groups of
-        // kGroup; a group's last adds its parts up, the last group's last
-        // adds the groups up and writes the rows: two rounds of a few
-        // independent loads instead of one long chain.  The order of the
-        // sums is the CTAs', whoever does them.
-        const Cut cut(total, ctas);
-        const int c0 = cut.owner(seg_start), c1 = cut.owner(seg_start + n_tiles - 1);
-        const int n = c1 - c0 + 1, groups = (n + kGroup - 1) / kGroup;
-        const int n_rows = min(ROWS, p.R - rt * ROWS);
-        // part k of the segment: CTA c0 + k; CTA c0's second part when it began with another segment.
-        // A group's sum: behind all parts, by its first CTA.
-        const int first_slot = c0 * 2 + (cut.begin(c0) < seg_start ? 1 : 0);
-        // parts [k0, k0 + cnt) of the segment, or its group sums, -> the rows, or group sum `to`
-        auto join = [&](int k0, int cnt, bool of_groups, int to) {
-          auto slot_of = [&](int k) {
-            if (!of_groups) return k0 + k == 0 ? first_slot : (c0 + k0 + k) * 2;
-            return k * kGroup + 1 == n ? c1 * 2 : 2 * p.ctas + c0 + k * kGroup;   // a group of one is its part
-          };
-#pragma unroll 1
-          for (int x = tid; x < n_rows * (D / 4); x += kConsumers) {
-            const int r = x / (D / 4), col = x % (D / 4) * 4;
-            float mm = -INFINITY, sum = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-            for (int kb = 0; kb < cnt; kb += 8) {
-              float2 ml[8];
-              float4 f[8];
+      }
+      proxy_fence();
+      tc_before_sync();
+      __syncwarp();
+      const bool last = ds.last, whole = ds.whole;
+      const int sb = ds.b, sh = ds.h, n_tiles = ds.n_tiles, seg_start = ds.seg_start;
+      if (lane == 0) bar_arrive(p_full);
+
+      if (last) {
+        if (kAhead && i + 1 < count) {   // the next segment's queries
+          bar_wait(ready + 8 * ((i + 1) & (C::DESCS - 1)), ((i + 1) / C::DESCS) & 1, failed);
+          load_queries(*desc_at(i + 1));
+        }
+        // ---- the rows' sums over the tokens' threads, while the last product runs
+        if (failed)
 #pragma unroll
-              for (int y = 0; y < 8; ++y) {
-                ml[y] = make_float2(-INFINITY, 0.f);
-                f[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (kb + y < cnt) {
-                  const int64_t at = (int64_t)slot_of(kb + y) * ROWS + r;
-                  ml[y] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
-                  f[y] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + col));
+          for (int r = 0; r < N; ++r) l[r] = NAN;
+        if (N == 16 && n_rows <= 8) store_rows<8, true>(l, ssum + warp * N, lane);
+        else store_rows<N, true>(l, ssum + warp * N, lane);
+        consumer_sync();
+        const int64_t slot_o = blockIdx.x * 2 + (seg_start - kHead > g0 ? 1 : 0);
+        if (tid < n_rows) {   // thread = row
+          const float sum = ssum[tid] + ssum[N + tid] + ssum[2 * N + tid] + ssum[3 * N + tid];
+          if (whole) {
+            alpha_s[tid] = sum == 0.f ? 0.f : 1.f / sum;
+            const float lse2 = sum == 0.f ? -INFINITY : mu_s[tid] + log2f(sum);
+            if (p.lse) p.lse[row_s[tid]] = lse2 * 0.6931471805599453f;
+            if (p.row_lse2) p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + tid] = lse2;
+          } else {
+            *reinterpret_cast<float2*>(p.part_ml + (slot_o * ROWS + tid) * 2) = make_float2(mu_s[tid], sum);
+          }
+        }
+        bar_wait(o_done, i & 1, failed);
+        tc_after_sync();
+        consumer_sync();
+        const int d = D == 128 ? tid : warp * 16 + lane;   // (D = 64: lanes below 16 hold a row of the output each)
+#pragma unroll
+        for (int c = 0; c < N; c += 16) {
+          if (c >= n_rows) break;
+          float o[16], rest[16];
+          tmem_load(tmem_o + my_lanes + c, o);
+          tmem_load(tmem_o + my_lanes + N + c, rest);
+          tmem_wait_load(o);
+          tmem_wait_load(rest);
+          if (D == 128 || lane < 16) {
+            float* part = p.part_o + (slot_o * ROWS + c) * D + d;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              if (c + r >= n_rows) break;
+              const float x = o[r] + rest[r];
+              if (whole) p.out[(int64_t)row_s[c + r] * D + d] = (uint16_t)pack2<HALF>(x * alpha_s[c + r], 0.f);
+              else part[r * D] = x;
+            }
+          }
+        }
+        tc_before_sync();
+        if (!whole) {
+          // ---- join.  The CTAs c0..c1 of the segment arrive in groups of
+          // kGroup; a group's last adds its parts up, the last group's last
+          // adds the groups up and writes the rows: two rounds of a few
+          // independent loads instead of one long chain.  The order of the
+          // sums is the CTAs', whoever does them.
+          const Cut cut(total, ctas);
+          const int c0 = cut.owner(seg_start), c1 = cut.owner(seg_start + n_tiles - 1);
+          const int n = c1 - c0 + 1, groups = (n + kGroup - 1) / kGroup;
+          // part k of the segment: CTA c0 + k; CTA c0's second part when it began with another segment.
+          // A group's sum: behind all parts, by its first CTA.
+          const int first_slot = c0 * 2 + (cut.begin(c0) < seg_start - kHead ? 1 : 0);
+          // parts [k0, k0 + cnt) of the segment, or its group sums, -> the rows, or group sum `to`
+          auto join = [&](int k0, int cnt, bool of_groups, int to) {
+            auto slot_of = [&](int k) {
+              if (!of_groups) return k0 + k == 0 ? first_slot : (c0 + k0 + k) * 2;
+              return k * kGroup + 1 == n ? c1 * 2 : 2 * p.ctas + c0 + k * kGroup;   // a group of one is its part
+            };
+#pragma unroll 2
+            for (int x = tid; x < n_rows * (D / 4); x += kConsumers) {
+              const int r = x / (D / 4), col = x % (D / 4) * 4;
+              float mm = kUnseen, sum = 0.f;
+              float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+              for (int kb = 0; kb < cnt; kb += 4) {
+                float2 ml[4];
+                float4 f[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  ml[y] = make_float2(kUnseen, 0.f);
+                  f[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+                  if (kb + y < cnt) {
+                    const int64_t at = (int64_t)slot_of(kb + y) * ROWS + r;
+                    ml[y] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
+                    f[y] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + col));
+                  }
+                }
+                const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), mm);
+                const float alpha = fast_exp2(mm - mn);
+                mm = mn;
+                sum *= alpha;
+                acc.x *= alpha; acc.y *= alpha; acc.z *= alpha; acc.w *= alpha;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const float w = fast_exp2(ml[y].x - mn);
+                  sum += w * ml[y].y;
+                  acc.x += w * f[y].x; acc.y += w * f[y].y; acc.z += w * f[y].z; acc.w += w * f[y].w;
                 }
               }
-              float mn = mm;
-#pragma unroll
-              for (int y = 0; y < 8; ++y) mn = fmaxf(mn, ml[y].x);
-              const float mu = finite_or_zero(mn), alpha = fast_exp2(mm - mu);
-              mm = mn;
-              sum *= alpha;
-              acc.x *= alpha; acc.y *= alpha; acc.z *= alpha; acc.w *= alpha;
-#pragma unroll
-              for (int y = 0; y < 8; ++y) {
-                const float w = fast_exp2(ml[y].x - mu);
-                sum += w * ml[y].y;
-                acc.x += w * f[y].x; acc.y += w * f[y].y; acc.z += w * f[y].z; acc.w += w * f[y].w;
+              if (to >= 0) {
+                const int64_t at = (int64_t)(2 * p.ctas + to) * ROWS + r;
+                *reinterpret_cast<float4*>(p.part_o + at * D + col) = acc;
+                if (col == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, sum);
+                continue;
+              }
+              const float inv = sum == 0.f ? 0.f : 1.f / sum;
+              *reinterpret_cast<uint2*>(p.out + (int64_t)row_s[r] * D + col) =
+                  make_uint2(pack2<HALF>(acc.x * inv, acc.y * inv), pack2<HALF>(acc.z * inv, acc.w * inv));
+              if (col == 0) {
+                const float lse2 = sum == 0.f ? -INFINITY : mm + log2f(sum);
+                if (p.lse) p.lse[row_s[r]] = lse2 * 0.6931471805599453f;
+                if (p.row_lse2) p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + r] = lse2;
               }
             }
-            if (to >= 0) {
-              const int64_t at = (int64_t)(2 * p.ctas + to) * ROWS + r;
-              *reinterpret_cast<float4*>(p.part_o + at * D + col) = acc;
-              if (col == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, sum);
-              continue;
+          };
+          // arrive at a counter that `of` CTAs share; true for the last one, which zeroes it
+          auto arrive = [&](int* counter, int of) {
+            consumer_sync();
+            if (tid == 0) {
+              __threadfence();   // the whole CTA's stores, which the barrier put in front of it
+              const int is_last = atomicAdd(counter, 1) == of - 1;
+              if (is_last) {
+                *counter = 0;
+                __threadfence();
+              }
+              *s_last = is_last;
             }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            const int R = rt * ROWS + r, t = R / p.G, g = R - t * p.G;
-            const int64_t row = ((int64_t)sb * p.HQ + sh * p.G + g) * p.T + t;
-            *reinterpret_cast<uint2*>(p.out + row * D + col) =
-                make_uint2(pack2<HALF>(acc.x * inv, acc.y * inv), pack2<HALF>(acc.z * inv, acc.w * inv));
-            if (col == 0) {
-              const float lse2 = sum == 0.f ? -INFINITY : finite_or_zero(mm) + log2f(sum);
-              if (p.lse) p.lse[row] = lse2 * 0.6931471805599453f;
-              if (p.row_lse2) p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + R] = lse2;
-            }
+            consumer_sync();
+            return *s_last != 0;
+          };
+          const int grp = (blockIdx.x - c0) / kGroup;
+          const int in_group = min(kGroup, n - grp * kGroup);
+          // (a group of one needs no counter and no sum; its CTA may begin the next segment, whose first group
+          // has them there)
+          if (in_group == 1 || arrive(p.counters + p.ctas + c0 + grp * kGroup, in_group)) {
+            if (groups > 1 && in_group > 1) join(grp * kGroup, in_group, false, c0 + grp * kGroup);
+            if (groups == 1 || arrive(p.counters + c0, groups)) join(0, groups == 1 ? n : groups, groups > 1, -1);
           }
-        };
-        // arrive at a counter that `of` CTAs share; true for the last one, which zeroes it
-        auto arrive = [&](int* counter, int of) {
-          consumer_sync();
-          if (tid == 0) {
-            __threadfence();   // the whole CTA's stores, which the barrier put in front of it
-            const int is_last = atomicAdd(counter, 1) == of - 1;
-            if (is_last) {
-              *counter = 0;
-              __threadfence();
-            }
-            *s_last = is_last;
-          }
-          consumer_sync();
-          return *s_last != 0;
-        };
-        const int grp = (blockIdx.x - c0) / kGroup;
-        const int in_group = min(kGroup, n - grp * kGroup);
-        // (a group of one needs no counter and no sum; its CTA may begin the next segment, whose first group
-        // has them there)
-        if (in_group == 1 || arrive(p.counters + p.ctas + c0 + grp * kGroup, in_group)) {
-          if (groups > 1 && in_group > 1) join(grp * kGroup, in_group, false, c0 + grp * kGroup);
-          if (groups == 1 || arrive(p.counters + c0, groups)) join(0, groups == 1 ? n : groups, groups > 1, -1);
         }
-        consumer_sync();   // s_last and the statistics are free again
+        consumer_sync();   // the row statistics and s_last are free again
       }
     }
+  }
+  tc_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(C::TMEM));
   }
 }
 
 // token_weights[b, j] += sum over the heads and new tokens of 2^(x - lse2).
 // One thread per token, the rows in order: no atomics, a fixed order of sums.
-template <int TILE>
 __global__ void weights_kernel(const __grid_constant__ Params p, float* weights, int64_t weights_b) {
   extern __shared__ float lse2[];
   pdl_wait();
@@ -813,7 +1002,7 @@ __global__ void weights_kernel(const __grid_constant__ Params p, float* weights,
   for (int r = threadIdx.x; r < rows; r += blockDim.x) lse2[r] = finite_or_zero(p.row_lse2[(int64_t)b * rows + r]);
   __syncthreads();
   if (j >= len) return;
-  const Span s = span_of<TILE>(p, len);
+  const Span s = span_of(p, len);
   if (j < s.lo && j >= p.sinks) return;
   const float* src = p.scores + (int64_t)b * rows * p.score_stride + j;
   float sum = 0.f;
@@ -871,7 +1060,7 @@ static int num_sms_of(int given) {
 }
 
 struct Plan {
-  int G, R, mt, row_tiles, cap, ctas;
+  int G, R, n, row_tiles, cap, ctas;
   int64_t score_stride;
   size_t part_o, part_ml, lse2, scores;
 };
@@ -885,7 +1074,6 @@ static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
   Plan p;
   p.G = a->q_heads / a->kv_heads;
   const int64_t R = (int64_t)p.G * a->new_tokens;
-  const int tile = a->head_dim == 64 ? 128 : 64;
   // 2^30 keeps token positions and the rows' products inside 32 bits
   if (cap > (1 << 30) || R > (1 << 20) || (int64_t)a->batch * a->kv_heads * R > (1ll << 31) - 1)
     return KVR_ERR_UNSUPPORTED;
@@ -893,14 +1081,15 @@ static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
   if (a->token_weights && (a->kv_heads * R > 12000 || a->batch > 65535)) return KVR_ERR_UNSUPPORTED;
   p.R = (int)R;
   p.cap = (int)cap;
-  p.mt = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  p.row_tiles = (p.R + 16 * p.mt - 1) / (16 * p.mt);
-  const int64_t tiles = std::max<int64_t>(1, (cap + tile - 1) / tile + 1) * a->batch * a->kv_heads * p.row_tiles;
+  p.n = R <= 16 ? 16 : R <= 32 ? 32 : 64;   // rows of a tile
+  p.row_tiles = (p.R + p.n - 1) / p.n;
+  const int64_t tiles = std::max<int64_t>(1, (cap + kTile - 1) / kTile + 1 + kHead) * a->batch * a->kv_heads * p.row_tiles;
   if (tiles > (1ll << 31) - 1) return KVR_ERR_UNSUPPORTED;
-  // two CTAs per SM; a join takes kGroup^2 parts and some
-  p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, std::min(2 * num_sms_of(a->num_sms), kGroup * 20)));
+  // one or two CTAs per SM (Cfg::CTAS); a join takes kGroup^2 parts and some
+  const int per_sm = p.n == 16 || (p.n == 32 && a->head_dim == 64) ? 2 : 1;
+  p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, std::min(per_sm * num_sms_of(a->num_sms), kGroup * 20)));
   p.score_stride = std::max<int64_t>(128, (cap + 127) / 128 * 128);
-  const size_t rows = (size_t)16 * p.mt * 3 * p.ctas;
+  const size_t rows = (size_t)p.n * 3 * p.ctas;
   p.part_o = rows * a->head_dim * sizeof(float);
   p.part_ml = rows * 2 * sizeof(float);
   const size_t all_rows = (size_t)a->batch * a->kv_heads * p.R;
@@ -952,10 +1141,10 @@ struct Maps {
   CUtensorMap k, v;
 };
 
-template <bool HALF, int D, int MT, bool TMA>
+template <bool HALF, int D, int N, bool TMA>
 static int launch(const Params& p, const Maps& maps, cudaStream_t s) {
-  using C = Cfg<D, MT>;
-  auto kern = attention_kernel<HALF, D, MT, TMA>;
+  using C = Cfg<D, N>;
+  auto kern = attention_kernel<HALF, D, N, TMA>;
   static bool ready[64] = {false};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
@@ -971,14 +1160,14 @@ static int launch(const Params& p, const Maps& maps, cudaStream_t s) {
 }
 
 template <bool HALF, int D, bool TMA>
-static int launch_mt(int mt, const Params& p, const Maps& maps, cudaStream_t s) {
-  if (mt == 1) return launch<HALF, D, 1, TMA>(p, maps, s);
-  if (mt == 2) return launch<HALF, D, 2, TMA>(p, maps, s);
-  return launch<HALF, D, 4, TMA>(p, maps, s);
+static int launch_n(int n, const Params& p, const Maps& maps, cudaStream_t s) {
+  if (n == 16) return launch<HALF, D, 16, TMA>(p, maps, s);
+  if (n == 32) return launch<HALF, D, 32, TMA>(p, maps, s);
+  return launch<HALF, D, 64, TMA>(p, maps, s);
 }
 template <bool HALF, int D>
-static int launch_tma(bool tma, int mt, const Params& p, const Maps& maps, cudaStream_t s) {
-  return tma ? launch_mt<HALF, D, true>(mt, p, maps, s) : launch_mt<HALF, D, false>(mt, p, maps, s);
+static int launch_tma(bool tma, int n, const Params& p, const Maps& maps, cudaStream_t s) {
+  return tma ? launch_n<HALF, D, true>(n, p, maps, s) : launch_n<HALF, D, false>(n, p, maps, s);
 }
 
 }  // namespace paged
@@ -1035,7 +1224,7 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   p.G = pl.G; p.R = pl.R; p.row_tiles = pl.row_tiles;
   p.window = a->window; p.sinks = a->window > 0 ? a->sinks : 0; p.cap = pl.cap;
   p.scale2 = a->scale * 1.4426950408889634f;
-  p.ctas = pl.ctas; p.min_tiles = 1;
+  p.ctas = pl.ctas;
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + pl.part_o);
   p.counters = a->counters;
@@ -1043,8 +1232,7 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   const bool half = a->dtype == 1;
   // TMA boxes: the largest number of tokens that divides both a page and a
   // tile; below 8 rows (one swizzle pattern) the rows are copied one by one.
-  const int tile = a->head_dim == 64 ? 128 : 64;
-  int box = tile;
+  int box = paged::kTile;
   while (a->page_size % box) box /= 2;
   p.box = box;
   paged::Maps maps;
@@ -1055,17 +1243,14 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
                    paged::page_map(&maps.v, a->value_pages, half, a->head_dim, a->page_size, a->kv_heads, a->num_pages,
                                    a->value_row_stride, a->value_head_stride, a->value_page_stride, box);
   if (a->head_dim == 64)
-    st = half ? paged::launch_tma<true, 64>(tma, pl.mt, p, maps, s) : paged::launch_tma<false, 64>(tma, pl.mt, p, maps, s);
+    st = half ? paged::launch_tma<true, 64>(tma, pl.n, p, maps, s) : paged::launch_tma<false, 64>(tma, pl.n, p, maps, s);
   else
-    st = half ? paged::launch_tma<true, 128>(tma, pl.mt, p, maps, s) : paged::launch_tma<false, 128>(tma, pl.mt, p, maps, s);
+    st = half ? paged::launch_tma<true, 128>(tma, pl.n, p, maps, s) : paged::launch_tma<false, 128>(tma, pl.n, p, maps, s);
   if (st != KVR_OK || !a->token_weights || pl.cap == 0) return st;
   const int rows = p.HKV * p.R;
   const dim3 grid((pl.cap + 255) / 256, p.B);
-  cudaError_t e = a->head_dim == 64
-                      ? pdl_launch(paged::weights_kernel<128>, grid, dim3(256), rows * sizeof(float), s, 1, p,
-                                   a->token_weights, a->weights_b_stride)
-                      : pdl_launch(paged::weights_kernel<64>, grid, dim3(256), rows * sizeof(float), s, 1, p,
-                                   a->token_weights, a->weights_b_stride);
+  cudaError_t e = pdl_launch(paged::weights_kernel, grid, dim3(256), rows * sizeof(float), s, 1, p, a->token_weights,
+                             a->weights_b_stride);
   if (e != cudaSuccess) { set_last_cuda_error(e); return KVR_ERR_CUDA; }
   return KVR_OK;
 }
