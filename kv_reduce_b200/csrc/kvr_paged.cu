@@ -325,7 +325,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
     bar_init(q_full, 1);
     bar_init_fence();
   }
-  pdl_wait();
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
+                 "r"(C::TMEM)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    tc_before_sync();
+  }
+  auto free_tmem = [&]() {
+    if (warp == kMmaWarp)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(*s_tmem), "r"(C::TMEM));
+  };
+  pdl_enter();
 
   // ---- this CTA's range of the flat tile list
   const int HR = p.HKV * p.row_tiles;
@@ -353,7 +364,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
     total *= HR;
     ctas = min(p.ctas, total);
     const int me = blockIdx.x;
-    if (me >= ctas) return;
+    if (me >= ctas) {
+      free_tmem();
+      return;
+    }
     const Cut cut(total, ctas);
     g0 = cut.begin(me);
     const int g1 = cut.begin(me + 1);
@@ -386,17 +400,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
     }
     if (tid == 0 && g1 == total) s_start[6] = total - kHead * p.B * HR;
     __syncthreads();
-    count = s_start[6] - s_start[4];
-    if (count == 0) return;   // nothing but heads
-    if (warp == kMmaWarp) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
-                   "r"(C::TMEM)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
-    }
-    tc_before_sync();
-    __syncthreads();
     tc_after_sync();
+    count = s_start[6] - s_start[4];
+    if (count == 0) {   // nothing but heads
+      __syncwarp();
+      free_tmem();
+      return;
+    }
   }
   const uint32_t tmem = *s_tmem, tmem_o = tmem + 2 * N;
   bool failed = false;
@@ -605,19 +615,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
     // the registers).
     constexpr int QV = N * C::PIECES / kConsumers;
     uint4 q[QV];
-    auto load_queries = [&](const Desc& d) {
+    auto load_queries = [&](int b, int h, int rt) {
 #pragma unroll
       for (int y = 0; y < QV; ++y) {
-        const int r = (y * kConsumers + tid) / C::PIECES, c = tid % C::PIECES, R = d.rt * N + r;
+        const int r = (y * kConsumers + tid) / C::PIECES, c = tid % C::PIECES, R = rt * N + r;
         q[y] = make_uint4(0, 0, 0, 0);
         if (R < p.R) {
           const int t = R / p.G, g = R - t * p.G;
-          q[y] = *reinterpret_cast<const uint4*>(p.q + (int64_t)d.b * p.q_b + (int64_t)(d.h * p.G + g) * p.q_h +
+          q[y] = *reinterpret_cast<const uint4*>(p.q + (int64_t)b * p.q_b + (int64_t)(h * p.G + g) * p.q_h +
                                                  (int64_t)t * p.q_t + c * 8);
         }
       }
     };
     constexpr bool kAhead = N <= 32;
+    load_queries(s_start[0], s_start[2] / p.row_tiles, s_start[2] % p.row_tiles);
     for (int i = 0; i < count; ++i) {
       bar_wait(ready + 8 * (i & (C::DESCS - 1)), (i / C::DESCS) & 1, failed);
       const Desc& ds = *desc_at(i);
@@ -627,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       uint8_t* vs = smem + v_slot * C::UNIT;
 
       if (ds.first) {
-        if (!kAhead || i == 0) load_queries(ds);
+        if (!kAhead && i > 0) load_queries(ds.b, ds.h, rt);
 #pragma unroll
         for (int y = 0; y < QV; ++y) {
           const int r = (y * kConsumers + tid) / C::PIECES, c = tid % C::PIECES;
@@ -844,7 +855,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       if (last) {
         if (kAhead && i + 1 < count) {   // the next segment's queries
           bar_wait(ready + 8 * ((i + 1) & (C::DESCS - 1)), ((i + 1) / C::DESCS) & 1, failed);
-          load_queries(*desc_at(i + 1));
+          const Desc& dn = *desc_at(i + 1);
+          load_queries(dn.b, dn.h, dn.rt);
         }
         // ---- the rows' sums over the tokens' threads, while the last product runs
         if (failed)
@@ -913,11 +925,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
               float mm = kUnseen, sum = 0.f;
               float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 1
-              for (int kb = 0; kb < cnt; kb += 4) {
-                float2 ml[4];
-                float4 f[4];
+              for (int kb = 0; kb < cnt; kb += 8) {
+                float2 ml[8];
+                float4 f[8];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
+                for (int y = 0; y < 8; ++y) {
                   ml[y] = make_float2(kUnseen, 0.f);
                   f[y] = make_float4(0.f, 0.f, 0.f, 0.f);
                   if (kb + y < cnt) {
@@ -926,13 +938,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
                     f[y] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + col));
                   }
                 }
-                const float mn = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), mm);
+                float mn = mm;
+#pragma unroll
+                for (int y = 0; y < 8; ++y) mn = fmaxf(mn, ml[y].x);
                 const float alpha = fast_exp2(mm - mn);
                 mm = mn;
                 sum *= alpha;
                 acc.x *= alpha; acc.y *= alpha; acc.z *= alpha; acc.w *= alpha;
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
+                for (int y = 0; y < 8; ++y) {
                   const float w = fast_exp2(ml[y].x - mn);
                   sum += w * ml[y].y;
                   acc.x += w * f[y].x; acc.y += w * f[y].y; acc.z += w * f[y].z; acc.w += w * f[y].w;
@@ -986,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_after_sync();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(C::TMEM));
+    free_tmem();
   }
 }
 
