@@ -548,9 +548,11 @@ static int plan_of(const kvr_verify_args* a, Plan* out) {
   p.seg_blocks = 4 * 32 * kUnroll;
   while (p.seg_blocks > 32 * kUnroll && rows * ((blocks + p.seg_blocks - 1) / p.seg_blocks) < 148 * 32) p.seg_blocks /= 2;
   p.segments = (int)((blocks + p.seg_blocks - 1) / p.seg_blocks);
-  p.race_blocks = 8 * 32;   // 8 blocks a lane: 2, 4, 16, 32 took 7, 2, 4 and 16 us longer on the same
+  // the race: 8 blocks a lane (2, 4, 16, 32 took 7, 2, 4 and 16 us longer on the same), fewer while that leaves
+  // half of the warps out
+  p.race_blocks = 8 * 32;
   while (p.race_blocks > 32 * kRaceUnroll &&
-         (int64_t)a->batch * ((blocks + p.race_blocks - 1) / p.race_blocks) < 148 * 32)
+         (int64_t)a->batch * ((blocks + p.race_blocks - 1) / p.race_blocks) < 148 * 16)
     p.race_blocks /= 2;
   p.race_segments = (int)((blocks + p.race_blocks - 1) / p.race_blocks);
   if (rows * p.segments > (1ll << 31) - 1 || (int64_t)a->batch * p.race_segments > (1ll << 31) - 1)
