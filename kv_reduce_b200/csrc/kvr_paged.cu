@@ -142,6 +142,7 @@ struct Desc {
   int b, h, rt, len;
   int n_tiles, seg_start;          // of the segment: tiles, flat index of the first
   int whole;                       // with `last`: all of the segment's tiles are this CTA's
+  uint32_t groups;                 // 16-token groups that a query sees, a bit each (one at least)
   uint32_t bad[4];   // tokens on pages outside the pool, a bit each
 };
 static_assert(sizeof(Desc) <= 64, "");
@@ -443,13 +444,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
     for (int i = 0; i < count; ++i) {
       bar_wait(ready + 8 * (i & (C::DESCS - 1)), (i / C::DESCS) & 1, failed);
       const bool first = desc_at(i)->first, last = desc_at(i)->last;
+      const uint32_t groups = desc_at(i)->groups;
       // the next tile's scores go first, unless its queries come after this segment's output
       if (!last && i + 1 < count) scores(i + 1, false);
       const int u = 2 * i + 1, slot = u % U;
       bar_wait(full + 8 * slot, (u / U) & 1, failed);
       bar_wait(p_full, i & 1, failed);
       tc_after_sync();
-      const bool add = !first || *s_add;
+      bool add = !first || *s_add;
       __syncwarp();
       const uint64_t v_op = operand(sbase + slot * C::UNIT, C::HALF_BYTES);
       if (elect_one()) {
@@ -457,7 +459,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
         if (!failed)
 #pragma unroll
           for (int kk = 0; kk < TILE / 16; ++kk)
-            mma(tmem_o, v_op + (kk * 2048 >> 4), p_op + (kk * 16 * C::P_ROW >> 4), o_kind, add || kk > 0);
+            if ((groups >> kk) & 1) {
+              mma(tmem_o, v_op + (kk * 2048 >> 4), p_op + (kk * 16 * C::P_ROW >> 4), o_kind, add);
+              add = true;
+            }
         mma_commit(empty + 8 * slot);
         mma_commit(o_done);
       }
@@ -499,6 +504,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       --ld_left;
       u.d.last = ld_left == 0 || ld_tile + 1 == ld_span.n;
       u.d.whole = ld_from == 0 && ld_tile + 1 == ld_span.n;
+      {
+        const int j = token0 + (lane & 7) * 16;
+        u.d.groups = __ballot_sync(0xffffffffu, j < ld_len && (j + 16 > ld_span.lo || j < p.sinks)) & 0xffu;
+        if (u.d.groups == 0) u.d.groups = 1;
+      }
       const int step = TMA ? p.box : 1;
 #pragma unroll
       for (int x = 0; x < LU; ++x) {
@@ -661,14 +671,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       const bool full_tile = ds.full;
       const int lo = p.window > 0 ? max(0, max(len - p.T, 0) - p.window + 1) : 0;
       if (!full_tile) {
-        // rows of V that no query sees hold whatever the page or an earlier
-        // tile left there, and 0 * NaN is NaN: zero them
+        // Rows of V that no query sees hold whatever the page or an earlier
+        // tile left there, and 0 * NaN is NaN: where their group of 16 is
+        // multiplied, they are zeroed (thread = token).
         bar_wait(full + 8 * v_slot, (v_unit / U) & 1, failed);
-        for (int x = tid; x < TILE * C::PIECES; x += kConsumers) {
-          const int r = x / C::PIECES, c = x % C::PIECES, j = token0 + r;
-          if (j < len && (j >= lo || j < p.sinks) && !((ds.bad[r >> 5] >> (r & 31)) & 1)) continue;
-          *reinterpret_cast<uint4*>(vs + (c >> 3) * C::HALF_BYTES + r * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
-        }
+        const int j = token0 + tid;
+        if (((ds.groups >> (tid >> 4)) & 1) &&
+            (!(j < len && (j >= lo || j < p.sinks)) || ((ds.bad[warp] >> lane) & 1)))
+#pragma unroll
+          for (int c = 0; c < C::PIECES; ++c)
+            *reinterpret_cast<uint4*>(vs + (c >> 3) * C::HALF_BYTES + tid * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
       }
 
       // ---- scores: thread = token, registers = rows

@@ -320,10 +320,13 @@ __global__ void __launch_bounds__(kThreads, 8) stats_kernel(const __grid_constan
 }
 
 // The sequence's outputs, and its zeros for the next call, by one warp.
-__device__ __forceinline__ void write_out(const Params& p, int b, int at, int64_t token, int best_rows) {
-  const int n_draft = drafted(p, b), lane = threadIdx.x & 31;
+// `drafted_token`: tokens[lane], read ahead (the first 32).
+__device__ __forceinline__ void write_out(const Params& p, int b, int n_draft, int at, int64_t token,
+                                          int64_t drafted_token, int best_rows) {
+  const int lane = threadIdx.x & 31;
   for (int k = lane; k <= p.K; k += 32) {
-    p.out_tokens[(int64_t)b * (p.K + 1) + k] = k < at ? p.tokens[(int64_t)b * p.tok_b + k] : k == at ? token : -1;
+    const int64_t old = k == lane ? drafted_token : k < at ? p.tokens[(int64_t)b * p.tok_b + k] : -1;
+    p.out_tokens[(int64_t)b * (p.K + 1) + k] = k < at ? old : k == at ? token : -1;
     if (k < p.K && (k > at || k >= n_draft)) p.accept_prob[b * p.K + k] = 0.f;
     p.arrived[b * (p.K + 1) + k] = 0;
     if (k < best_rows) p.best[(int64_t)b * best_rows + k] = 0;
@@ -333,6 +336,10 @@ __device__ __forceinline__ void write_out(const Params& p, int b, int at, int64_
     p.done[b] = 0;
     p.refused[b] = 0;
   }
+}
+__device__ __forceinline__ int64_t token_ahead(const Params& p, int b) {
+  const int lane = threadIdx.x & 31;
+  return lane < p.K ? p.tokens[(int64_t)b * p.tok_b + lane] : -1;
 }
 
 // The noise of a block of N elements.
@@ -417,6 +424,7 @@ __global__ void __launch_bounds__(kThreads, 8) race_kernel(const __grid_constant
     }
   }
   unsigned long long best = lanes_best(where < 0 ? 0ull : race_key(top, where));
+  const int64_t ahead = token_ahead(p, b);
   int last = 0;
   if (lane == 0) {
     if (best) atomicMax(p.best + b, best);
@@ -437,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 8) race_kernel(const __grid_constant
     }
     best = lanes_best(where < 0 ? 0ull : race_key(top, where));
   }
-  write_out(p, b, at, race_index(best), 1);
+  write_out(p, b, n_draft, at, race_index(best), ahead, 1);
 }
 
 // t = 0: x_k is accepted while it is the argmax of target_k (the lowest index
@@ -490,6 +498,7 @@ __global__ void __launch_bounds__(kThreads, 8) greedy_kernel(const __grid_consta
   if (lane == 0) buf[threadIdx.x >> 5] = best;
   __syncthreads();
   if (threadIdx.x >= 32) return;
+  const int64_t ahead = token_ahead(p, b);
   int last = 0;
   if (lane == 0) {
 #pragma unroll
@@ -509,17 +518,19 @@ __global__ void __launch_bounds__(kThreads, 8) greedy_kernel(const __grid_consta
   if (!__shfl_sync(~0u, last, 0)) return;
   // the sequence's last CTA: the first token that is not its row's argmax (rows behind it may be unread)
   const volatile unsigned long long* rows = p.best + (int64_t)b * (p.K + 1);
+  const unsigned long long mine = lane <= n_draft ? rows[lane] : 0ull;
   int at = n_draft;
   for (int i = lane; i < n_draft; i += 32) {
-    const int64_t x = race_index(rows[i]);
-    if (x < 0 || x != p.tokens[(int64_t)b * p.tok_b + i]) at = min(at, i);
+    const int64_t x = race_index(i == lane ? mine : rows[i]);
+    if (x < 0 || x != (i == lane ? ahead : p.tokens[(int64_t)b * p.tok_b + i])) at = min(at, i);
   }
   at = __reduce_min_sync(~0u, at);
   for (int i = lane; i < at; i += 32) p.accept_prob[b * p.K + i] = 1.f;
   if (lane == 0 && at < n_draft) p.accept_prob[b * p.K + at] = 0.f;
-  const int64_t token = race_index(rows[at]);
+  const unsigned long long here = __shfl_sync(~0u, mine, at & 31);
+  const int64_t token = race_index(at < 32 ? here : rows[at]);
   __syncwarp();
-  write_out(p, b, at, token, p.K + 1);
+  write_out(p, b, n_draft, at, token, ahead, p.K + 1);
 }
 
 // ------------------------------------------------------------------- host
