@@ -87,7 +87,8 @@ struct Params {
   int64_t v_page, v_head, v_row;
   const int* table;
   int64_t table_b;
-  int table_width, num_pages, page;
+  int num_pages, page, page_shift;
+  uint32_t page_magic;   // j / page = j * page_magic >> page_shift for j < 2^30
   const int* lengths;
   uint16_t* out;
   float* lse;       // [B, HQ, T] or null
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
   int* row_s = pos_s + N;          // the rows of the output
   float* smax = alpha_s + 3 * N;   // [4][N]
   float* ssum = smax + 4 * N;      // [4][N]
-  // A ring unit's data is there / is read; a tile's descriptor is there (before its data); score tile done / read;
+  // (in this order)  A ring unit's data is there / is read; a tile's descriptor is there (before its data); score tile done / read;
   // P written; the output up to a tile done; a segment's queries written.
   const uint32_t full = sbase + C::OFF_BAR, empty = full + 8 * U, ready = empty + 8 * U, s_full = ready + 8 * C::DESCS,
                  s_empty = s_full + 16, p_full = s_empty + 16, o_done = p_full + 8, q_full = o_done + 8;
@@ -312,19 +313,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_last + 1);
   int* s_add = s_last + 2;                                     // the output holds something before its first product
 
-  if (tid == 0) {
-    for (int i = 0; i < U; ++i) {
-      bar_init(full + 8 * i, 1);
-      bar_init(empty + 8 * i, 1);
-    }
-    for (int i = 0; i < C::DESCS; ++i) bar_init(ready + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) {
-      bar_init(s_full + 8 * i, 1);
-      bar_init(s_empty + 8 * i, kWarps);
-    }
-    bar_init(p_full, kWarps);
-    bar_init(o_done, 1);
-    bar_init(q_full, 1);
+  if (tid < C::BARS) {
+    // (s_empty and p_full are arrived at by the consumers' warps, the others by one thread)
+    const uint32_t bar = full + 8 * tid;
+    bar_init(bar, (bar >= s_empty && bar <= p_full) ? kWarps : 1);
     bar_init_fence();
   }
   if (warp == kMmaWarp) {
@@ -344,10 +336,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
   const int HR = p.HKV * p.row_tiles;
   int total, ctas, g0, count;   // units in all, CTAs that take part, this one's first unit, and its tiles
   {
-    const int per = (p.B + kThreads - 1) / kThreads;
-    const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += span_of(p, length_of(p, b)).n + kHead;
+    // three warps find the first unit's sequence, three the end's
+    constexpr int kHalf = kThreads / 2;
+    const int half = tid >= kHalf, t = tid - half * kHalf;
+    const int per = (p.B + kHalf - 1) / kHalf;
+    const int b0 = min(t * per, p.B), b1 = min(b0 + per, p.B);
+    int mine = 0, raw0 = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int raw = p.lengths[b];
+      if (b == b0) raw0 = raw;
+      mine += span_of(p, min(max(raw, 0), p.cap)).n + kHead;
+    }
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -359,8 +358,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
     int before = incl - mine;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += s_scan[w];
+    for (int w = 0; w < kHalf / 32; ++w) {
+      if (w + half * (kHalf / 32) < warp) before += s_scan[w];   // (both halves' sums are the same)
       total += s_scan[w];
     }
     total *= HR;
@@ -372,32 +371,26 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
     }
     const Cut cut(total, ctas);
     g0 = cut.begin(me);
-    const int g1 = cut.begin(me + 1);
-    // the threads whose sequences hold units g0 and g1 find the sequences
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const int g = which ? g1 : g0;
-      if (mine > 0 && before * HR <= g && g < (before + mine) * HR) {
-        int b = b0, at = before;
-        int raw = p.lengths[b];
-        int nb = span_of(p, min(max(raw, 0), p.cap)).n + kHead;
-        while (g >= (at + nb) * HR) {
-          at += nb;
-          raw = p.lengths[++b];
-          nb = span_of(p, min(max(raw, 0), p.cap)).n + kHead;
-        }
-        const int off = g - at * HR, hr = off / nb, in_seg = off - hr * nb;
-        // tiles in front of unit g: those units less the heads in front
-        const int tiles = g - kHead * (b * HR + hr) - min(in_seg, kHead);
-        if (which) {
-          s_start[6] = tiles;
-        } else {
-          s_start[0] = b;
-          s_start[1] = raw;
-          s_start[2] = hr;
-          s_start[3] = max(in_seg - kHead, 0);
-          s_start[4] = tiles;
-        }
+    const int g1 = cut.begin(me + 1), g = half ? g1 : g0;
+    if (mine > 0 && before * HR <= g && g < (before + mine) * HR) {   // this thread's sequences hold unit g
+      int b = b0, at = before, raw = raw0;
+      int nb = span_of(p, min(max(raw, 0), p.cap)).n + kHead;
+      while (g >= (at + nb) * HR) {
+        at += nb;
+        raw = p.lengths[++b];
+        nb = span_of(p, min(max(raw, 0), p.cap)).n + kHead;
+      }
+      const int off = g - at * HR, hr = off / nb, in_seg = off - hr * nb;
+      // tiles in front of unit g: the units less the heads in front
+      const int tiles = g - kHead * (b * HR + hr) - min(in_seg, kHead);
+      if (half) {
+        s_start[6] = tiles;
+      } else {
+        s_start[0] = b;
+        s_start[1] = raw;
+        s_start[2] = hr;
+        s_start[3] = max(in_seg - kHead, 0);
+        s_start[4] = tiles;
       }
     }
     if (tid == 0 && g1 == total) s_start[6] = total - kHead * p.B * HR;
@@ -491,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       if (ld_left <= 0) return;
       const int token0 = (ld_tile < ld_span.ns ? ld_tile : ld_span.lo_tile + ld_tile - ld_span.ns) * TILE;
       u.d.b = ld_b;
-      u.d.h = ld_hr / p.row_tiles;
+      u.d.h = p.row_tiles == 1 ? ld_hr : ld_hr / p.row_tiles;
       u.d.rt = ld_hr - u.d.h * p.row_tiles;
       u.d.token0 = token0;
       u.d.len = ld_len;
@@ -517,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
         u.id[x] = 0;
         u.row[x] = 0;
         if (at < TILE && j < ld_len && (j + step > ld_span.lo || j < p.sinks)) {
-          const int pg = j / p.page;
+          const int pg = (int)((uint64_t)(uint32_t)j * p.page_magic >> p.page_shift);   // j / page
           u.row[x] = j - pg * p.page;
           u.state[x] = ld_over ? 2 : 1;
           u.id[x] = __ldg(p.table + (int64_t)ld_b * p.table_b + pg);
@@ -1249,7 +1242,13 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   p.v = static_cast<const uint16_t*>(a->value_pages);
   p.v_page = a->value_page_stride; p.v_head = a->value_head_stride; p.v_row = a->value_row_stride;
   p.table = a->block_table; p.table_b = a->table_stride;
-  p.table_width = a->table_width; p.num_pages = a->num_pages; p.page = a->page_size;
+  p.num_pages = a->num_pages; p.page = a->page_size;
+  // Division by the page size as a product: with 2^s >= page and m = ceil(2^(30+s) / page), m page exceeds 2^(30+s)
+  // by less than 2^s, so j m / 2^(30+s) exceeds j / page by less than 1 / page for j < 2^30.  m < 2^32.
+  int shift = 0;
+  while ((1ll << shift) < a->page_size) ++shift;
+  p.page_shift = 30 + shift;
+  p.page_magic = (uint32_t)(((1ull << p.page_shift) + a->page_size - 1) / a->page_size);
   p.lengths = a->lengths;
   p.out = static_cast<uint16_t*>(a->out);
   p.lse = a->lse;
