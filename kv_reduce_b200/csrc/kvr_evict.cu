@@ -236,7 +236,7 @@ constexpr int kCopyTokens = 32, kCopyThreads = 256;
 
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ kvr_paged_evict_args a) {
   __shared__ int64_t src[kCopyTokens][2], dst[kCopyTokens][2];
-  pdl_wait();
+  pdl_wait();   // (and no early trigger: a selection that starts beside this kernel's last CTAs slows them by a tenth)
   const int b = blockIdx.y, i0 = blockIdx.x * kCopyTokens;
   if (threadIdx.x < kCopyTokens) {
     const int i = i0 + threadIdx.x;

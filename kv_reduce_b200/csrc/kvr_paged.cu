@@ -1023,7 +1023,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
 // One thread per token, the rows in order: no atomics, a fixed order of sums.
 __global__ void weights_kernel(const __grid_constant__ Params p, float* weights, int64_t weights_b) {
   extern __shared__ float lse2[];
-  pdl_wait();
+  pdl_enter();
   const int b = blockIdx.y, rows = p.HKV * p.R;
   const int len = length_of(p, b);
   const int j = blockIdx.x * blockDim.x + threadIdx.x;

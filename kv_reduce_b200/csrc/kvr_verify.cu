@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 8) stats_kernel(const __grid_constan
   const int seg = unit % p.segments, row = unit / p.segments;   // row = (k * B + b) * 2 + (draft)
   const int side = row & 1, k = (row >> 1) / p.B, b = (row >> 1) - k * p.B;
   if (k >= p.K) return;
-  pdl_wait();
+  pdl_enter();
   const int n_draft = drafted(p, b);
   if (k >= n_draft) return;
   if (p.skip && k > 0 && refused_at(p, b) < k) return;   // an earlier position of this sequence is refused already
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 8) race_kernel(const __grid_constant
   const int unit = blockIdx.x * kWarps + (threadIdx.x >> 5), b = unit / p.race_segments;
   if (b >= p.B) return;
   const int begin = (unit - b * p.race_segments) * p.race_blocks, end = min(begin + p.race_blocks, blocks_of<T>(p.V));
-  pdl_wait();
+  pdl_enter();
   const int n_draft = drafted(p, b), at = min(refused_at(p, b), n_draft);
   const bool residual = at < n_draft;
   const float* noise = p.noise + (int64_t)b * p.n_b;
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 8) greedy_kernel(const __grid_consta
   const int seg = (blockIdx.x - row * chunks) * kWarps + (threadIdx.x >> 5);
   __shared__ unsigned long long buf[kWarps];
   __shared__ int s_unread;
-  pdl_wait();
+  pdl_enter();
   const int n_draft = drafted(p, b);
   bool unread = k > n_draft;
   if (p.skip && k > 0) {   // one look for the whole CTA
