@@ -465,7 +465,8 @@ int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream_t stream);
  * order, into the pages of new_block_table, which must not be pages that a
  * block table still uses.  Writes kept [B, keep] (old positions, rising, -1
  * behind the last), new_lengths [B], new_weights [B, keep] (0 behind the
- * last).  Rows whose page number is not in the pool are not copied.
+ * last), none of them in place.  Rows whose page number is not in the pool
+ * are not copied.
  * table_width*page_size <= 320000; new_table_width*page_size must hold
  * min(keep, table_width*page_size) tokens (KVR_ERR_CAPACITY).              */
 typedef struct {

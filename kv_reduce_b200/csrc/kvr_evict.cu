@@ -14,7 +14,14 @@
 //  * copy_kernel: the kept rows into the new pages, all heads of a token by
 //    the same CTA.  What bounds it is the rows' bytes, read once and written
 //    once; the new pages are others than the old, so the order of copies does
-//    not matter and pages that sequences share stay as they are.
+//    not matter and pages that sequences share stay as they are.  The last
+//    `recent` tokens are kept whatever the weights say: their rows are copied
+//    while the selection runs.
+//
+// Measured (bf16): 32 sequences of 4K to 16K to 4096, of them 1024 recent, 8
+// heads of 64: 0.54 GB in 99 us, 5450 GB/s (107 us without the early copies;
+// the copy alone runs at 94% of a plain copy's rate, the selection takes 15
+// us); one of 5000 to 1024, 2 heads of 128: 11 us, the selection's latency.
 #include "kvr_common.cuh"
 
 #include <algorithm>
@@ -118,7 +125,9 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   __shared__ int s_digit[2];
   const int tid = threadIdx.x, rank = CL == 1 ? 0 : blockIdx.x % CL, b = blockIdx.x / CL;
   for (int i = tid; i < 2 * kBins; i += kThreads) (&hist[0][0])[i] = 0;
-  pdl_enter();
+  // what came before is done: now the copies that need no selection may start
+  pdl_wait();
+  pdl_trigger();
   const int len = min(max(p.lengths[b], 0), p.cap);
   const float* w = p.weights + (int64_t)b * p.weights_b;
   int* kept = p.kept + (int64_t)b * p.keep;
@@ -234,14 +243,31 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
 
 constexpr int kCopyTokens = 32, kCopyThreads = 256;
 
-__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ kvr_paged_evict_args a) {
+// Blocks of kCopyTokens slots; first the `early` last ones of every sequence,
+// which hold recent tokens only, then the others.
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ kvr_paged_evict_args a, int blocks,
+                                                            int early, int cap) {
   __shared__ int64_t src[kCopyTokens][2], dst[kCopyTokens][2];
-  pdl_wait();   // (and no early trigger: a selection that starts beside this kernel's last CTAs slows them by a tenth)
-  const int b = blockIdx.y, i0 = blockIdx.x * kCopyTokens;
+  const int n_early = a.batch * early, late = blocks - early;
+  const bool is_early = (int)blockIdx.x < n_early;
+  const int u = is_early ? blockIdx.x : blockIdx.x - n_early;
+  const int b = u / (is_early ? early : late), i0 = (is_early ? late + u % early : u % late) * kCopyTokens;
+  // The selection passed its own wait before this kernel could start, so lengths, tables and pages are there;
+  // `kept` is only behind this one's wait.  (No early trigger here: a selection that starts beside this kernel's
+  // last CTAs slows them by a tenth.)
+  if (!is_early) pdl_wait();
   if (threadIdx.x < kCopyTokens) {
     const int i = i0 + threadIdx.x;
     int64_t s = -1, sv = 0, d = 0, dv = 0;
-    const int j = i < a.keep ? a.kept[(int64_t)b * a.keep + i] : -1;
+    int j = -1;
+    if (i < a.keep) {
+      if (is_early) {
+        const int len = min(max(a.lengths[b], 0), cap);
+        j = len > a.keep ? len - a.keep + i : i < len ? i : -1;
+      } else {
+        j = a.kept[(int64_t)b * a.keep + i];
+      }
+    }
     if (j >= 0) {
       const int from = a.block_table[(int64_t)b * a.table_stride + j / a.page_size];
       const int to = i / a.page_size < a.new_table_width
@@ -274,6 +300,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
     *reinterpret_cast<uint4*>(kp + dst[t][0] + ko) = k;
     *reinterpret_cast<uint4*>(vp + dst[t][1] + vo) = v;
   }
+  if (is_early) pdl_wait();   // this kernel must not be done before the selection
 }
 
 // Slices of at most 40,000 weights: 160 KB of shared memory, counts of 16 bits.
@@ -313,6 +340,8 @@ extern "C" int kvr_paged_evict(const kvr_paged_evict_args* a, kvr_stream_t strea
       (cap > 0 && (!a->block_table || !a->new_block_table || !a->token_weights)) ||
       (a->num_pages > 0 && (!a->key_pages || !a->value_pages)))
     return KVR_ERR_INVALID_ARGUMENT;
+  // every CTA of a sequence reads what these would overwrite
+  if (a->new_lengths == a->lengths || a->new_weights == a->token_weights) return KVR_ERR_INVALID_ARGUMENT;
   const int64_t strides[] = {a->key_page_stride, a->key_head_stride, a->key_row_stride,
                              a->value_page_stride, a->value_head_stride, a->value_row_stride};
   for (int64_t x : strides)
@@ -337,10 +366,15 @@ extern "C" int kvr_paged_evict(const kvr_paged_evict_args* a, kvr_stream_t strea
                   : cluster == 2 ? evict::launch_select<2>(p, a->batch, s)
                                  : evict::launch_select<1>(p, a->batch, s);
   const int64_t rows = std::min<int64_t>(a->keep, cap);
-  if (e == cudaSuccess && rows > 0)
-    e = pdl_launch(evict::copy_kernel,
-                   dim3((unsigned)((rows + evict::kCopyTokens - 1) / evict::kCopyTokens), (unsigned)a->batch),
-                   dim3(evict::kCopyThreads), 0, s, 1, *a);
+  if (e == cudaSuccess && rows > 0) {
+    // slots [keep - recent, keep): whole blocks of them need no selection
+    const int blocks = (int)((rows + evict::kCopyTokens - 1) / evict::kCopyTokens);
+    const int first_early = (a->keep - a->recent + evict::kCopyTokens - 1) / evict::kCopyTokens;
+    const int early = std::max(0, blocks - first_early);
+    if ((int64_t)blocks * a->batch > (1ll << 31) - 1) return KVR_ERR_UNSUPPORTED;
+    e = pdl_launch(evict::copy_kernel, dim3((unsigned)(blocks * a->batch)), dim3(evict::kCopyThreads), 0, s, 1, *a, blocks,
+                   early, (int)cap);
+  }
   if (e != cudaSuccess) { set_last_cuda_error(e); return KVR_ERR_CUDA; }
   return KVR_OK;
 }

@@ -126,6 +126,10 @@ def test_c_abi_refusals(built_lib):
     assert lib.kvr_paged_evict(e, None) == _lib.KVR_ERR_INVALID_ARGUMENT      # null pointers
     e.keep = 40
     assert lib.kvr_paged_evict(e, None) == _lib.KVR_ERR_CAPACITY
+    e.keep = 8                               # lengths in place (refused before a pointer is read)
+    e.lengths = e.new_lengths = e.kept = e.new_weights = e.block_table = e.new_block_table = 64
+    e.token_weights = e.key_pages = e.value_pages = 128
+    assert lib.kvr_paged_evict(e, None) == _lib.KVR_ERR_INVALID_ARGUMENT
     v = _lib.VerifyArgs()
     v.batch, v.draft_tokens, v.vocab, v.temperature = 1, 2, 100, -1.0
     assert lib.kvr_verify(v, None) == _lib.KVR_ERR_INVALID_ARGUMENT
