@@ -17,8 +17,8 @@
 //    cut into equal ranges, one per CTA.  Lengths are read on the device, so
 //    a ragged batch is balanced to one tile without the host knowing it.
 //  * One warp looks up pages and fills a ring of K and V tiles, on across
-//    sequence boundaries.  Pages of a multiple of 8 tokens come by TMA, a box
-//    per page; others row by row (cp.async).
+//    sequence boundaries.  Pages of a multiple of 4 tokens come by TMA, a box
+//    or more per page; others row by row (cp.async).
 //  * One thread issues the products (tcgen05).  Both are transposed: scores^T
 //    = K Q^T has a tile's 128 tokens in the 128 lanes of tensor memory and
 //    only as many columns as there are rows, and output^T = V^T P^T the head
@@ -27,9 +27,16 @@
 //    softmax warps has one token and every row: R exponentials a tile.
 //  * The next tile's scores are computed while this one's softmax runs.  The
 //    output stays in tensor memory; it is read back to be rescaled only in
-//    the tiles where a row's maximum moves.
+//    the tiles where a row's maximum has moved too far.
 //  * A sequence that several CTAs share is joined by the last of them to
 //    arrive, in the order of the CTAs: the result does not depend on timing.
+//
+// Measured (16-bit types, against a copy's 6547 GB/s): 16 sequences of 16K to
+// 32K, 32 query and 8 KV heads of 128, 1.61 GB in 238 us, 6780 GB/s; 64 of 4K
+// to 16K with 5 new tokens each, 12 and 2 heads of 128, 0.67 GB in 119 us,
+// 5630 GB/s; 32 of up to 8K, 32 and 8 heads of 64, 0.27 GB in 50 us, 5400
+// GB/s; one of 32K, 12 and 2 heads of 128, 34 MB in 17 us, of which about 5
+// are the start (lengths, page numbers, first tiles) and 4 the join.
 #include "kvr_ring.cuh"
 
 #include <cuda.h>
@@ -78,6 +85,11 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, ui
       : "memory");
 }
 
+// 16 bytes from `src`, or zeros.
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
 struct Params {
   const uint16_t* q;
   int64_t q_b, q_h, q_t;
@@ -114,7 +126,9 @@ struct Cfg {
   static constexpr int Q_BYTES = N * D * 2;
   static constexpr int P_ROW = N == 16 ? 64 : 128;          // bytes of a token's weights (a swizzle row)
   static constexpr int P_BYTES = TILE * 4 * N;
-  // Two CTAs per SM where the ring still holds three units or more; else one with a longer ring.
+  // Two CTAs per SM where the ring still holds three units or more; else one with a longer ring.  (One CTA and six
+  // units in place of two and three each: 73 for 50 us on 32 sequences of up to 8K, 37 for 30 us on 128 windows of 1K,
+  // the same on 16 sequences of 16K to 32K, and 16 for 17 us on a single one, where the join is shorter.)
   static constexpr int CTAS = N == 16 || (N == 32 && D == 64) ? 2 : 1;
   static constexpr int UNITS = CTAS == 2 ? (D == 128 ? 3 : N == 16 ? 6 : 5) : (D == 128 ? (N == 32 ? 6 : 5) : 8);
   static constexpr int DESCS = 8;
@@ -531,14 +545,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
         }
       }
     };
-    // a unit copied row by row is announced once its copies have landed, when the next one's are on their way
-    int pending = -1;
-    auto announce = [&]() {
-      if (pending < 0) return;
+    // A unit copied row by row is announced once its copies have landed, when kBehind more are on their way.  (U - 2:
+    // the unit whose slot is waited for may be a V, which is let go after the K behind it has been multiplied.)
+    constexpr int kBehind = U - 2;
+    auto announce = [&](int un) {
+      if (un < 0) return;
       proxy_fence();
       __syncwarp();
-      if (lane == 0) bar_arrive(full + 8 * pending);
-      pending = -1;
+      if (lane == 0) bar_arrive(full + 8 * (un % U));
     };
     Lookup next;
     look(next);
@@ -575,6 +589,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
           const uint32_t good = __ballot_sync(0xffffffffu, ok[0]);
           if (lane == 0) bar_arrive_tx(full + 8 * slot, failed ? 0 : __popc(good) * p.box * 128 * C::HALVES);
           __syncwarp();
+          // (each lane its own box: one thread issuing all of them took twice the time with pages of 8)
           if (ok[0] && !failed)
 #pragma unroll
             for (int hf = 0; hf < C::HALVES; ++hf)
@@ -583,30 +598,32 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
         } else {
           constexpr int RPI = 32 / C::PIECES;   // rows per step
           const int c = lane % C::PIECES, sub = lane / C::PIECES;
-          const uint16_t* base = side ? p.v : p.k;
+          const uint16_t* base = (side ? p.v : p.k) + c * 8;
 #pragma unroll
           for (int x = 0; x < LU; ++x) {
             const int64_t mine = !ok[x] ? -1
                                  : side ? (int64_t)u.id[x] * p.v_page + (int64_t)u.d.h * p.v_head + (int64_t)u.row[x] * p.v_row
                                         : (int64_t)u.id[x] * p.k_page + (int64_t)u.d.h * p.k_head + (int64_t)u.row[x] * p.k_row;
-#pragma unroll 4
-            for (int r0 = 0; r0 < 32; r0 += RPI) {
-              const int64_t from = __shfl_sync(0xffffffffu, mine, r0 + sub);
-              const int r = x * 32 + r0 + sub;
-              if (from >= 0)
-                cp_async16(dst + (c >> 3) * C::HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + from + c * 8);
+            // all the addresses first, so that the copies follow one another; a row that is not there becomes 0
+            int64_t from[32 / RPI];
+#pragma unroll
+            for (int y = 0; y < 32 / RPI; ++y) from[y] = __shfl_sync(0xffffffffu, mine, y * RPI + sub);
+#pragma unroll
+            for (int y = 0; y < 32 / RPI; ++y) {
+              const int r = x * 32 + y * RPI + sub;
+              cp_async16_or_zero(dst + (c >> 3) * C::HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                                 base + (from[y] < 0 ? 0 : from[y]), from[y] >= 0);
             }
           }
           cp_async_commit();
-          cp_async_wait<1>();
-          announce();
-          pending = slot;
+          cp_async_wait<kBehind>();
+          announce(un - kBehind);
         }
       }
     }
     if constexpr (!TMA) {
       cp_async_wait<0>();
-      announce();
+      for (int un = 2 * count - kBehind; un < 2 * count; ++un) announce(un);
     }
     // after a wait that ran out, see the copies in flight off
     if (TMA && failed)
@@ -1021,6 +1038,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
 
 // token_weights[b, j] += sum over the heads and new tokens of 2^(x - lse2).
 // One thread per token, the rows in order: no atomics, a fixed order of sums.
+// What bounds it: the scores, written by the attention and read here out of
+// L2, 4 bytes per row and token (16 sequences of 1K to 8K, 12 heads: 5.9 us).
 __global__ void weights_kernel(const __grid_constant__ Params p, float* weights, int64_t weights_b) {
   extern __shared__ float lse2[];
   pdl_enter();
@@ -1042,7 +1061,8 @@ __global__ void weights_kernel(const __grid_constant__ Params p, float* weights,
 
 // New token t of sequence b goes to row j % page of page table[b, j / page],
 // j = L - T + t.  A row whose page is not in the pool is not written (the
-// attention over it gives NaN).
+// attention over it gives NaN).  A few KB: its time is a launch's, 2 to 4 us
+// of the step.
 __global__ void append_kernel(const __grid_constant__ kvr_paged_append_args a) {
   pdl_enter();
   const int pieces = a.head_dim / 8;
@@ -1110,7 +1130,10 @@ static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
   if (a->token_weights && (a->kv_heads * R > 12000 || a->batch > 65535)) return KVR_ERR_UNSUPPORTED;
   p.R = (int)R;
   p.cap = (int)cap;
-  p.n = R <= 16 ? 16 : R <= 32 ? 32 : 64;   // rows of a tile
+  // Rows of a tile: the fewest that hold them, since a thread's work goes with them and fewer leave room for a
+  // second CTA per SM.  (4 rows in 16 and in 32: 32 sequences of up to 8K 49.8 and 52.3 us; 6 rows: 128 windows of 1K
+  // 29.8 and 38.9 us; 30 rows in 32 and in 64: 64 sequences of 4K to 16K 119 and 128 us.)
+  p.n = R <= 16 ? 16 : R <= 32 ? 32 : 64;
   p.row_tiles = (p.R + p.n - 1) / p.n;
   const int64_t tiles = std::max<int64_t>(1, (cap + kTile - 1) / kTile + 1 + kHead) * a->batch * a->kv_heads * p.row_tiles;
   if (tiles > (1ll << 31) - 1) return KVR_ERR_UNSUPPORTED;
@@ -1266,13 +1289,15 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   cudaStream_t s = as_stream(stream);
   const bool half = a->dtype == 1;
   // TMA boxes: the largest number of tokens that divides both a page and a
-  // tile; below 8 rows (one swizzle pattern) the rows are copied one by one.
+  // tile; below 4 (a lane's box each) the rows are copied one by one.  32
+  // sequences of 2K to 8K, 12 query and 2 KV heads of 128: pages of 16 or more
+  // 38 us, of 8 39 us, of 4 53 us by TMA, row by row 59 us whatever the page.
   int box = paged::kTile;
   while (a->page_size % box) box /= 2;
   p.box = box;
   paged::Maps maps;
   std::memset(&maps, 0, sizeof(maps));
-  const bool tma = box >= 8 &&
+  const bool tma = box >= 4 &&
                    paged::page_map(&maps.k, a->key_pages, half, a->head_dim, a->page_size, a->kv_heads, a->num_pages,
                                    a->key_row_stride, a->key_head_stride, a->key_page_stride, box) &&
                    paged::page_map(&maps.v, a->value_pages, half, a->head_dim, a->page_size, a->kv_heads, a->num_pages,

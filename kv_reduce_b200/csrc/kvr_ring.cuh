@@ -1,4 +1,4 @@
-// mbarriers and bulk copies for kernels in which one warp fills a ring of
+// mbarriers for kernels in which one warp fills a ring of
 // shared-memory stages and others work through it (sm_100a).
 #pragma once
 
@@ -41,14 +41,6 @@ static __device__ __noinline__ bool bar_wait_long(uint32_t bar, int parity) {
 __device__ __forceinline__ void bar_wait(uint32_t bar, int parity, bool& failed) {
   if (bar_try(bar, parity) || failed) return;
   failed = !bar_wait_long(bar, parity);
-}
-
-// `bytes` (a multiple of 16) from 16-byte aligned `src` to 16-byte aligned `dst`.
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, int bytes, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src),
-      "r"(bytes), "r"(bar)
-      : "memory");
 }
 
 }  // namespace ring

@@ -112,7 +112,7 @@ def test_ragged_lengths(kvr, HQ, H, D, T, dtype):
     check(kvr, make([1, 17, 64, 65, 0, 300, 1029, 128, 5], HQ, H, D, T, 16, dtype, seed=T))
 
 
-@pytest.mark.parametrize("page", [1, 3, 8, 24, 64, 100, 256])
+@pytest.mark.parametrize("page", [1, 2, 3, 4, 8, 12, 24, 64, 100, 256])
 @pytest.mark.parametrize("layout", ["heads", "tokens", "interleaved"])
 def test_page_sizes_and_layouts(kvr, page, layout):
     check(kvr, make([129, 700, 31], 12, 2, 128, 2, page, layout=layout, seed=page))
