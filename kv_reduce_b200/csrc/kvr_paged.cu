@@ -129,8 +129,8 @@ struct Cfg {
   // Two CTAs per SM where the ring still holds three units or more; else one with a longer ring.  (One CTA and six
   // units in place of two and three each: 73 for 50 us on 32 sequences of up to 8K, 37 for 30 us on 128 windows of 1K,
   // the same on 16 sequences of 16K to 32K, and 16 for 17 us on a single one, where the join is shorter.)
-  static constexpr int CTAS = N == 16 || (N == 32 && D == 64) ? 2 : 1;
-  static constexpr int UNITS = CTAS == 2 ? (D == 128 ? 3 : N == 16 ? 6 : 5) : (D == 128 ? (N == 32 ? 6 : 5) : 8);
+  static constexpr int CTAS = N == 16 || D == 64 ? 2 : 1;
+  static constexpr int UNITS = CTAS == 2 ? (D == 128 ? 3 : N == 16 ? 6 : 5) : N == 32 ? 6 : 5;
   static constexpr int DESCS = 8;
   static constexpr int OFF_Q = UNITS * UNIT;
   static constexpr int OFF_P = OFF_Q + Q_BYTES;
@@ -1037,26 +1037,37 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
 }
 
 // token_weights[b, j] += sum over the heads and new tokens of 2^(x - lse2).
-// One thread per token, the rows in order: no atomics, a fixed order of sums.
-// What bounds it: the scores, written by the attention and read here out of
-// L2, 4 bytes per row and token (16 sequences of 1K to 8K, 12 heads: 5.9 us).
-__global__ void weights_kernel(const __grid_constant__ Params p, float* weights, int64_t weights_b) {
-  extern __shared__ float lse2[];
+// A CTA takes 256 / W tokens, 256 / W threads every W-th row; their sums are
+// added in order: no atomics, a fixed order of sums.  What bounds it: round
+// trips where tokens are few (W = 8), else the scores, written by the
+// attention and read here out of L2, 4 bytes per row and token (W = 1).
+constexpr int kWeightThreads = 256;
+template <int W>
+__global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_constant__ Params p, float* weights,
+                                                                 int64_t weights_b) {
+  constexpr int TOKENS = kWeightThreads / W;
+  __shared__ float sums[W][TOKENS];
   pdl_enter();
-  const int b = blockIdx.y, rows = p.HKV * p.R;
-  const int len = length_of(p, b);
-  const int j = blockIdx.x * blockDim.x + threadIdx.x;
-  if ((int)(blockIdx.x * blockDim.x) >= len) return;
-  for (int r = threadIdx.x; r < rows; r += blockDim.x) lse2[r] = finite_or_zero(p.row_lse2[(int64_t)b * rows + r]);
-  __syncthreads();
-  if (j >= len) return;
+  const int b = blockIdx.y, rows = p.HKV * p.R, part = threadIdx.x / TOKENS, at = threadIdx.x % TOKENS;
+  const int len = length_of(p, b), j0 = blockIdx.x * TOKENS, j = j0 + at;
   const Span s = span_of(p, len);
-  if (j < s.lo && j >= p.sinks) return;
+  if (j0 >= len || (j0 + TOKENS <= s.lo && j0 >= p.sinks)) return;
+  const bool seen = j < len && (j >= s.lo || j < p.sinks);
   const float* src = p.scores + (int64_t)b * rows * p.score_stride + j;
+  const float* lse2 = p.row_lse2 + (int64_t)b * rows;
   float sum = 0.f;
+  if (seen) {
 #pragma unroll 4
-  for (int r = 0; r < rows; ++r) sum += fast_exp2(src[(int64_t)r * p.score_stride] - lse2[r]);
-  weights[(int64_t)b * weights_b + j] += sum;
+    for (int r = part; r < rows; r += W) sum += fast_exp2(src[(int64_t)r * p.score_stride] - finite_or_zero(lse2[r]));
+  }
+  if constexpr (W > 1) {
+    sums[part][at] = sum;
+    __syncthreads();
+    if (part > 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) sum += sums[w][at];
+  }
+  if (seen) weights[(int64_t)b * weights_b + j] += sum;
 }
 
 // New token t of sequence b goes to row j % page of page table[b, j / page],
@@ -1126,19 +1137,29 @@ static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
   // 2^30 keeps token positions and the rows' products inside 32 bits
   if (cap > (1 << 30) || R > (1 << 20) || (int64_t)a->batch * a->kv_heads * R > (1ll << 31) - 1)
     return KVR_ERR_UNSUPPORTED;
-  // weights_kernel: 48 KB of row statistics, the batch along the grid's y
-  if (a->token_weights && (a->kv_heads * R > 12000 || a->batch > 65535)) return KVR_ERR_UNSUPPORTED;
+  // weights_kernel: the batch along the grid's y
+  if (a->token_weights && a->batch > 65535) return KVR_ERR_UNSUPPORTED;
   p.R = (int)R;
   p.cap = (int)cap;
   // Rows of a tile: the fewest that hold them, since a thread's work goes with them and fewer leave room for a
   // second CTA per SM.  (4 rows in 16 and in 32: 32 sequences of up to 8K 49.8 and 52.3 us; 6 rows: 128 windows of 1K
   // 29.8 and 38.9 us; 30 rows in 32 and in 64: 64 sequences of 4K to 16K 119 and 128 us.)
-  p.n = R <= 16 ? 16 : R <= 32 ? 32 : 64;
+  p.n = R <= 16 ? 16 : R <= 32 || a->head_dim == 64 ? 32 : 64;
+  // (head dimension 64: 32 rows with two CTAs per SM in place of 64 with one take 26 for 33 us on 16 sequences of 4K
+  // with 56 rows, 185 for 227 us on 64 of 16K.)
+  // With little work several tiles of 16 rows beat one: K and V come from L2 again, but more CTAs share the softmax,
+  // and the joins, which take longer than the tiles.  (64 rows of one sequence of 16K: 20.6 us in 16, 26.4 in 32, 45.0
+  // in 64; 30 rows, 16 of 4K, 7 tiles per CTA: 25.7 in 16 and 27.7 in 32; 16 of 16K, 27 per CTA: 89 and 62;
+  // 128 rows, 4 of 16K, 14 per CTA: 38.6 in 16 and 51.0 in 64; 64 rows, 16 of 16K, 27 per CTA: 74.5 and 66.4.)
+  const int64_t sees = a->window > 0 ? std::min<int64_t>(cap, (int64_t)a->window + a->new_tokens + a->sinks) : cap;
+  if ((sees + kTile - 1) / kTile * a->batch * a->kv_heads * ((R + 15) / 16) <=
+      (p.n == 64 ? 14 : 8) * 2 * (int64_t)num_sms_of(a->num_sms))
+    p.n = 16;
   p.row_tiles = (p.R + p.n - 1) / p.n;
   const int64_t tiles = std::max<int64_t>(1, (cap + kTile - 1) / kTile + 1 + kHead) * a->batch * a->kv_heads * p.row_tiles;
   if (tiles > (1ll << 31) - 1) return KVR_ERR_UNSUPPORTED;
   // one or two CTAs per SM (Cfg::CTAS); a join takes kGroup^2 parts and some
-  const int per_sm = p.n == 16 || (p.n == 32 && a->head_dim == 64) ? 2 : 1;
+  const int per_sm = p.n == 16 || a->head_dim == 64 ? 2 : 1;
   p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, std::min(per_sm * num_sms_of(a->num_sms), kGroup * 20)));
   p.score_stride = std::max<int64_t>(128, (cap + 127) / 128 * 128);
   const size_t rows = (size_t)p.n * 3 * p.ctas;
@@ -1214,8 +1235,9 @@ static int launch(const Params& p, const Maps& maps, cudaStream_t s) {
 template <bool HALF, int D, bool TMA>
 static int launch_n(int n, const Params& p, const Maps& maps, cudaStream_t s) {
   if (n == 16) return launch<HALF, D, 16, TMA>(p, maps, s);
-  if (n == 32) return launch<HALF, D, 32, TMA>(p, maps, s);
-  return launch<HALF, D, 64, TMA>(p, maps, s);
+  if constexpr (D == 128)
+    if (n == 64) return launch<HALF, D, 64, TMA>(p, maps, s);
+  return launch<HALF, D, 32, TMA>(p, maps, s);
 }
 template <bool HALF, int D>
 static int launch_tma(bool tma, int n, const Params& p, const Maps& maps, cudaStream_t s) {
@@ -1307,10 +1329,17 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   else
     st = half ? paged::launch_tma<true, 128>(tma, pl.n, p, maps, s) : paged::launch_tma<false, 128>(tma, pl.n, p, maps, s);
   if (st != KVR_OK || !a->token_weights || pl.cap == 0) return st;
-  const int rows = p.HKV * p.R;
-  const dim3 grid((pl.cap + 255) / 256, p.B);
-  cudaError_t e = pdl_launch(paged::weights_kernel, grid, dim3(256), rows * sizeof(float), s, 1, p, a->token_weights,
-                             a->weights_b_stride);
+  // Few CTAs: the rows split over eight warps (their share of a step with one sequence of 4K and 64 rows: 6 us, with
+  // one thread for all rows 12; with 256 rows 11 and 32).  More CTAs than the GPU holds at a time only cost: 16 sequences
+  // of 1K to 8K with 12 rows, 25 us a step for 23.
+  const int wide = (pl.cap + paged::kWeightThreads - 1) / paged::kWeightThreads;
+  cudaError_t e;
+  if ((int64_t)wide * p.B < 2 * paged::num_sms_of(a->num_sms))
+    e = pdl_launch(paged::weights_kernel<8>, dim3((pl.cap + 31) / 32, p.B), dim3(paged::kWeightThreads), 0, s, 1, p,
+                   a->token_weights, a->weights_b_stride);
+  else
+    e = pdl_launch(paged::weights_kernel<1>, dim3(wide, p.B), dim3(paged::kWeightThreads), 0, s, 1, p, a->token_weights,
+                   a->weights_b_stride);
   if (e != cudaSuccess) { set_last_cuda_error(e); return KVR_ERR_CUDA; }
   return KVR_OK;
 }

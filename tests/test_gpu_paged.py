@@ -127,6 +127,17 @@ def test_window_and_sinks(kvr, window, sinks, T):
     check(kvr, make(lengths, 8, 2, 64, T, 24, "fp16", seed=window + T), window, sinks)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,HQ,H", [(1, 18, 1), (5, 12, 2), (4, 16, 2), (9, 16, 2), (33, 8, 1)])
+def test_wide_tables_and_batches(kvr, T, HQ, H, D):
+    """Enough room for tiles of more than 16 rows: by the table's width (few
+    tokens in use), and by the batch."""
+    check(kvr, make([3, 40, 333, 0, 129], HQ, H, D, T, 16, seed=T, max_pages=4000))
+    check(kvr, make([3, 40, 333], HQ, H, D, T, 12, "fp16", seed=T, max_pages=8000), 40000, 3)
+    lengths = [(i * 37) % 300 for i in range(1200 // H)]
+    check(kvr, make(lengths, HQ, H, D, T, 16, seed=T + 1), 130, 5)
+
+
 @pytest.mark.parametrize("T,HQ,H", [(8, 6, 1), (9, 16, 2), (11, 6, 1), (16, 8, 1), (33, 8, 1), (3, 64, 1)])
 def test_many_rows(kvr, T, HQ, H):
     """48 to 264 query rows per KV head: every row-tile count; queries before
