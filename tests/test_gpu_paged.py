@@ -138,6 +138,14 @@ def test_wide_tables_and_batches(kvr, T, HQ, H, D):
     check(kvr, make(lengths, HQ, H, D, T, 16, seed=T + 1), 130, 5)
 
 
+@pytest.mark.parametrize("page", [1, 2, 3, 10])
+@pytest.mark.parametrize("T,HQ,H,D", [(5, 12, 2, 128), (9, 8, 1, 128), (33, 8, 1, 128), (9, 8, 1, 64)])
+def test_small_pages_in_wide_tables(kvr, T, HQ, H, D, page):
+    """Rows copied one by one into rings of every length."""
+    check(kvr, make([3, 1040, 333, 0, 129], HQ, H, D, T, page, seed=T + page, max_pages=60000 // page))
+    check(kvr, make([2000, 40], HQ, H, D, T, page, seed=page, max_pages=150000 // page), 70000, 3)
+
+
 @pytest.mark.parametrize("T,HQ,H", [(8, 6, 1), (9, 16, 2), (11, 6, 1), (16, 8, 1), (33, 8, 1), (3, 64, 1)])
 def test_many_rows(kvr, T, HQ, H):
     """48 to 264 query rows per KV head: every row-tile count; queries before
