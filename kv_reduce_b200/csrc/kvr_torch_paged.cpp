@@ -7,11 +7,14 @@
 //   kvr::verify_draft     accepted drafted tokens and the next one
 //
 // Checks raise ValueError before anything is allocated or launched.  Outputs
-// come from the caching allocator.  The join's scratch is cached per
-// (device, stream): launches on one stream follow each other, and a completed
-// launch leaves the counters at zero.  Inside a CUDA graph capture a call
-// takes its scratch from the graph's own memory (a memset node zeroes the
-// counters on each replay), so a graph never depends on a cached buffer.
+// come from the caching allocator.  Scratch is cached per (operator, device,
+// stream), and a call holds it until its last launch is in the stream: the
+// operators run without Python's lock, and a sampled verification is two
+// launches with its counters non-zero between them, so another thread's call
+// must not come in between.  Launches on one stream follow each other, and a
+// completed call leaves the counters at zero.  Inside a CUDA graph capture a
+// call takes its scratch from the graph's own memory (a memset node zeroes
+// the counters on each replay), so a graph never depends on a cached buffer.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -24,6 +27,7 @@
 #include <map>
 #include <mutex>
 #include <string>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -55,32 +59,64 @@ bool rows16(const at::Tensor& t) {
 // elements are contiguous and rows start on 16 bytes; others are copied.
 at::Tensor rows(const at::Tensor& t) { return rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
+enum class Op { attention, verify };
 struct Scratch {
+  std::mutex mu;   // held from taking the buffers to the call's last launch
   at::Tensor workspace, counters;
 };
-std::mutex g_mu;
-std::map<std::pair<int, uintptr_t>, Scratch> g_scratch;
+std::mutex g_mu;   // the map and the list below
+std::map<std::tuple<Op, int, uintptr_t>, Scratch> g_scratch;
 // Buffers outgrown by a later call; launches in flight may still hold them,
 // and the growth is geometric, so they are kept.
 std::vector<at::Tensor> g_outgrown;
 
-Scratch scratch_for(const at::Device& dev, cudaStream_t stream, int64_t bytes, int64_t counters) {
-  const auto u8 = at::TensorOptions().dtype(at::kByte).device(dev);
-  const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-    return {at::empty({std::max<int64_t>(bytes, 16)}, u8), at::zeros({std::max<int64_t>(counters, 1)}, i32)};
-  std::lock_guard<std::mutex> lock(g_mu);
-  Scratch& s = g_scratch[{dev.index(), reinterpret_cast<uintptr_t>(stream)}];
-  if (!s.workspace.defined() || s.workspace.numel() < bytes) {
-    if (s.workspace.defined()) g_outgrown.push_back(s.workspace);
-    s.workspace = at::empty({std::max<int64_t>(2 * bytes, 1 << 20)}, u8);
+// A call's scratch, for as long as this object lives.
+class Lease {
+ public:
+  at::Tensor workspace, counters;
+
+  Lease(Op op, const at::Device& dev, cudaStream_t stream, int64_t bytes, int64_t n_counters) {
+    const auto u8 = at::TensorOptions().dtype(at::kByte).device(dev);
+    const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+      workspace = at::empty({std::max<int64_t>(bytes, 16)}, u8);
+      counters = at::zeros({std::max<int64_t>(n_counters, 1)}, i32);
+      return;
+    }
+    {
+      std::lock_guard<std::mutex> lock(g_mu);
+      cached_ = &g_scratch[{op, dev.index(), reinterpret_cast<uintptr_t>(stream)}];   // (nodes of a map stay put)
+    }
+    held_ = std::unique_lock<std::mutex>(cached_->mu);
+    if (!cached_->workspace.defined() || cached_->workspace.numel() < bytes) {
+      outgrow(cached_->workspace);
+      cached_->workspace = at::empty({std::max<int64_t>(2 * bytes, 1 << 20)}, u8);
+    }
+    if (!cached_->counters.defined() || cached_->counters.numel() < n_counters) {
+      outgrow(cached_->counters);
+      cached_->counters = at::zeros({std::max<int64_t>(2 * n_counters, 4096)}, i32);
+    }
+    workspace = cached_->workspace;
+    counters = cached_->counters;
   }
-  if (!s.counters.defined() || s.counters.numel() < counters) {
-    if (s.counters.defined()) g_outgrown.push_back(s.counters);
-    s.counters = at::zeros({std::max<int64_t>(2 * counters, 4096)}, i32);
+
+  // The status of the call's launches: after a failed one the counters may
+  // not be zero, so the next call gets others.
+  int launched(int st) {
+    if (st != KVR_OK && cached_) outgrow(cached_->counters);
+    return st;
   }
-  return s;
-}
+
+ private:
+  static void outgrow(at::Tensor& t) {
+    if (!t.defined()) return;
+    std::lock_guard<std::mutex> lock(g_mu);
+    g_outgrown.push_back(std::move(t));
+    t = at::Tensor();
+  }
+  Scratch* cached_ = nullptr;
+  std::unique_lock<std::mutex> held_;
+};
 
 bool is_half_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
 
@@ -192,7 +228,7 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& query, cons
     size_t ws = 0, counters = 0, scores = 0;
     raise_status("kvr_paged_attention_plan", kvr_paged_attention_plan(&a, &ws, &counters, &scores));
     cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
-    const Scratch s = scratch_for(dev, stream, (int64_t)ws, (int64_t)counters);
+    Lease s(Op::attention, dev, stream, (int64_t)ws, (int64_t)counters);
     a.workspace = s.workspace.data_ptr();
     a.workspace_bytes = (size_t)s.workspace.numel();
     a.counters = s.counters.data_ptr<int>();
@@ -202,7 +238,7 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& query, cons
       a.scores = x.data_ptr();
       a.scores_bytes = scores;
     }
-    raise_status("kvr_paged_attention", kvr_paged_attention(&a, stream));
+    raise_status("kvr_paged_attention", s.launched(kvr_paged_attention(&a, stream)));
   }
   if (!with_lse) lse = at::empty({0}, f32);
   return {out, lse};
@@ -324,10 +360,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_draft(const at::Tensor& ta
   size_t zeroed = 0, ws = 0;
   raise_status("kvr_verify_plan", kvr_verify_plan(&a, &zeroed, &ws));
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
-  const Scratch s = scratch_for(dev, stream, (int64_t)ws, (int64_t)(zeroed + 3) / 4);
+  Lease s(Op::verify, dev, stream, (int64_t)ws, (int64_t)(zeroed + 3) / 4);
   a.zeroed = s.counters.data_ptr(), a.zeroed_bytes = (size_t)s.counters.numel() * 4;
   a.workspace = s.workspace.data_ptr(), a.workspace_bytes = (size_t)s.workspace.numel();
-  raise_status("kvr_verify", kvr_verify(&a, stream));
+  raise_status("kvr_verify", s.launched(kvr_verify(&a, stream)));
   return {out, accepted, prob};
 }
 
