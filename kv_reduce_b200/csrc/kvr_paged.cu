@@ -152,6 +152,19 @@ struct Cfg {
 // The reference of a row that no token has been seen by: far below any score.
 constexpr float kUnseen = -1e30f;
 
+// The weights' range in the second product.  A reference is a maximum so far,
+// less kBelow, and moves when an exponent passes kBelow + 8; the weights' rest
+// is multiplied by kRest and has accumulators of its own.  bf16 has fp32's
+// range and needs neither.  fp16 ends at 2^-24 (2^-25 rounds to 0): a token 17
+// below the largest score, natural log, had no weight left, and a long cache
+// has many of those.  With both, weights stay below 2^15, the largest is 2^7 or
+// more, and hi + rest is off by 2^-36 at most: 2^-43 of the largest weight a
+// token.
+template <bool HALF>
+constexpr float kBelow = HALF ? 7.f : 0.f;
+template <bool HALF>
+constexpr float kRest = HALF ? 2048.f : 1.f;
+
 struct Desc {
   int first, last, full, token0;   // full: every row sees every token
   int b, h, rt, len;
@@ -721,8 +734,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       };
       // ---- exponents against the rows' references, each a maximum so far.
       // Any reference does while 2^(score - reference) stays in range: it
-      // moves, and the output is rescaled, only when an exponent passes 8 or a
-      // row is seen for the first time (kUnseen makes its exponents huge).
+      // moves, and the output is rescaled, only when an exponent passes
+      // kBelow + 8 or a row is seen for the first time (kUnseen makes its
+      // exponents huge).
       auto exponents = [&]() {
         float hot = -INFINITY;
 #pragma unroll
@@ -731,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
           x[r] = __fmaf_rn(x[r], factor, -mu_s[r]);
           if (r < n_rows) hot = fmaxf(hot, x[r]);
         }
-        return hot > 8.f;
+        return hot > kBelow<HALF> + 8.f;
       };
       load_scores();
       if (p.scores != nullptr) {
@@ -758,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
           const float before = mu_s[tid];
           float mn = before;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) mn = fmaxf(mn, smax[w * N + tid]);
+          for (int w = 0; w < kWarps; ++w) mn = fmaxf(mn, smax[w * N + tid] - kBelow<HALF>);
           mu_s[tid] = mn;
           alpha_s[tid] = fast_exp2(before - mn);
         }
@@ -788,8 +802,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       __syncwarp();
       if (lane == 0) bar_arrive(s_empty + 8 * (i & 1));
       // ---- P.  The tensor cores take it in the pages' type: as the rounded
-      // value and the rounded rest, side by side, so that the output's own
-      // rounding stays the largest error (one rounded value alone doubles it).
+      // value and the rounded rest (times kRest), side by side, so that the
+      // output's own rounding stays the largest error (one rounded value alone
+      // doubles it).
 #pragma unroll
       for (int r0 = 0; r0 < N; r0 += 8) {
         if (r0 >= n_rows) break;
@@ -801,7 +816,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
           l[r] += p0;
           l[r + 1] += p1;
           hi[y] = pack2<HALF>(p0, p1);
-          rest[y] = pack2<HALF>(p0 - to_float<HALF>((uint16_t)hi[y]), p1 - to_float<HALF>((uint16_t)(hi[y] >> 16)));
+          rest[y] = pack2<HALF>((p0 - to_float<HALF>((uint16_t)hi[y])) * kRest<HALF>,
+                                (p1 - to_float<HALF>((uint16_t)(hi[y] >> 16))) * kRest<HALF>);
         }
         *reinterpret_cast<uint4*>(smem + C::OFF_P + C::p_at(tid, r0, 0)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         *reinterpret_cast<uint4*>(smem + C::OFF_P + C::p_at(tid, r0, 1)) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
@@ -853,7 +869,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
                 const int pos = pos_s[c + r];
                 if (!(y <= pos && (p.window == 0 || y > pos - p.window || y < p.sinks))) continue;
                 o[r] += v * (to_float<HALF>(*reinterpret_cast<const uint16_t*>(smem + C::OFF_P + C::p_at(tr, c + r, 0))) +
-                             to_float<HALF>(*reinterpret_cast<const uint16_t*>(smem + C::OFF_P + C::p_at(tr, c + r, 1))));
+                             to_float<HALF>(*reinterpret_cast<const uint16_t*>(smem + C::OFF_P + C::p_at(tr, c + r, 1))) *
+                                 (1.f / kRest<HALF>));
               }
             }
             tmem_store(tmem_o + my_lanes + c, o);
@@ -917,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               if (c + r >= n_rows) break;
-              const float x = o[r] + rest[r];
+              const float x = o[r] + rest[r] * (1.f / kRest<HALF>);
               if (whole) p.out[(int64_t)row_s[c + r] * D + d] = (uint16_t)pack2<HALF>(x * alpha_s[c + r], 0.f);
               else part[r * D] = x;
             }
