@@ -409,7 +409,9 @@ int kvr_exchange_free(void* ptr);
  * kvr_paged_append: the T = new_tokens newest tokens of every sequence,
  * positions lengths[b]-T .. lengths[b]-1 (lengths already count them), from
  * key/value [B, HKV, T, D] (strides in elements, multiples of 8).  Positions
- * below 0 and rows whose page number is not in [0, num_pages) are skipped. */
+ * below 0 and rows whose page number is not in [0, num_pages) are skipped.
+ * new_counts [B] or NULL: sequences with fewer new tokens than T; only their
+ * last new_counts[b] of the T rows are written.                             */
 typedef struct {
   const void* key; int64_t key_b_stride, key_h_stride, key_t_stride;
   const void* value; int64_t value_b_stride, value_h_stride, value_t_stride;
@@ -418,6 +420,7 @@ typedef struct {
   const int* block_table; int64_t table_stride; int table_width; int num_pages;
   const int* lengths;
   int batch, kv_heads, head_dim, new_tokens, page_size;
+  const int* new_counts;
 } kvr_paged_append_args;
 int kvr_paged_append(const kvr_paged_append_args* a, kvr_stream_t stream);
 
@@ -427,6 +430,9 @@ int kvr_paged_append(const kvr_paged_append_args* a, kvr_stream_t stream);
  * only those with j > i-window or j < sinks.  A query that sees nothing
  * gives zeros (lse -inf).  A sequence longer than its table row, or with a
  * page number outside the pool among the tokens it sees, gives NaN.
+ * new_counts [B] or NULL: sequences with fewer new tokens than T; the queries
+ * before their last new_counts[b] are padding: whatever they hold, they give
+ * zeros (lse -inf) and add no weight.
  *   query [B, HQ, T, D] (strides in elements, multiples of 8), out
  *   [B, HQ, T, D] contiguous in the query's type, lse [B, HQ, T] natural
  *   log or NULL.
@@ -453,6 +459,7 @@ typedef struct {
   void* workspace; size_t workspace_bytes;
   int* counters;
   void* scores; size_t scores_bytes;
+  const int* new_counts;
 } kvr_paged_attention_args;
 int kvr_paged_attention_plan(const kvr_paged_attention_args* a, size_t* workspace_bytes,
                              size_t* counter_count, size_t* scores_bytes);

@@ -186,6 +186,7 @@ class PagedAppendArgs(Structure):
         ("block_table", c_void_p), ("table_stride", c_int64), ("table_width", c_int), ("num_pages", c_int),
         ("lengths", c_void_p),
         ("batch", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("new_tokens", c_int), ("page_size", c_int),
+        ("new_counts", c_void_p),
     ]
 
 
@@ -202,7 +203,7 @@ class PagedAttentionArgs(Structure):
         ("batch", c_int), ("q_heads", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("new_tokens", c_int),
         ("page_size", c_int), ("window", c_int), ("sinks", c_int), ("scale", ctypes.c_float), ("num_sms", c_int),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("counters", c_void_p),
-        ("scores", c_void_p), ("scores_bytes", c_size_t),
+        ("scores", c_void_p), ("scores_bytes", c_size_t), ("new_counts", c_void_p),
     ]
 
 

@@ -102,10 +102,11 @@ struct Params {
   int num_pages, page, page_shift;
   uint32_t page_magic;   // j / page = j * page_magic >> page_shift for j < 2^30
   const int* lengths;
+  const int* counts;   // [B] or null: how many of the T new tokens a sequence has, the last ones
   uint16_t* out;
   float* lse;       // [B, HQ, T] or null
   float* scores;    // [B, HKV, R, score_stride] or null: x_ij for the weights kernel
-  float* row_lse2;  // [B, HKV, R], with scores
+  float* row_lse2;  // [B, HKV, R], with scores; inf for a row that is no token's
   int64_t score_stride;
   int B, HQ, HKV, T, G, R, row_tiles, window, sinks, cap;
   float scale2;     // scale * log2(e)
@@ -681,7 +682,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
         if (tid < N) {
           const int R = min(rt * N + tid, p.R - 1), t = R / p.G;
           mu_s[tid] = kUnseen;
-          pos_s[tid] = len - p.T + t;
+          // a row that pads a sequence of fewer new tokens stands nowhere: tiles that every row sees are computed
+          // for it too, and what it has in the end is not written
+          pos_s[tid] = p.counts == nullptr || t >= p.T - p.counts[ds.b] ? len - p.T + t : -1;
           row_s[tid] = (ds.b * p.HQ + ds.h * p.G + R - t * p.G) * p.T + t;
         }
         if (tid == 0) *s_add = 0;
@@ -909,10 +912,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
         if (tid < n_rows) {   // thread = row
           const float sum = ssum[tid] + ssum[N + tid] + ssum[2 * N + tid] + ssum[3 * N + tid];
           if (whole) {
-            alpha_s[tid] = sum == 0.f ? 0.f : 1.f / sum;
-            const float lse2 = sum == 0.f ? -INFINITY : mu_s[tid] + log2f(sum);
+            const bool none = sum == 0.f || pos_s[tid] < 0;
+            alpha_s[tid] = none ? 0.f : 1.f / sum;
+            const float lse2 = none ? -INFINITY : mu_s[tid] + log2f(sum);
             if (p.lse) p.lse[row_s[tid]] = lse2 * 0.6931471805599453f;
-            if (p.row_lse2) p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + tid] = lse2;
+            if (p.row_lse2)
+              p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + tid] = pos_s[tid] < 0 ? INFINITY : lse2;
           } else {
             *reinterpret_cast<float2*>(p.part_ml + (slot_o * ROWS + tid) * 2) = make_float2(mu_s[tid], sum);
           }
@@ -935,7 +940,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
             for (int r = 0; r < 16; ++r) {
               if (c + r >= n_rows) break;
               const float x = o[r] + rest[r] * (1.f / kRest<HALF>);
-              if (whole) p.out[(int64_t)row_s[c + r] * D + d] = (uint16_t)pack2<HALF>(x * alpha_s[c + r], 0.f);
+              if (whole)
+                p.out[(int64_t)row_s[c + r] * D + d] =
+                    (uint16_t)pack2<HALF>(alpha_s[c + r] == 0.f ? 0.f : x * alpha_s[c + r], 0.f);
               else part[r * D] = x;
             }
           }
@@ -1006,14 +1013,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
                 if (col == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, sum);
                 continue;
               }
-              const float inv = sum == 0.f ? 0.f : 1.f / sum;
+              const bool none = sum == 0.f || pos_s[r] < 0;
+              if (none)
+#pragma unroll
+                for (int z = 0; z < 8; ++z) acc[z] = 0.f;
+              const float inv = none ? 0.f : 1.f / sum;
               *reinterpret_cast<uint4*>(p.out + (int64_t)row_s[r] * D + col) =
                   make_uint4(pack2<HALF>(acc[0] * inv, acc[1] * inv), pack2<HALF>(acc[2] * inv, acc[3] * inv),
                              pack2<HALF>(acc[4] * inv, acc[5] * inv), pack2<HALF>(acc[6] * inv, acc[7] * inv));
               if (col == 0) {
-                const float lse2 = sum == 0.f ? -INFINITY : mm + log2f(sum);
+                const float lse2 = none ? -INFINITY : mm + log2f(sum);
                 if (p.lse) p.lse[row_s[r]] = lse2 * 0.6931471805599453f;
-                if (p.row_lse2) p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + r] = lse2;
+                if (p.row_lse2)
+                  p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + r] = pos_s[r] < 0 ? INFINITY : lse2;
               }
             }
           };
@@ -1075,7 +1087,11 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_co
   float sum = 0.f;
   if (seen) {
 #pragma unroll 4
-    for (int r = part; r < rows; r += W) sum += fast_exp2(src[(int64_t)r * p.score_stride] - finite_or_zero(lse2[r]));
+    for (int r = part; r < rows; r += W) {
+      const float y = lse2[r];
+      const float w = fast_exp2(src[(int64_t)r * p.score_stride] - finite_or_zero(y));
+      sum += y == INFINITY ? 0.f : w;   // (the scores of a row that is no token's may be anything)
+    }
   }
   if constexpr (W > 1) {
     sums[part][at] = sum;
@@ -1088,7 +1104,7 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_co
 }
 
 // New token t of sequence b goes to row j % page of page table[b, j / page],
-// j = L - T + t.  A row whose page is not in the pool is not written (the
+// j = L - T + t; with counts, only the last of the T.  A row whose page is not in the pool is not written (the
 // attention over it gives NaN).  A few KB: its time is a launch's, 2 to 4 us
 // of the step.
 __global__ void append_kernel(const __grid_constant__ kvr_paged_append_args a) {
@@ -1103,6 +1119,7 @@ __global__ void append_kernel(const __grid_constant__ kvr_paged_append_args a) {
     const int h = (int)(y % a.kv_heads);
     y /= a.kv_heads;
     const int t = (int)(y % a.new_tokens), b = (int)(y / a.new_tokens);
+    if (a.new_counts && t < a.new_tokens - a.new_counts[b]) continue;
     const int64_t j = (int64_t)a.lengths[b] - a.new_tokens + t;
     if (j < 0 || j >= (int64_t)a.table_width * a.page_size) continue;
     const int pg = (int)(j / a.page_size), row = (int)(j - (int64_t)pg * a.page_size);
@@ -1312,6 +1329,7 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   p.page_shift = 30 + shift;
   p.page_magic = (uint32_t)(((1ull << p.page_shift) + a->page_size - 1) / a->page_size);
   p.lengths = a->lengths;
+  p.counts = a->new_counts;
   p.out = static_cast<uint16_t*>(a->out);
   p.lse = a->lse;
   p.row_lse2 = a->token_weights ? static_cast<float*>(a->scores) : nullptr;

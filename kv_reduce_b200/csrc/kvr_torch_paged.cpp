@@ -139,8 +139,16 @@ void check_pages(const at::Tensor& kp, const at::Tensor& vp, const at::Tensor& t
                     "lengths must be a contiguous int32 [batch] tensor.");
 }
 
+const int* counts_of(const std::optional<at::Tensor>& counts, const at::Tensor& lengths) {
+  if (!counts.has_value() || !counts->defined()) return nullptr;
+  TORCH_CHECK_VALUE(counts->device() == lengths.device() && counts->scalar_type() == at::kInt && counts->dim() == 1 &&
+                        counts->size(0) == lengths.size(0) && (counts->size(0) <= 1 || counts->stride(0) == 1),
+                    "new_counts must be a contiguous int32 [batch] tensor.");
+  return counts->data_ptr<int>();
+}
+
 void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tensor& kp, const at::Tensor& vp,
-                  const at::Tensor& table, const at::Tensor& lengths) {
+                  const at::Tensor& table, const at::Tensor& lengths, const std::optional<at::Tensor>& new_counts) {
   check_pages(kp, vp, table, lengths, key.device());
   TORCH_CHECK_VALUE(value.device() == key.device(), "All tensors must be on the same CUDA device.");
   TORCH_CHECK_VALUE(key.dim() == 4 && key.sizes() == value.sizes() && key.size(0) == lengths.size(0) &&
@@ -149,6 +157,7 @@ void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
   TORCH_CHECK_VALUE(key.scalar_type() == kp.scalar_type() && value.scalar_type() == kp.scalar_type(),
                     "key and value must have the pages' dtype.");
   TORCH_CHECK_VALUE(key.size(3) % 8 == 0, "head_dim must be a multiple of 8.");
+  const int* counts = counts_of(new_counts, lengths);
   c10::cuda::CUDAGuard guard(key.device());
   if (key.numel() == 0) return;
   const at::Tensor k = rows(key), v = rows(value);
@@ -169,13 +178,15 @@ void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
   a.lengths = lengths.data_ptr<int>();
   a.batch = (int)k.size(0), a.kv_heads = (int)k.size(1), a.new_tokens = (int)k.size(2), a.head_dim = (int)k.size(3);
   a.page_size = (int)kp.size(2);
+  a.new_counts = counts;
   raise_status("kvr_paged_append", kvr_paged_append(&a, c10::cuda::getCurrentCUDAStream().stream()));
 }
 
 std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& query, const at::Tensor& kp, const at::Tensor& vp,
                                                    const at::Tensor& table, const at::Tensor& lengths,
                                                    std::optional<double> scale, int64_t window, int64_t sinks,
-                                                   const std::optional<at::Tensor>& token_weights, bool with_lse) {
+                                                   const std::optional<at::Tensor>& token_weights, bool with_lse,
+                                                   const std::optional<at::Tensor>& new_counts) {
   const at::Device dev = query.device();
   check_pages(kp, vp, table, lengths, dev);
   TORCH_CHECK_VALUE(query.dim() == 4, "query must have shape [batch, query_heads, new_tokens, head_dim].");
@@ -188,6 +199,7 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& query, cons
   TORCH_CHECK_VALUE(window >= 0 && sinks >= 0 && window <= INT32_MAX / 2 && sinks <= INT32_MAX / 2,
                     "window and sinks must not be negative.");
   TORCH_CHECK_VALUE(table.size(1) * kp.size(2) <= (1 << 30), "block_table addresses more than 2^30 tokens.");
+  const int* counts = counts_of(new_counts, lengths);
   const bool weighted = token_weights.has_value() && token_weights->defined();
   if (weighted) {
     const at::Tensor& w = *token_weights;
@@ -224,6 +236,7 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& query, cons
     a.batch = (int)q.size(0), a.q_heads = (int)q.size(1), a.new_tokens = (int)q.size(2), a.head_dim = (int)q.size(3);
     a.kv_heads = (int)kp.size(1), a.page_size = (int)kp.size(2);
     a.window = (int)window, a.sinks = (int)sinks;
+    a.new_counts = counts;
     a.scale = scale.has_value() ? (float)*scale : (float)(1.0 / std::sqrt((double)q.size(3)));
     size_t ws = 0, counters = 0, scores = 0;
     raise_status("kvr_paged_attention_plan", kvr_paged_attention_plan(&a, &ws, &counters, &scores));
@@ -371,9 +384,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> verify_draft(const at::Tensor& ta
 
 TORCH_LIBRARY_FRAGMENT(kvr, m) {
   m.def("paged_append(Tensor key, Tensor value, Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor block_table, "
-        "Tensor lengths) -> ()");
+        "Tensor lengths, Tensor? new_counts=None) -> ()");
   m.def("paged_attention(Tensor query, Tensor key_pages, Tensor value_pages, Tensor block_table, Tensor lengths, "
-        "float? scale=None, int window=0, int sinks=0, Tensor(a!)? token_weights=None, bool return_lse=False) "
+        "float? scale=None, int window=0, int sinks=0, Tensor(a!)? token_weights=None, bool return_lse=False, "
+        "Tensor? new_counts=None) "
         "-> (Tensor, Tensor)");
   m.def("paged_evict(Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor block_table, Tensor lengths, "
         "Tensor token_weights, Tensor new_block_table, int keep, int recent, int first) -> (Tensor, Tensor, Tensor)");

@@ -21,9 +21,11 @@ CUDA graphs with the library kernels as opaque nodes.
         geom, key_scale_pairs=None) -> out
                               packed_review.py:23-31 + :78 on a streaming layer
     kvr::lse_merge(part_ml, part_o) -> out           (cross-GPU partial merge)
-    kvr::paged_append(key, value, key_pages, value_pages, block_table, lengths)
+    kvr::paged_append(key, value, key_pages, value_pages, block_table, lengths,
+        new_counts=None)
     kvr::paged_attention(query, key_pages, value_pages, block_table, lengths,
-        scale=None, window=0, sinks=0, token_weights=None, return_lse=False)
+        scale=None, window=0, sinks=0, token_weights=None, return_lse=False,
+        new_counts=None)
         -> (out, lse)
     kvr::paged_evict(key_pages, value_pages, block_table, lengths,
         token_weights, new_block_table, keep, recent, first)
@@ -75,13 +77,13 @@ def _(part_ml, part_o):
 
 
 @torch.library.register_fake("kvr::paged_append")
-def _(key, value, key_pages, value_pages, block_table, lengths):
+def _(key, value, key_pages, value_pages, block_table, lengths, new_counts=None):
     return None
 
 
 @torch.library.register_fake("kvr::paged_attention")
 def _(query, key_pages, value_pages, block_table, lengths, scale=None, window=0, sinks=0, token_weights=None,
-      return_lse=False):
+      return_lse=False, new_counts=None):
     lse = query.new_empty(query.shape[:3] if return_lse else (0,), dtype=torch.float32)
     return query.new_empty(query.shape), lse
 

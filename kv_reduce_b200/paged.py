@@ -38,14 +38,18 @@ def _bind_ops() -> None:
 
 
 def paged_append(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
-                 block_table: torch.Tensor, lengths: torch.Tensor) -> None:
+                 block_table: torch.Tensor, lengths: torch.Tensor, new_counts: Optional[torch.Tensor] = None) -> None:
     """Write the newest T tokens' key and value [batch, kv_heads, T, head_dim]
     into their pages, at positions ``lengths - T .. lengths - 1`` (the lengths
     already count them).  Positions below 0, and rows whose page number is not
-    in the pool, are skipped."""
+    in the pool, are skipped.
+
+    ``new_counts`` (int32 [batch]): sequences with fewer new tokens than T.
+    Theirs are the last ``new_counts[b]`` of the T; the rows before are padding
+    and are not written."""
     if _append_op is None:
         _bind_ops()
-    _append_op(key, value, key_pages, value_pages, block_table, lengths)
+    _append_op(key, value, key_pages, value_pages, block_table, lengths, new_counts)
 
 
 def paged_decode_attention(
@@ -60,6 +64,7 @@ def paged_decode_attention(
     sinks: int = 0,
     token_weights: Optional[torch.Tensor] = None,
     return_lse: bool = False,
+    new_counts: Optional[torch.Tensor] = None,
 ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Attention of the newest T tokens of every sequence over its pages.
 
@@ -72,6 +77,10 @@ def paged_decode_attention(
     ``token_weights`` (fp32 [batch, >= max_pages * page_size]): the weight
     that each cached token got, summed over heads and queries, is added to it.
 
+    ``new_counts`` (int32 [batch]): sequences with fewer new tokens than T.
+    Their queries are the last ``new_counts[b]`` of the T; those before are
+    padding, see nothing and add no weight.
+
     Returns the output like ``query`` (contiguous), and with ``return_lse``
     the natural log of the softmax sums, fp32 [batch, query_heads, T].  A
     query that sees no token gives zeros and -inf.  A sequence longer than
@@ -81,7 +90,7 @@ def paged_decode_attention(
     if _attention_op is None:
         _bind_ops()
     out, lse = _attention_op(query, key_pages, value_pages, block_table, lengths, scale, window, sinks, token_weights,
-                             return_lse)
+                             return_lse, new_counts)
     return (out, lse) if return_lse else out
 
 
@@ -152,6 +161,10 @@ class PagedKVCache:
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(self.batch)]
         self._lengths = [0] * self.batch
+        # what the last advance gave each sequence, whether that differed, and the counts that the device has
+        self._new, self._ragged = [0] * self.batch, False
+        self.new_counts = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
+        self._counts_of = list(self._new)
 
     # ------------------------------------------------------------- lengths
     def get_seq_length(self) -> int:
@@ -172,7 +185,9 @@ class PagedKVCache:
 
     def advance(self, tokens: Union[int, Sequence[int]]) -> None:
         """Lengthen the sequences (by one number, or one each) and give them
-        pages; the rows are written by ``append``."""
+        pages; the rows are written by ``append``.  Where the numbers differ,
+        ``append`` and ``attention`` take the largest as T and each sequence's
+        new tokens as the last of the T."""
         more = [int(tokens)] * self.batch if isinstance(tokens, int) else [int(t) for t in tokens]
         if len(more) != self.batch or min(more) < 0:
             raise ValueError(f"advance needs a number of tokens >= 0 for each of {self.batch} sequences.")
@@ -184,6 +199,7 @@ class PagedKVCache:
         for pages, n in zip(self._pages, need):
             pages.extend(self._free.pop() for _ in range(n))
         self._lengths = [n + m for n, m in zip(self._lengths, more)]
+        self._new, self._ragged = more, min(more) != max(more)
         self._upload(any(n > 0 for n in need))
 
     def crop(self, lengths: Union[int, Sequence[int]]) -> None:
@@ -200,19 +216,37 @@ class PagedKVCache:
             if self.token_weights is not None and t < self._lengths[b]:
                 for w in self.token_weights:
                     w[b, t:self._lengths[b]] = 0
+        self._new = [max(0, m - (n - t)) for m, n, t in zip(self._new, self._lengths, to)]
         self._lengths = to
         self._upload(freed)
 
     # ---------------------------------------------------------- operations
+    def _counts(self) -> torch.Tensor:
+        """``_new`` on the device."""
+        if self._counts_of != self._new:
+            self.new_counts.copy_(torch.tensor(self._new, dtype=torch.int32))
+            self._counts_of = list(self._new)
+        return self.new_counts
+
     def append(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
-        """Write the tokens that ``advance`` made room for."""
-        paged_append(key, value, self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths)
+        """Write the tokens that ``advance`` made room for: key and value
+        [batch, kv_heads, T, head_dim], T the most that a sequence was given,
+        each sequence's own the last of them."""
+        if key.shape[2] != max(self._new):
+            raise ValueError(f"append takes the {max(self._new)} tokens that advance made room for, not {key.shape[2]}.")
+        paged_append(key, value, self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths,
+                     self._counts() if min(self._new) != max(self._new) else None)
 
     def attention(self, layer: int, query: torch.Tensor, *, scale: Optional[float] = None, window: int = 0,
                   sinks: int = 0) -> torch.Tensor:
+        """Attention of the newest T tokens, query [batch, query_heads, T,
+        head_dim].  After an ``advance`` by different numbers the queries of a
+        sequence are its new tokens' only, the last of the T; the outputs
+        before them are zeros."""
         weights = None if self.token_weights is None else self.token_weights[layer]
         return paged_decode_attention(query, self.key_pages[layer], self.value_pages[layer], self.block_table,
-                                      self.lengths, scale=scale, window=window, sinks=sinks, token_weights=weights)
+                                      self.lengths, scale=scale, window=window, sinks=sinks, token_weights=weights,
+                                      new_counts=self._counts() if self._ragged else None)
 
     def evict(self, keep: int, *, recent: int = 0, first: int = 0) -> bool:
         """Bring every sequence down to ``keep`` tokens (see ``paged_evict``),
@@ -241,5 +275,6 @@ class PagedKVCache:
         for pages in self._pages:
             self._free.extend(reversed(pages))
         self._pages, self._lengths = fresh, left
+        self._new, self._ragged = [0] * self.batch, False
         self._upload(True)
         return True
