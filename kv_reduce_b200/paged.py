@@ -262,16 +262,20 @@ class PagedKVCache:
         need = [-(-n // self.page_size) for n in left]
         if sum(need) > len(self._free):
             raise ValueError("not enough free pages to evict into.")
-        fresh = [[self._free.pop() for _ in range(n)] for n in need]
+        # (the pages leave the free list, and the weights change, once every layer's call has been accepted)
+        spare = iter(self._free[:-sum(need) - 1:-1])
+        fresh = [[next(spare) for _ in range(n)] for n in need]
         width = -(-min(keep, self.max_pages * self.page_size) // self.page_size)
         rows = [p + [-1] * (width - len(p)) for p in fresh]
         new_table = torch.tensor(rows, dtype=torch.int32).to(self.device)
-        for layer, weights in enumerate(self.token_weights):
-            _, _, kept = paged_evict(self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths,
-                                     weights, new_table, keep=keep, recent=recent, first=first)
+        kept = [paged_evict(self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths, weights,
+                            new_table, keep=keep, recent=recent, first=first)[2]
+                for layer, weights in enumerate(self.token_weights)]
+        for weights, w in zip(self.token_weights, kept):
             n = min(keep, weights.shape[1])
             weights.zero_()
-            weights[:, :n].copy_(kept[:, :n])
+            weights[:, :n].copy_(w[:, :n])
+        del self._free[-sum(need):]
         for pages in self._pages:
             self._free.extend(reversed(pages))
         self._pages, self._lengths = fresh, left
