@@ -265,11 +265,13 @@ class PagedKVCache:
         # (the pages leave the free list, and the weights change, once every layer's call has been accepted)
         spare = iter(self._free[:-sum(need) - 1:-1])
         fresh = [[next(spare) for _ in range(n)] for n in need]
-        width = -(-min(keep, self.max_pages * self.page_size) // self.page_size)
+        width = -(-keep // self.page_size)
         rows = [p + [-1] * (width - len(p)) for p in fresh]
         new_table = torch.tensor(rows, dtype=torch.int32).to(self.device)
-        kept = [paged_evict(self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths, weights,
-                            new_table, keep=keep, recent=recent, first=first)[2]
+        # the columns in use: the operator's limit is on the table's width, and a pool may be far wider than a sequence
+        table = self.block_table[:, :max(len(p) for p in self._pages)]
+        kept = [paged_evict(self.key_pages[layer], self.value_pages[layer], table, self.lengths, weights, new_table,
+                            keep=keep, recent=recent, first=first)[2]
                 for layer, weights in enumerate(self.token_weights)]
         for weights, w in zip(self.token_weights, kept):
             n = min(keep, weights.shape[1])

@@ -52,3 +52,19 @@ def test_a_refusal_at_a_later_layer(monkeypatch):
     assert torch.equal(calls[0], c.block_table[:, :2]) and len(calls) == 3
     for i, w in enumerate(c.token_weights):
         assert (w[:, :8] == 3.0 + i).all() and (w[:, 8:] == 0).all()
+
+
+def test_eviction_looks_at_the_columns_in_use(monkeypatch):
+    """A pool of more tokens than the operator takes, with short sequences."""
+    c = paged.PagedKVCache(1, 2, 1, 8, num_pages=30000, page_size=16, device="cpu", track_weights=True)
+    c.advance([100, 70])
+    tables = []
+
+    def op(k, v, table, lengths, w, new_table, keep, recent, first):
+        tables.append(table.clone())
+        return torch.zeros(2, keep, dtype=torch.int32), lengths.clamp_max(keep), torch.zeros(2, keep)
+
+    monkeypatch.setattr(paged, "_evict_op", op)
+    want = c.block_table[:, :7].clone()
+    assert c.evict(40) and torch.equal(tables[0], want)
+    assert c.seq_lengths() == [40, 40] and c.free_pages() == 30000 - 6
