@@ -438,7 +438,9 @@ int kvr_paged_append(const kvr_paged_append_args* a, kvr_stream_t stream);
  *   log or NULL.
  *   token_weights [B, >= table_width*page_size] fp32 or NULL: the weight
  *   every cached token got, summed over heads and queries, is added to it
- *   (a second launch; needs `scores`).
+ *   (a second launch; needs `scores`.  Scores are held for a part of the
+ *   batch at a time, 2 GiB or one sequence's; a batch of more takes a pair
+ *   of launches per part).
  * Supported: D in {64, 128}, table_width*page_size <= 2^30.
  * kvr_paged_attention_plan gives the bytes of workspace, the ints of
  * counters (zero before the first launch, left zero by every completed one)

@@ -1153,8 +1153,18 @@ static int num_sms_of(int given) {
   return sms[dev & 63];
 }
 
+// Scores of the weights' launch are held for as many sequences at a time as
+// fit here (one at least): they take 4 bytes per row and token of the table's
+// width, and a pool's table may be far wider than its sequences (20 GB for 64
+// sequences of 32 heads and 5 new tokens in a table of 512K tokens).  A part
+// costs some 20 us: 64 sequences of 200 to 8000, 12 heads, 5 new tokens, a table
+// of 512K take 237 us at once with 8 GB, 300 with this, 600 with 512 MB, which
+// would also slow tables of 64K tokens (32 sequences of 2K to 16K, 32 heads: 329 for 418).
+constexpr size_t kScoreBytes = 2048ull << 20;
+
 struct Plan {
   int G, R, n, row_tiles, cap, ctas;
+  int part;   // sequences per launch (with token weights)
   int64_t score_stride;
   size_t part_o, part_ml, lse2, scores;
 };
@@ -1199,7 +1209,9 @@ static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
   const size_t rows = (size_t)p.n * 3 * p.ctas;
   p.part_o = rows * a->head_dim * sizeof(float);
   p.part_ml = rows * 2 * sizeof(float);
-  const size_t all_rows = (size_t)a->batch * a->kv_heads * p.R;
+  const size_t seq_rows = (size_t)a->kv_heads * p.R, seq_scores = seq_rows * p.score_stride * sizeof(float);
+  p.part = a->token_weights ? (int)std::min<size_t>(a->batch, std::max<size_t>(1, kScoreBytes / seq_scores)) : a->batch;
+  const size_t all_rows = p.part * seq_rows;
   p.lse2 = a->token_weights ? (all_rows * sizeof(float) + 255) / 256 * 256 : 0;
   p.scores = a->token_weights ? all_rows * p.score_stride * sizeof(float) : 0;
   *out = p;
@@ -1286,8 +1298,21 @@ using namespace kvr;
 extern "C" int kvr_paged_attention_plan(const kvr_paged_attention_args* a, size_t* workspace_bytes,
                                         size_t* counter_count, size_t* scores_bytes) {
   paged::Plan p;
-  const int st = paged::plan_of(a, &p);
+  int st = paged::plan_of(a, &p);
   if (st != KVR_OK) return st;
+  if (p.part < a->batch) {   // what a part or the last, smaller one needs
+    kvr_paged_attention_args part = *a;
+    paged::Plan last;
+    part.batch = a->batch % p.part ? a->batch % p.part : p.part;
+    st = paged::plan_of(&part, &last);
+    if (st != KVR_OK) return st;
+    part.batch = p.part;
+    st = paged::plan_of(&part, &p);
+    if (st != KVR_OK) return st;
+    p.part_o = std::max(p.part_o + p.part_ml, last.part_o + last.part_ml);
+    p.part_ml = 0;
+    p.ctas = std::max(p.ctas, last.ctas);
+  }
   if (workspace_bytes) *workspace_bytes = p.part_o + p.part_ml;
   if (counter_count) *counter_count = 2 * (size_t)p.ctas;
   if (scores_bytes) *scores_bytes = p.lse2 + p.scores;
@@ -1299,6 +1324,23 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   int st = paged::plan_of(a, &pl);
   if (st != KVR_OK) return st;
   if (a->batch == 0) return KVR_OK;
+  if (pl.part < a->batch && a->query && a->out && a->lengths && a->block_table) {
+    for (int b = 0; b < a->batch; b += pl.part) {
+      kvr_paged_attention_args part = *a;
+      const int64_t rows = (int64_t)b * a->q_heads * a->new_tokens;
+      part.batch = std::min(pl.part, a->batch - b);
+      part.query = static_cast<const uint16_t*>(a->query) + b * a->q_b_stride;
+      part.out = static_cast<uint16_t*>(a->out) + rows * a->head_dim;
+      part.lse = a->lse ? a->lse + rows : nullptr;
+      part.block_table = a->block_table + b * a->table_stride;
+      part.lengths = a->lengths + b;
+      part.new_counts = a->new_counts ? a->new_counts + b : nullptr;
+      part.token_weights = a->token_weights + b * a->weights_b_stride;
+      st = kvr_paged_attention(&part, stream);
+      if (st != KVR_OK) return st;
+    }
+    return KVR_OK;
+  }
   if (!a->query || !a->out || !a->lengths || (pl.cap > 0 && !a->block_table) ||
       (a->num_pages > 0 && (!a->key_pages || !a->value_pages)))
     return KVR_ERR_INVALID_ARGUMENT;

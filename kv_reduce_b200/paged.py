@@ -161,6 +161,7 @@ class PagedKVCache:
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(self.batch)]
         self._lengths = [0] * self.batch
+        self._width = 0      # pages of the longest sequence
         # what the last advance gave each sequence, whether that differed, and the counts that the device has
         self._new, self._ragged = [0] * self.batch, False
         self.new_counts = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
@@ -182,6 +183,7 @@ class PagedKVCache:
             rows = [p + [-1] * (self.max_pages - len(p)) for p in self._pages]
             self.block_table.copy_(torch.tensor(rows, dtype=torch.int32))
         self.lengths.copy_(torch.tensor(self._lengths, dtype=torch.int32))
+        self._width = max(len(p) for p in self._pages)
 
     def advance(self, tokens: Union[int, Sequence[int]]) -> None:
         """Lengthen the sequences (by one number, or one each) and give them
@@ -243,9 +245,15 @@ class PagedKVCache:
         head_dim].  After an ``advance`` by different numbers the queries of a
         sequence are its new tokens' only, the last of the T; the outputs
         before them are zeros."""
-        weights = None if self.token_weights is None else self.token_weights[layer]
-        return paged_decode_attention(query, self.key_pages[layer], self.value_pages[layer], self.block_table,
-                                      self.lengths, scale=scale, window=window, sinks=sinks, token_weights=weights,
+        weights, table = None, self.block_table
+        if self.token_weights is not None:
+            weights = self.token_weights[layer]
+            # the scores' memory goes by the table's width: the columns in use.  (A captured step keeps all of them:
+            # its sequences may be longer when it is replayed.)
+            if not (self.device.type == "cuda" and torch.cuda.is_current_stream_capturing()):
+                table = table[:, :self._width]
+        return paged_decode_attention(query, self.key_pages[layer], self.value_pages[layer], table, self.lengths,
+                                      scale=scale, window=window, sinks=sinks, token_weights=weights,
                                       new_counts=self._counts() if self._ragged else None)
 
     def evict(self, keep: int, *, recent: int = 0, first: int = 0) -> bool:
@@ -269,7 +277,7 @@ class PagedKVCache:
         rows = [p + [-1] * (width - len(p)) for p in fresh]
         new_table = torch.tensor(rows, dtype=torch.int32).to(self.device)
         # the columns in use: the operator's limit is on the table's width, and a pool may be far wider than a sequence
-        table = self.block_table[:, :max(len(p) for p in self._pages)]
+        table = self.block_table[:, :self._width]
         kept = [paged_evict(self.key_pages[layer], self.value_pages[layer], table, self.lengths, weights, new_table,
                             keep=keep, recent=recent, first=first)[2]
                 for layer, weights in enumerate(self.token_weights)]
