@@ -66,6 +66,7 @@ struct Params {
   // scratch
   float2* part;               // [B, K, 2, segments]: (max, sum) of the target's and the draft's segments
   float4* stats;              // [B, K]: the same of the rows, target then draft
+  int4* raced;                // [B, race_segments]: the segments' winners (Racer) where the race is over the target alone
 };
 
 __device__ __forceinline__ float zero_if_none(float m) { return m == -INFINITY ? 0.f : m; }
@@ -361,21 +362,45 @@ __device__ __forceinline__ void load_noise(const float* p, int e, int V, float (
   }
 }
 
-// weight / e over one block, in logarithms: x c - log2 e has the same order
-// and needs neither the row's maximum nor its sum.
+// The best entry so far of a race over the target alone.  Weight / e of two
+// entries compares as (x - y) c with log2 e_x - log2 e_y: the row's maximum and
+// sum, which nothing has computed for this row, are not needed.  Only the
+// difference is scaled: x c by itself overflows for small temperatures and for
+// masks of the type's lowest value, and loses the bits that decide between
+// equal logits.
+struct Racer {
+  float x = -INFINITY, l = 0.f;   // logit, log2 of its exponential number
+  int at = -1;
+  __device__ __forceinline__ void take(float f, float le, int i, float c) {   // in rising order of i
+    if ((f - x) * c > le - l) {   // (-inf, no weight, and NaN never are; anything else beats the initial -inf)
+      x = f;
+      l = le;
+      at = i;
+    }
+  }
+  __device__ __forceinline__ void merge(const Racer& o, float c) {   // the same winner whichever is merged into which
+    if (o.at < 0) return;
+    const float d = (o.x - x) * c, t = o.l - l;
+    if (at < 0 || d > t || (!(d < t) && o.at < at)) *this = o;
+  }
+};
+__device__ __forceinline__ Racer lanes_race(Racer r, float c) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    Racer other;
+    other.x = __shfl_xor_sync(~0u, r.x, o);
+    other.l = __shfl_xor_sync(~0u, r.l, o);
+    other.at = __shfl_xor_sync(~0u, r.at, o);
+    r.merge(other, c);
+  }
+  return r;
+}
 template <typename T>
-__device__ __forceinline__ void race_target(const uint4& w, const float (&e)[Vec<T>::N], float c, int at, float& top,
-                                            int& where) {
+__device__ __forceinline__ void race_target(const uint4& w, const float (&e)[Vec<T>::N], float c, int at, Racer& r) {
   float f[Vec<T>::N];
   Vec<T>::get(w, f);
 #pragma unroll
-  for (int j = 0; j < Vec<T>::N; ++j) {
-    const float key = f[j] * c - __log2f(e[j]);
-    if (key > top) {
-      top = key;
-      where = at + j;
-    }
-  }
+  for (int j = 0; j < Vec<T>::N; ++j) r.take(f[j], __log2f(e[j]), at + j, c);
 }
 
 constexpr int kRaceUnroll = 2;
@@ -392,8 +417,9 @@ __global__ void __launch_bounds__(kThreads, 8) race_kernel(const __grid_constant
   const bool residual = at < n_draft;
   const float* noise = p.noise + (int64_t)b * p.n_b;
   const Row<T> rt(static_cast<const T*>(p.target) + (int64_t)b * p.t_b + (int64_t)at * p.t_k);
-  float mt = 0.f, md = 0.f, it = 0.f, id = 0.f, top = -INFINITY;
+  float mt = 0.f, md = 0.f, it = 0.f, id = 0.f, top = 0.f;
   int where = -1;
+  Racer racer;
   if (residual) {
     const Row<T> rd(static_cast<const T*>(p.draft) + (int64_t)b * p.d_b + (int64_t)at * p.d_k);
     const float4 st = p.stats[b * p.K + at];
@@ -401,7 +427,6 @@ __global__ void __launch_bounds__(kThreads, 8) race_kernel(const __grid_constant
     md = zero_if_none(st.z);
     it = st.y > 0.f ? 1.f / st.y : 0.f;
     id = st.w > 0.f ? 1.f / st.w : 0.f;
-    top = 0.f;
 #pragma unroll kRaceUnroll
     for (int g = begin + lane; g < end; g += 32) {
       float f[N], d[N], e[N];
@@ -424,32 +449,48 @@ __global__ void __launch_bounds__(kThreads, 8) race_kernel(const __grid_constant
       float e[N];
       const uint4 w = rt.load(g, p.V);
       load_noise(noise, g * N, p.V, e);
-      race_target<T>(w, e, p.c, g * N, top, where);
+      race_target<T>(w, e, p.c, g * N, racer);
     }
   }
-  unsigned long long best = lanes_best(where < 0 ? 0ull : race_key(top, where));
+  unsigned long long best = 0;
+  if (residual) best = lanes_best(where < 0 ? 0ull : race_key(top, where));
+  else racer = lanes_race(racer, p.c);
   const int64_t ahead = token_ahead(p, b);
+  int4* raced = p.raced + (int64_t)b * p.race_segments;
   int last = 0;
   if (lane == 0) {
     if (best) atomicMax(p.best + b, best);
+    if (!residual)
+      raced[unit - b * p.race_segments] = make_int4(__float_as_int(racer.x), __float_as_int(racer.l), racer.at, 0);
     __threadfence();
     last = atomicAdd(p.done + b, 1) == p.race_segments - 1;
     if (last) __threadfence();
   }
   if (!__shfl_sync(~0u, last, 0)) return;
-  best = *reinterpret_cast<volatile unsigned long long*>(p.best + b);
-  if (best == 0 && residual) {   // p = q up to rounding leaves nothing to draw from: draw from p
-    top = -INFINITY;
-    where = -1;
-    for (int g = lane; g < blocks_of<T>(p.V); g += 32) {
-      float e[N];
-      const uint4 w = rt.load(g, p.V);
-      load_noise(noise, g * N, p.V, e);
-      race_target<T>(w, e, p.c, g * N, top, where);
+  int64_t token = -1;
+  if (residual) token = race_index(*reinterpret_cast<volatile unsigned long long*>(p.best + b));
+  if (token < 0) {
+    racer = Racer();
+    if (residual) {   // p = q up to rounding leaves nothing to draw from: draw from p
+      for (int g = lane; g < blocks_of<T>(p.V); g += 32) {
+        float e[N];
+        const uint4 w = rt.load(g, p.V);
+        load_noise(noise, g * N, p.V, e);
+        race_target<T>(w, e, p.c, g * N, racer);
+      }
+    } else {   // the segments' winners, in order
+      for (int i = lane; i < p.race_segments; i += 32) {
+        const int4 x = __ldcg(raced + i);
+        Racer other;
+        other.x = __int_as_float(x.x);
+        other.l = __int_as_float(x.y);
+        other.at = x.z;
+        racer.merge(other, p.c);
+      }
     }
-    best = lanes_best(where < 0 ? 0ull : race_key(top, where));
+    token = lanes_race(racer, p.c).at;
   }
-  write_out(p, b, n_draft, at, race_index(best), ahead, 1);
+  write_out(p, b, n_draft, at, token, ahead, 1);
 }
 
 // t = 0: x_k is accepted while it is the argmax of target_k (the lowest index
@@ -577,7 +618,9 @@ static int plan_of(const kvr_verify_args* a, Plan* out) {
   p.skip = rows * a->vocab * (a->dtype == 2 ? 4 : 2) > (32 << 20);
   const size_t B = a->batch, K1 = a->draft_tokens + 1;
   p.zeroed = B * K1 * 8 + B * K1 * 4 + 2 * B * 4;
-  p.scratch = greedy ? 0 : B * (K1 - 1) * (sizeof(float4) + 2 * (size_t)p.segments * sizeof(float2));
+  p.scratch = greedy ? 0
+                     : B * p.race_segments * sizeof(int4) +
+                           B * (K1 - 1) * (sizeof(float4) + 2 * (size_t)p.segments * sizeof(float2));
   *out = p;
   return KVR_OK;
 }
@@ -639,7 +682,8 @@ extern "C" int kvr_verify(const kvr_verify_args* a, kvr_stream_t stream) {
   p.arrived = reinterpret_cast<int*>(p.best + rows);
   p.done = p.arrived + rows;
   p.refused = p.done + p.B;
-  p.stats = static_cast<float4*>(a->workspace);
+  p.raced = static_cast<int4*>(a->workspace);
+  p.stats = reinterpret_cast<float4*>(p.raced + (greedy ? 0 : (size_t)p.B * p.race_segments));
   p.part = reinterpret_cast<float2*>(p.stats + (size_t)p.B * K);
   cudaStream_t s = as_stream(stream);
   const cudaError_t e = a->dtype == 0   ? verify::launch<__nv_bfloat16>(p, greedy, s)
