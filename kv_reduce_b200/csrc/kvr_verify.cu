@@ -435,7 +435,8 @@ __global__ void __launch_bounds__(kThreads, 8) race_kernel(const __grid_constant
       load_noise(noise, g * N, p.V, e);
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float x = fast_exp2((f[j] - mt) * p.c) * it - fast_exp2((d[j] - md) * p.c) * id;
+        // (each product rounded: contracted into one fused operation, equal p and q would leave a rounding error)
+        const float x = __fsub_rn(__fmul_rn(fast_exp2((f[j] - mt) * p.c), it), __fmul_rn(fast_exp2((d[j] - md) * p.c), id));
         const float score = __fdividef(x, e[j]);
         if (score > top) {
           top = score;

@@ -50,3 +50,18 @@ def test_small_temperatures(kvr, dtype, temp, V):  # noqa: F811
     best = t[:, 3] == t[:, 3].amax(-1, keepdim=True)
     if temp <= 1e-3:
         assert torch.equal(r.tokens[:, 3], torch.where(best, noise, math.inf).argmin(-1))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [100, 9001])
+def test_equal_models_leave_nothing_to_draw_from(kvr, dtype, V):  # noqa: F811
+    """Where p and q are equal their difference is 0, not a rounding error: a
+    refusal (u = 1, a token outside the vocabulary) draws from p."""
+    t, _, tokens, u, noise = make(60, 2, V, dtype, 0.8, seed=V)
+    tokens[::2, 0] = V
+    r = kvr.verify_draft_tokens(t, t[:, :2].contiguous(), tokens, torch.ones_like(u), noise, temperature=0.8)
+    assert (r.accepted == 0).all()
+    score = torch.softmax(t[:, 0].double() / 0.8, -1) / noise.double()
+    top = score.topk(2).values
+    sure = top[:, 1] < top[:, 0] * (1 - 2.0 ** -16)
+    assert sure.double().mean() > 0.9 and torch.equal(r.tokens[sure, 0], score.argmax(-1)[sure])
