@@ -476,7 +476,7 @@ int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream_t stream);
  * behind the last), new_lengths [B], new_weights [B, keep] (0 behind the
  * last), none of them in place.  Rows whose page number is not in the pool
  * are not copied.
- * table_width*page_size <= 320000; new_table_width*page_size must hold
+ * table_width*page_size <= 320000, keep <= 2^30; new_table_width*page_size must hold
  * min(keep, table_width*page_size) tokens (KVR_ERR_CAPACITY).              */
 typedef struct {
   void* key_pages; int64_t key_page_stride, key_head_stride, key_row_stride;

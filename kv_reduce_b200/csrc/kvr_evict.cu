@@ -333,7 +333,8 @@ extern "C" int kvr_paged_evict(const kvr_paged_evict_args* a, kvr_stream_t strea
     return KVR_ERR_INVALID_ARGUMENT;
   if (a->head_dim % 8) return KVR_ERR_UNSUPPORTED;
   const int64_t cap = (int64_t)a->table_width * a->page_size;
-  if (cap > 8ll * evict::kMaxSlice || a->batch > 65535) return KVR_ERR_UNSUPPORTED;
+  // (keep at most 2^30: slots and what a thread adds to them stay inside 32 bits)
+  if (cap > 8ll * evict::kMaxSlice || a->batch > 65535 || a->keep > (1 << 30)) return KVR_ERR_UNSUPPORTED;
   if ((int64_t)a->new_table_width * a->page_size < std::min<int64_t>(a->keep, cap)) return KVR_ERR_CAPACITY;
   if (a->batch == 0) return KVR_OK;
   if (!a->lengths || !a->kept || !a->new_lengths || !a->new_weights ||
