@@ -1379,7 +1379,8 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   p.score_stride = pl.score_stride;
   p.B = a->batch; p.HQ = a->q_heads; p.HKV = a->kv_heads; p.T = a->new_tokens;
   p.G = pl.G; p.R = pl.R; p.row_tiles = pl.row_tiles;
-  p.window = a->window; p.sinks = a->window > 0 ? a->sinks : 0; p.cap = pl.cap;
+  // (no more than what a table can hold, 2^30: the sums with positions stay inside 32 bits)
+  p.window = std::min(a->window, 1 << 30); p.sinks = a->window > 0 ? std::min(a->sinks, pl.cap) : 0; p.cap = pl.cap;
   p.scale2 = a->scale * 1.4426950408889634f;
   p.ctas = pl.ctas;
   p.part_o = static_cast<float*>(a->workspace);
