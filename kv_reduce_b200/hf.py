@@ -312,6 +312,8 @@ def speculative_generate(target, draft, input_ids: torch.Tensor, *, max_new_toke
         r = verify_draft_tokens(logits, q_logits, proposal, uniforms, noise, temperature=temperature)
         accepted = int(r.accepted[0])
         new = r.tokens[0, :accepted + 1]
+        if int(new[-1]) < 0:     # not an id: an embedding would read out of range
+            raise RuntimeError("no token can follow: the target's logits are NaN or -inf throughout.")
         packed.crop(start + 1 + accepted)
         packed.commit()
         cache.crop([held + 1 + accepted])
