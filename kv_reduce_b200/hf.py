@@ -215,12 +215,27 @@ class PagedTargetCache(DynamicCache):
         return bool(self.keep) and self.pages.evict(self.keep, recent=self.recent, first=self.first)
 
 
+def _pads_left(mask: Optional[torch.Tensor]) -> bool:
+    """Whether a prompt's attention mask ([batch, tokens], or [batch, 1,
+    queries, keys] of truth values or of what is added to the scores) hides the
+    first token of a sequence from itself."""
+    if mask is None:
+        return False
+    first = mask[:, 0] if mask.dim() == 2 else mask[:, 0, 0, 0]
+    return not bool((first == 0 if first.is_floating_point() else first != 0).all())
+
+
 def install_target(model) -> None:
     """Route attention steps over a ``PagedTargetCache`` through the paged
     kernels: any number of new tokens, every sequence at its own length.  The
     prompt's forward (an empty cache) stays the model's own.  Positions come
     from ``position_ids``; pass them where sequences differ in length or
-    tokens have been evicted."""
+    tokens have been evicted.
+
+    Prompts of different lengths are padded on the right and the cache then
+    cropped to each one's own (``cache.crop(lengths)``); left padding would
+    stay in the cache and is refused.  After the prompt the attention mask is
+    not read: a token sees its sequence's tokens up to itself."""
     for layer in model.model.layers:
         attn = layer.self_attn
         original = attn.forward
@@ -232,6 +247,9 @@ def install_target(model) -> None:
             if not isinstance(cache, PagedTargetCache) or (
                     cache.pages.get_seq_length() == 0 if self.layer_idx == 0 else cache.prompt):
                 if isinstance(cache, PagedTargetCache):
+                    if self.layer_idx == 0 and _pads_left(attention_mask):
+                        raise ValueError("a paged target cache takes prompts padded on the right: "
+                                         "crop it to each prompt's length afterwards.")
                     cache.prompt = True
                 return _original(hidden_states, position_embeddings, attention_mask, past_key_values, **kwargs)
             if self.layer_idx == 0:
