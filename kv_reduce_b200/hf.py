@@ -234,7 +234,8 @@ def install_target(model) -> None:
 
     Prompts of different lengths are padded on the right and the cache then
     cropped to each one's own (``cache.crop(lengths)``); left padding would
-    stay in the cache and is refused.  After the prompt the attention mask is
+    stay in the cache and is refused.  A sliding layer's own window holds where
+    the cache's is not tighter.  After the prompt the attention mask is
     not read: a token sees its sequence's tokens up to itself."""
     for layer in model.model.layers:
         attn = layer.self_attn
@@ -262,7 +263,11 @@ def install_target(model) -> None:
             v = self.v_proj(hidden_states).view(view).transpose(1, 2)
             q, k = apply_rotary_pos_emb(q, k, *position_embeddings)
             cache.pages.append(self.layer_idx, k, v)
-            out = cache.pages.attention(self.layer_idx, q, scale=self.scaling, window=cache.window, sinks=cache.sinks)
+            window, sinks = cache.window, cache.sinks
+            own = getattr(self, "sliding_window", None) or 0
+            if own and not 0 < window <= own:        # a sliding layer's own window, unless the cache's is tighter
+                window, sinks = own, 0
+            out = cache.pages.attention(self.layer_idx, q, scale=self.scaling, window=window, sinks=sinks)
             return self.o_proj(out.transpose(1, 2).reshape(*shape, -1).contiguous()), None
 
         attn.forward = types.MethodType(forward, attn)

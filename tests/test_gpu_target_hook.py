@@ -31,3 +31,26 @@ def test_prompts_padded_on_the_right(built_lib):
     with pytest.raises(ValueError, match="right"):
         model(ids[:, :90], attention_mask=mask.flip(1), use_cache=True,
               past_key_values=hf.PagedTargetCache.for_model(model, 3, max_tokens=128))
+
+
+@torch.inference_mode()
+def test_sliding_layers(built_lib):
+    """A model with a sliding layer: its own logits, past the window."""
+    transformers = pytest.importorskip("transformers")
+    from kv_reduce_b200 import hf
+
+    torch.manual_seed(3)
+    cfg = transformers.Qwen2Config(vocab_size=512, hidden_size=768, intermediate_size=1024, num_hidden_layers=2,
+                                   num_attention_heads=6, num_key_value_heads=2, use_sliding_window=True,
+                                   sliding_window=24, max_window_layers=1, attn_implementation="sdpa")
+    model = transformers.Qwen2ForCausalLM(cfg).to(device="cuda", dtype=torch.bfloat16).eval()
+    for x in model.model.layers:                     # (attention that counts: the output's weights are small at random)
+        x.self_attn.v_proj.weight.mul_(8)
+    ids = torch.randint(0, 512, (1, 150), device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    want = model(ids).logits.float()
+    hf.install_target(model)
+    cache = hf.PagedTargetCache.for_model(model, 1, max_tokens=160)
+    got = [model(ids[:, a:b], past_key_values=cache, use_cache=True).logits
+           for a, b in ((0, 100), (100, 101), (101, 109), (109, 150))]
+    cos = torch.nn.functional.cosine_similarity(torch.cat(got, 1).float(), want, dim=-1)
+    assert cos.min().item() > 0.995

@@ -46,3 +46,19 @@ def test_left_padding_is_refused(calls, attn):
         model(ids[:, :1], past_key_values=cache, use_cache=True, position_ids=torch.tensor([[6], [4]]))
         assert cache.pages.seq_lengths() == [7, 5] and len(calls) == 2
         calls.clear()
+
+
+@torch.inference_mode()
+def test_sliding_layers_keep_their_window(calls):
+    """A layer with a window of its own is given it; the cache's may be tighter."""
+    model = tiny(use_sliding_window=True, sliding_window=10, max_window_layers=1)
+    assert [x.self_attn.sliding_window for x in model.model.layers] == [None, 10]
+    hf.install_target(model)
+    ids = torch.arange(6)[None]
+    for kw, want in ((dict(), [(0, 0), (10, 0)]), (dict(window=7, sinks=2), [(7, 2), (7, 2)]),
+                     (dict(window=20, sinks=2), [(20, 2), (10, 0)])):
+        cache = hf.PagedTargetCache.for_model(model, 1, max_tokens=32, **kw)
+        for _ in range(2):
+            model(ids, past_key_values=cache, use_cache=True)
+        assert calls == want
+        calls.clear()
