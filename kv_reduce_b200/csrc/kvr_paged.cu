@@ -42,6 +42,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cstring>
 
 namespace kvr {
@@ -151,7 +152,13 @@ struct Cfg {
 };
 
 // The reference of a row that no token has been seen by: far below any score.
-constexpr float kUnseen = -1e30f;
+constexpr float kUnseen = -FLT_MAX;
+
+// A fused x factor - mu keeps the digits of the product that are rounded off
+// in mu and in tiles that a mask cuts: up to half the spacing of numbers like
+// mu.  Below this that is 2^-15 on an exponent; past it (where from 2^27 on an
+// exponent would leave the range) the product is rounded first here too.
+constexpr float kFusedUpTo = 512.f;
 
 // The weights' range in the second product.  A reference is a maximum so far,
 // less kBelow, and moves when an exponent passes kBelow + 8; the weights' rest
@@ -646,6 +653,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
     // ------------------------------------------------------------ consumers
     const uint32_t my_lanes = (uint32_t)warp << 21;   // tensor-memory lanes 32 w ..
     float l[N];                                       // this thread's tokens' share of the rows' sums
+    bool huge = false;                                // a reference is past kFusedUpTo
     // A segment's query rows, row r = t * G + g; read while the segment before it is finished (N = 64: not, for
     // the registers).
     constexpr int QV = N * C::PIECES / kConsumers;
@@ -745,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
 #pragma unroll
         for (int r = 0; r < N; ++r) {
           if ((r & 3) == 0 && r >= n_rows) break;
-          x[r] = __fmaf_rn(x[r], factor, -mu_s[r]);
+          x[r] = huge ? __fsub_rn(__fmul_rn(x[r], factor), mu_s[r]) : __fmaf_rn(x[r], factor, -mu_s[r]);
           if (r < n_rows) hot = fmaxf(hot, x[r]);
         }
         return hot > kBelow<HALF> + 8.f;
@@ -771,6 +779,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
           else store_rows<N, false>(v, smax + warp * N, lane);
         }
         consumer_sync();
+        bool far = false;
         if (tid < n_rows) {   // thread = row
           const float before = mu_s[tid];
           float mn = before;
@@ -778,8 +787,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
           for (int w = 0; w < kWarps; ++w) mn = fmaxf(mn, smax[w * N + tid] - kBelow<HALF>);
           mu_s[tid] = mn;
           alpha_s[tid] = fast_exp2(before - mn);
+          far = fabsf(mn) > kFusedUpTo && mn != kUnseen;
         }
-        consumer_sync();
+        huge = consumer_any(far);
         if (!ds.first) {
 #pragma unroll
           for (int c = 0; c < N; c += 16)

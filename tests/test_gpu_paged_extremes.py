@@ -1,9 +1,11 @@
 """Paged attention where scores, values or lengths leave the ordinary range.
 Tolerances as derived in test_gpu_paged.py."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_paged import check, kvr, make  # noqa: F401  (kvr: the fixture)
+from test_gpu_paged import check, kvr, make, reference  # noqa: F401  (kvr: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -36,8 +38,6 @@ def test_one_token_outweighs_the_others(kvr, HQ, H, D, T, gap, dtype):  # noqa: 
 
 def check_few(kvr, data, few):  # noqa: F811
     """The whole batch runs; `few` sequences are compared with the formula."""
-    from test_gpu_paged import reference
-
     q, k, v, table, n = data
     out, lse = kvr.paged_decode_attention(q, k, v, table, n, scale=1.0, return_lse=True)
     want, size, want_lse, _ = reference(q[few], k, v, table[few], n[few], scale=1.0)
@@ -45,3 +45,38 @@ def check_few(kvr, data, few):  # noqa: F811
     err = (out[few].double() - want).abs()
     assert (err <= (2 * u + 2 ** -12) * size + 1e-7).all(), f"out off by {(err / size).max().item():.2e}"
     assert (lse[few].double() - want_lse).abs().max().item() <= 2 ** -14
+
+
+def far_scores(lengths, HQ, H, D, T, dtype, size, seed):
+    """Scores of about `size` (either sign), products of two numbers that the
+    type holds, so exact: a few equal ones on top and the others a step or
+    more below."""
+    q, k, v, table, n = make(lengths, HQ, H, D, T, 16, dtype, seed=seed, garbage=False)
+    root = 2.0 ** round(math.log2(abs(size)) / 2)
+    q.zero_()
+    k.zero_()
+    q[..., 3] = root
+    step = torch.randint(0, 4, k.shape[:3], device="cuda", generator=torch.Generator("cuda").manual_seed(seed))
+    step = torch.where(torch.rand(step.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) < 0.9,
+                       step + 1, 0)
+    k[..., 3] = (root * (1.5 - step / 64) if size > 0 else -root * (1 + step / 64)).to(k.dtype)
+    return q, k, v, table, n
+
+
+@pytest.mark.parametrize("dtype,size", [("bf16", 2.0 ** x) for x in (20, 30, 60, 118)] +
+                         [("bf16", -2.0 ** x) for x in (20, 30, 60, 118)] + [("fp16", 2.0 ** 28), ("fp16", -2.0 ** 28)])
+@pytest.mark.parametrize("HQ,H,D,T,window", [(12, 2, 128, 1, 0), (8, 2, 64, 3, 0), (12, 2, 128, 3, 200)])
+def test_scores_far_from_zero(kvr, HQ, H, D, T, window, dtype, size):  # noqa: F811
+    """Only differences of scores count, however large the scores: down to
+    those below -1e30, and where fp32's spacing is more than the exponents'
+    range."""
+    lengths = [1500, 130, 129, 1, 0, 9000]
+    q, k, v, table, n = far_scores(lengths, HQ, H, D, T, dtype, size, seed=HQ)
+    out, lse = kvr.paged_decode_attention(q, k, v, table, n, scale=1.0, window=window, return_lse=True)
+    want, _, want_lse, _ = reference(q, k, v, table, n, window, scale=1.0)
+    u = 2.0 ** -9 if dtype == "bf16" else 2.0 ** -12
+    _, size_v, _, _ = reference(q, k, v.abs(), table, n, window, scale=1.0)
+    assert ((out.double() - want).abs() <= (2 * u + 2 ** -12) * size_v + 1e-7).all()
+    empty = want_lse == -math.inf
+    assert torch.equal(lse == -math.inf, empty)
+    assert ((lse.double() - want_lse).abs() <= 2.0 ** -22 * want_lse.abs() + 2 ** -14)[~empty].all()
