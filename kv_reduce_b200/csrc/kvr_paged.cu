@@ -56,10 +56,6 @@ constexpr int kLoadWarp = 4, kMmaWarp = 5;
 constexpr int kThreads = kConsumers + 64;
 constexpr int kGroup = 16;                    // CTAs a join takes at a time
 
-// Rows that no mask leaves anything to keep m = -inf; 0 stands in for it
-// wherever it would be subtracted.
-__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
-
 template <bool HALF>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -107,7 +103,7 @@ struct Params {
   uint16_t* out;
   float* lse;       // [B, HQ, T] or null
   float* scores;    // [B, HKV, R, score_stride] or null: x_ij for the weights kernel
-  float* row_lse2;  // [B, HKV, R], with scores; inf for a row that is no token's
+  float2* row_stat; // [B, HKV, R], with scores: reference and log2 of the sum; inf, inf for a row that is no token's
   int64_t score_stride;
   int B, HQ, HKV, T, G, R, row_tiles, window, sinks, cap;
   float scale2;     // scale * log2(e)
@@ -926,8 +922,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
             alpha_s[tid] = none ? 0.f : 1.f / sum;
             const float lse2 = none ? -INFINITY : mu_s[tid] + log2f(sum);
             if (p.lse) p.lse[row_s[tid]] = lse2 * 0.6931471805599453f;
-            if (p.row_lse2)
-              p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + tid] = pos_s[tid] < 0 ? INFINITY : lse2;
+            if (p.row_stat)
+              p.row_stat[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + tid] =
+                  pos_s[tid] < 0 ? make_float2(INFINITY, INFINITY) : make_float2(mu_s[tid], none ? 0.f : log2f(sum));
           } else {
             *reinterpret_cast<float2*>(p.part_ml + (slot_o * ROWS + tid) * 2) = make_float2(mu_s[tid], sum);
           }
@@ -1034,8 +1031,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
               if (col == 0) {
                 const float lse2 = none ? -INFINITY : mm + log2f(sum);
                 if (p.lse) p.lse[row_s[r]] = lse2 * 0.6931471805599453f;
-                if (p.row_lse2)
-                  p.row_lse2[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + r] = pos_s[r] < 0 ? INFINITY : lse2;
+                if (p.row_stat)
+                  p.row_stat[(int64_t)(sb * p.HKV + sh) * p.R + rt * N + r] =
+                      pos_s[r] < 0 ? make_float2(INFINITY, INFINITY) : make_float2(mm, none ? 0.f : log2f(sum));
               }
             }
           };
@@ -1075,7 +1073,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
   }
 }
 
-// token_weights[b, j] += sum over the heads and new tokens of 2^(x - lse2).
+// token_weights[b, j] += sum over the heads and new tokens of 2^((x - m) - log2 l),
+// with m and l apart: their sum is rounded to the spacing of numbers like m.
 // A CTA takes 256 / W tokens, 256 / W threads every W-th row; their sums are
 // added in order: no atomics, a fixed order of sums.  What bounds it: round
 // trips where tokens are few (W = 8), else the scores, written by the
@@ -1093,14 +1092,14 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_co
   if (j0 >= len || (j0 + TOKENS <= s.lo && j0 >= p.sinks)) return;
   const bool seen = j < len && (j >= s.lo || j < p.sinks);
   const float* src = p.scores + (int64_t)b * rows * p.score_stride + j;
-  const float* lse2 = p.row_lse2 + (int64_t)b * rows;
+  const float2* stat = p.row_stat + (int64_t)b * rows;
   float sum = 0.f;
   if (seen) {
 #pragma unroll 4
     for (int r = part; r < rows; r += W) {
-      const float y = lse2[r];
-      const float w = fast_exp2(src[(int64_t)r * p.score_stride] - finite_or_zero(y));
-      sum += y == INFINITY ? 0.f : w;   // (the scores of a row that is no token's may be anything)
+      const float2 y = stat[r];
+      const float w = fast_exp2((src[(int64_t)r * p.score_stride] - y.x) - y.y);
+      sum += y.y == INFINITY ? 0.f : w;   // (the scores of a row that is no token's may be anything)
     }
   }
   if constexpr (W > 1) {
@@ -1176,7 +1175,7 @@ struct Plan {
   int G, R, n, row_tiles, cap, ctas;
   int part;   // sequences per launch (with token weights)
   int64_t score_stride;
-  size_t part_o, part_ml, lse2, scores;
+  size_t part_o, part_ml, stats, scores;
 };
 
 static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
@@ -1222,7 +1221,7 @@ static int plan_of(const kvr_paged_attention_args* a, Plan* out) {
   const size_t seq_rows = (size_t)a->kv_heads * p.R, seq_scores = seq_rows * p.score_stride * sizeof(float);
   p.part = a->token_weights ? (int)std::min<size_t>(a->batch, std::max<size_t>(1, kScoreBytes / seq_scores)) : a->batch;
   const size_t all_rows = p.part * seq_rows;
-  p.lse2 = a->token_weights ? (all_rows * sizeof(float) + 255) / 256 * 256 : 0;
+  p.stats = a->token_weights ? (all_rows * sizeof(float2) + 255) / 256 * 256 : 0;
   p.scores = a->token_weights ? all_rows * p.score_stride * sizeof(float) : 0;
   *out = p;
   return KVR_OK;
@@ -1325,7 +1324,7 @@ extern "C" int kvr_paged_attention_plan(const kvr_paged_attention_args* a, size_
   }
   if (workspace_bytes) *workspace_bytes = p.part_o + p.part_ml;
   if (counter_count) *counter_count = 2 * (size_t)p.ctas;
-  if (scores_bytes) *scores_bytes = p.lse2 + p.scores;
+  if (scores_bytes) *scores_bytes = p.stats + p.scores;
   return KVR_OK;
 }
 
@@ -1362,7 +1361,7 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
     if (!paged::mult8(x)) return KVR_ERR_MISALIGNED;
   if (!a->workspace || a->workspace_bytes < pl.part_o + pl.part_ml || !a->counters) return KVR_ERR_WORKSPACE;
   if (!aligned16(a->workspace)) return KVR_ERR_MISALIGNED;
-  if (a->token_weights && (!a->scores || a->scores_bytes < pl.lse2 + pl.scores)) return KVR_ERR_WORKSPACE;
+  if (a->token_weights && (!a->scores || a->scores_bytes < pl.stats + pl.scores)) return KVR_ERR_WORKSPACE;
   if (a->token_weights && !aligned16(a->scores)) return KVR_ERR_MISALIGNED;
 
   paged::Params p;
@@ -1384,8 +1383,8 @@ extern "C" int kvr_paged_attention(const kvr_paged_attention_args* a, kvr_stream
   p.counts = a->new_counts;
   p.out = static_cast<uint16_t*>(a->out);
   p.lse = a->lse;
-  p.row_lse2 = a->token_weights ? static_cast<float*>(a->scores) : nullptr;
-  p.scores = a->token_weights ? reinterpret_cast<float*>(static_cast<uint8_t*>(a->scores) + pl.lse2) : nullptr;
+  p.row_stat = a->token_weights ? static_cast<float2*>(a->scores) : nullptr;
+  p.scores = a->token_weights ? reinterpret_cast<float*>(static_cast<uint8_t*>(a->scores) + pl.stats) : nullptr;
   p.score_stride = pl.score_stride;
   p.B = a->batch; p.HQ = a->q_heads; p.HKV = a->kv_heads; p.T = a->new_tokens;
   p.G = pl.G; p.R = pl.R; p.row_tiles = pl.row_tiles;

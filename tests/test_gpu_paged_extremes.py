@@ -80,3 +80,15 @@ def test_scores_far_from_zero(kvr, HQ, H, D, T, window, dtype, size):  # noqa: F
     empty = want_lse == -math.inf
     assert torch.equal(lse == -math.inf, empty)
     assert ((lse.double() - want_lse).abs() <= 2.0 ** -22 * want_lse.abs() + 2 ** -14)[~empty].all()
+
+
+@pytest.mark.parametrize("dtype,size", [("bf16", x) for x in (2.0 ** 12, 2.0 ** 20, -2.0 ** 30, 2.0 ** 118, -2.0 ** 118)] +
+                         [("fp16", 2.0 ** 14), ("fp16", -2.0 ** 28)])
+@pytest.mark.parametrize("HQ,H,D,T", [(12, 2, 128, 1), (8, 2, 64, 3)])
+def test_weights_of_scores_far_from_zero(kvr, HQ, H, D, T, dtype, size):  # noqa: F811
+    """Each token's share, not rounded to the spacing of the scores."""
+    q, k, v, table, n = far_scores([1500, 130, 129, 1, 0, 9000], HQ, H, D, T, dtype, size, seed=HQ)
+    w = torch.full((6, table.shape[1] * 16), 0.25, device="cuda")
+    kvr.paged_decode_attention(q, k, v, table, n, scale=1.0, token_weights=w)
+    want = reference(q, k, v, table, n, scale=1.0)[3]
+    assert ((w.double() - 0.25 - want).abs() <= 2 ** -14 * want + 1e-6).all()
