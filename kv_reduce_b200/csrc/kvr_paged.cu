@@ -946,7 +946,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               if (c + r >= n_rows) break;
-              const float x = o[r] + rest[r] * (1.f / kRest<HALF>);
+              // (an infinite value that the row sees makes the rest, 0 or negative, NaN or of the other sign: o has it)
+              const float y = rest[r] * (1.f / kRest<HALF>), x = fabsf(y) <= FLT_MAX ? o[r] + y : o[r];
               if (whole)
                 p.out[(int64_t)row_s[c + r] * D + d] =
                     (uint16_t)pack2<HALF>(alpha_s[c + r] == 0.f ? 0.f : x * alpha_s[c + r], 0.f);

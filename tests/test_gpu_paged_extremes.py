@@ -92,3 +92,24 @@ def test_weights_of_scores_far_from_zero(kvr, HQ, H, D, T, dtype, size):  # noqa
     kvr.paged_decode_attention(q, k, v, table, n, scale=1.0, token_weights=w)
     want = reference(q, k, v, table, n, scale=1.0)[3]
     assert ((w.double() - 0.25 - want).abs() <= 2 ** -14 * want + 1e-6).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("HQ,H,D,T", [(12, 2, 128, 1), (8, 2, 64, 4), (12, 2, 128, 5), (8, 1, 128, 9)])
+def test_infinite_values_that_are_seen(kvr, HQ, H, D, T, dtype):  # noqa: F811
+    """They reach the output as what they are: an infinity of its sign, NaN
+    where both signs meet or a value is NaN; other elements are untouched."""
+    lengths = [300, 129, 40, 9000]
+    q, k, v, table, n = make(lengths, HQ, H, D, T, 16, dtype, seed=T)
+    clean = kvr.paged_decode_attention(q, k, v, table, n)
+    bad = [(0, math.inf), (1, -math.inf), (2, math.nan), (3, math.inf), (3, -math.inf)]
+    for b, length in enumerate(lengths):
+        for at in (5, length // 2, length - T):           # tokens that every query sees
+            for c, x in bad[:4]:
+                v[table[b, at // 16].long(), :, at % 16, 10 * c] = x
+        v[table[b, 3 // 16].long(), :, 3, 30] = -math.inf
+    out = kvr.paged_decode_attention(q, k, v, table, n)
+    assert (out[..., 0] == math.inf).all() and (out[..., 10] == -math.inf).all()
+    assert out[..., 20].isnan().all() and out[..., 30].isnan().all()
+    others = [i for i in range(D) if i not in (0, 10, 20, 30)]
+    assert torch.equal(out[..., others], clean[..., others])
