@@ -170,7 +170,7 @@ template <bool HALF>
 constexpr float kRest = HALF ? 2048.f : 1.f;
 
 struct Desc {
-  int first, last, full, token0;   // full: every row sees every token
+  int first, last, full, token0;   // full: every row sees every token; last: 2 where the sequence is too long for its table
   int b, h, rt, len;
   int n_tiles, seg_start;          // of the segment: tiles, flat index of the first
   int whole;                       // with `last`: all of the segment's tiles are this CTA's
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       u.d.full = token0 + TILE <= ld_len - p.T + 1 &&
                  (p.window == 0 || token0 > ld_len - 1 - p.window || token0 + TILE <= p.sinks);
       --ld_left;
-      u.d.last = ld_left == 0 || ld_tile + 1 == ld_span.n;
+      u.d.last = ld_left == 0 || ld_tile + 1 == ld_span.n ? (ld_over ? 2 : 1) : 0;
       u.d.whole = ld_from == 0 && ld_tile + 1 == ld_span.n;
       {
         const int j = token0 + (lane & 7) * 16;
@@ -897,7 +897,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       proxy_fence();
       tc_before_sync();
       __syncwarp();
-      const bool last = ds.last, whole = ds.whole;
+      const int last = ds.last;
+      const bool whole = ds.whole;
       const int sb = ds.b, sh = ds.h, n_tiles = ds.n_tiles, seg_start = ds.seg_start;
       if (lane == 0) bar_arrive(p_full);
 
@@ -908,7 +909,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
           load_queries(dn.b, dn.h, dn.rt);
         }
         // ---- the rows' sums over the tokens' threads, while the last product runs
-        if (failed)
+        if (failed || last == 2)
 #pragma unroll
           for (int r = 0; r < N; ++r) l[r] = NAN;
         if (N == 16 && n_rows <= 8) store_rows<8, true>(l, ssum + warp * N, lane);
@@ -918,7 +919,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
         if (tid < n_rows) {   // thread = row
           const float sum = ssum[tid] + ssum[N + tid] + ssum[2 * N + tid] + ssum[3 * N + tid];
           if (whole) {
-            const bool none = sum == 0.f || pos_s[tid] < 0;
+            const bool none = sum == 0.f || (pos_s[tid] < 0 && last != 2);
             alpha_s[tid] = none ? 0.f : 1.f / sum;
             const float lse2 = none ? -INFINITY : mu_s[tid] + log2f(sum);
             if (p.lse) p.lse[row_s[tid]] = lse2 * 0.6931471805599453f;
@@ -1021,7 +1022,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
                 if (col == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, sum);
                 continue;
               }
-              const bool none = sum == 0.f || pos_s[r] < 0;
+              const bool none = sum == 0.f || (pos_s[r] < 0 && last != 2);
               if (none)
 #pragma unroll
                 for (int z = 0; z < 8; ++z) acc[z] = 0.f;

@@ -113,3 +113,20 @@ def test_infinite_values_that_are_seen(kvr, HQ, H, D, T, dtype):  # noqa: F811
     assert out[..., 20].isnan().all() and out[..., 30].isnan().all()
     others = [i for i in range(D) if i not in (0, 10, 20, 30)]
     assert torch.equal(out[..., others], clean[..., others])
+
+
+@pytest.mark.parametrize("HQ,H,D,T", [(12, 2, 128, 1), (12, 2, 128, 9), (8, 1, 64, 33)])
+def test_sequences_longer_than_a_short_table(kvr, HQ, H, D, T):  # noqa: F811
+    """NaN for every query of such a sequence, also where the table holds fewer
+    tokens than there are queries, or none."""
+    q, k, v, table, n = make([20, 30, 8], HQ, H, D, T, 4, seed=T)
+    for width in (0, 1, 2):
+        for window in (0, 5):
+            out, lse = kvr.paged_decode_attention(q, k, v, table[:, :width], n, window=window, return_lse=True)
+            assert out[:2].isnan().all() and lse[:2].isnan().all()
+            if width == 2:                               # the last one fits, whoever its neighbours are
+                alone = kvr.paged_decode_attention(q[2:], k, v, table[2:, :2], n[2:], window=window)
+                u = 2.0 ** -7
+                assert torch.allclose(out[2:].float(), alone.float(), rtol=u, atol=u) and not alone.isnan().any()
+            else:
+                assert out[2].isnan().all()
