@@ -59,6 +59,14 @@ bool rows16(const at::Tensor& t) {
 // elements are contiguous and rows start on 16 bytes; others are copied.
 at::Tensor rows(const at::Tensor& t) { return rows16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
+// Whether elements share memory along an axis (an expanded tensor): threads
+// would write to one place.
+bool shares_memory(const at::Tensor& t) {
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) == 0) return true;
+  return false;
+}
+
 enum class Op { attention, verify };
 struct Scratch {
   std::mutex mu;   // held from taking the buffers to the call's last launch
@@ -157,6 +165,7 @@ void paged_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
   TORCH_CHECK_VALUE(key.scalar_type() == kp.scalar_type() && value.scalar_type() == kp.scalar_type(),
                     "key and value must have the pages' dtype.");
   TORCH_CHECK_VALUE(key.size(3) % 8 == 0, "head_dim must be a multiple of 8.");
+  TORCH_CHECK_VALUE(!shares_memory(kp) && !shares_memory(vp), "pages that are written must not be expanded tensors.");
   const int* counts = counts_of(new_counts, lengths);
   c10::cuda::CUDAGuard guard(key.device());
   if (key.numel() == 0) return;
@@ -207,6 +216,8 @@ std::tuple<at::Tensor, at::Tensor> paged_attention(const at::Tensor& query, cons
                           w.size(0) == query.size(0) && w.size(1) >= table.size(1) * kp.size(2) &&
                           (w.size(1) <= 1 || w.stride(1) == 1),
                       "token_weights must be fp32 [batch, >= block_table.shape[1] * page_size] with contiguous rows.");
+    TORCH_CHECK_VALUE(w.size(0) <= 1 || w.stride(0) >= table.size(1) * kp.size(2),
+                      "token_weights are added to: their rows must not share memory.");
   }
   c10::cuda::CUDAGuard guard(dev);
   at::Tensor out = at::empty(query.sizes(), query.options().memory_format(at::MemoryFormat::Contiguous));
@@ -277,6 +288,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_evict(const at::Tensor& kp,
                     "new_block_table must hold pages for min(keep, block_table.shape[1] * page_size) tokens.");
   TORCH_CHECK_VALUE(cap <= 320000, "eviction takes block tables of up to 320000 tokens.");
   TORCH_CHECK_VALUE(kp.size(3) % 8 == 0, "head_dim must be a multiple of 8.");
+  TORCH_CHECK_VALUE(!shares_memory(kp) && !shares_memory(vp), "pages that are written must not be expanded tensors.");
   c10::cuda::CUDAGuard guard(dev);
   const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
   at::Tensor kept = at::empty({B, keep}, i32), new_lengths = at::empty({B}, i32);
