@@ -81,18 +81,18 @@ __device__ __forceinline__ uint32_t ordered(float w) {
 }
 
 // Exclusive sum over the block; *total the whole.
-__device__ __forceinline__ int block_scan(int x, int* buf, int* total) {
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* buf, uint32_t* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = x;
+  uint32_t incl = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(~0u, incl, o);
+    const uint32_t y = __shfl_up_sync(~0u, incl, o);
     if (lane >= o) incl += y;
   }
   __syncthreads();
   if (lane == 31) buf[warp] = incl;
   __syncthreads();
-  int before = 0, all = 0;
+  uint32_t before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += buf[w];
@@ -120,7 +120,7 @@ template <int CL>
 __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ Params p) {
   extern __shared__ float slice[];     // [p.slice]
   __shared__ __align__(16) uint32_t hist[2][kBins];
-  __shared__ int buf[kThreads / 32];
+  __shared__ uint32_t buf[kThreads / 32];
   __shared__ uint32_t s_counts;        // tokens kept for certain | ties << 16
   __shared__ int s_digit[2];
   const int tid = threadIdx.x, rank = CL == 1 ? 0 : blockIdx.x % CL, b = blockIdx.x / CL;
@@ -189,8 +189,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
           }
         }
       }
-      int total;
-      int before = block_scan((int)(c[0] + c[1] + c[2] + c[3]), buf, &total);
+      uint32_t total;
+      int before = (int)block_scan(c[0] + c[1] + c[2] + c[3], buf, &total);
 #pragma unroll
       for (int j = 3; j >= 0; --j) {
         if (before < need && need <= before + (int)c[j]) {
@@ -209,17 +209,17 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   }
   // prefix is the key of the last token to be kept; `need` of its ties are, the first ones
   const int run = ((n + kThreads - 1) / kThreads) | 1, r0 = min(tid * run, n), r1 = min(r0 + run, n);
-  int mine = 0;
+  uint32_t mine = 0;   // (a slice may hold 40,000 ties: the upper half needs its sign bit)
   for (int i = r0; i < r1; ++i) {
     const uint32_t k = ordered(slice[i]);
     const bool cand = i >= lo && i < hi;
-    mine += !cand || (any && k > prefix) ? 1 : any && k == prefix ? 1 << 16 : 0;
+    mine += !cand || (any && k > prefix) ? 1u : any && k == prefix ? 1u << 16 : 0u;
   }
-  int total;
-  const int before = block_scan(mine, buf, &total);
-  int sure = before & 0xffff, ties = (int)((uint32_t)before >> 16);
+  uint32_t total;
+  const uint32_t before = block_scan(mine, buf, &total);
+  int sure = (int)(before & 0xffff), ties = (int)(before >> 16);
   if (CL > 1) {
-    if (tid == 0) s_counts = (uint32_t)total;
+    if (tid == 0) s_counts = total;
     cluster_sync();
     // lane r asks CTA r
     const int lane = tid & 31;
