@@ -150,11 +150,16 @@ struct Cfg {
 // The reference of a row that no token has been seen by: far below any score.
 constexpr float kUnseen = -FLT_MAX;
 
-// A fused x factor - mu keeps the digits of the product that are rounded off
-// in mu and in tiles that a mask cuts: up to half the spacing of numbers like
-// mu.  Below this that is 2^-15 on an exponent; past it (where from 2^27 on an
-// exponent would leave the range) the product is rounded first here too.
-constexpr float kFusedUpTo = 512.f;
+// x factor - m of two rows, the product rounded first.  Fused, it would keep the
+// digits that are rounded off in m and in tiles that a mask cuts: half the
+// spacing of numbers like m, which from 2^27 on is more than the exponents'
+// range.
+__device__ __forceinline__ void two_exponents(float& x0, float& x1, float factor, float2 m) {
+  asm("{\n.reg .b64 x, f, m, one;\nmov.b64 x, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 m, {%3, %4};\n"
+      "mov.b64 one, {%5, %5};\nmul.rn.f32x2 x, x, f;\nfma.rn.f32x2 x, m, one, x;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "+f"(x0), "+f"(x1)
+      : "f"(factor), "f"(m.x), "f"(m.y), "f"(-1.f));
+}
 
 // The weights' range in the second product.  A reference is a maximum so far,
 // less kBelow, and moves when an exponent passes kBelow + 8; the weights' rest
@@ -649,7 +654,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
     // ------------------------------------------------------------ consumers
     const uint32_t my_lanes = (uint32_t)warp << 21;   // tensor-memory lanes 32 w ..
     float l[N];                                       // this thread's tokens' share of the rows' sums
-    bool huge = false;                                // a reference is past kFusedUpTo
     // A segment's query rows, row r = t * G + g; read while the segment before it is finished (N = 64: not, for
     // the registers).
     constexpr int QV = N * C::PIECES / kConsumers;
@@ -747,10 +751,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
       auto exponents = [&]() {
         float hot = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < N; ++r) {
+        for (int r = 0; r < N; r += 2) {
           if ((r & 3) == 0 && r >= n_rows) break;
-          x[r] = huge ? __fsub_rn(__fmul_rn(x[r], factor), mu_s[r]) : __fmaf_rn(x[r], factor, -mu_s[r]);
+          two_exponents(x[r], x[r + 1], factor, *reinterpret_cast<const float2*>(mu_s + r));
           if (r < n_rows) hot = fmaxf(hot, x[r]);
+          if (r + 1 < n_rows) hot = fmaxf(hot, x[r + 1]);
         }
         return hot > kBelow<HALF> + 8.f;
       };
@@ -775,7 +780,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
           else store_rows<N, false>(v, smax + warp * N, lane);
         }
         consumer_sync();
-        bool far = false;
         if (tid < n_rows) {   // thread = row
           const float before = mu_s[tid];
           float mn = before;
@@ -783,9 +787,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, N>::CTAS) attention_kernel(co
           for (int w = 0; w < kWarps; ++w) mn = fmaxf(mn, smax[w * N + tid] - kBelow<HALF>);
           mu_s[tid] = mn;
           alpha_s[tid] = fast_exp2(before - mn);
-          far = fabsf(mn) > kFusedUpTo && mn != kUnseen;
         }
-        huge = consumer_any(far);
+        consumer_sync();
         if (!ds.first) {
 #pragma unroll
           for (int c = 0; c < N; c += 16)
