@@ -184,7 +184,14 @@ class PagedTargetCache(DynamicCache):
     """The target model's cache in pages.  ``max_tokens``: what each sequence
     may hold; with ``keep`` the cache is brought back to that many tokens, the
     ``first`` ones, the ``recent`` ones and the heaviest of the others, by
-    ``evict()``.  ``window`` and ``sinks`` restrict the attention."""
+    ``evict()``.  ``window`` and ``sinks`` restrict the attention of the steps
+    after the prompt.
+
+    A token's weight is what the steps' queries gave it, those of refused
+    drafts among them.  The prompt's own attention runs in the model and is
+    not counted: an eviction right after the first step ranks the prompt by
+    that step's few queries alone, so leave ``recent`` room, or evict after
+    some steps."""
 
     def __init__(self, num_layers: int, batch: int, kv_heads: int, head_dim: int, *, max_tokens: int,
                  page_size: int = 16, dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda",
@@ -287,8 +294,9 @@ def speculative_generate(target, draft, input_ids: torch.Tensor, *, max_new_toke
 
     Returns the ids with the new tokens, and how many drafted tokens each
     round accepted.  ``window``, ``sinks``, ``keep``, ``recent``, ``first``
-    are the target cache's (``PagedTargetCache``); ``draft_kw`` the draft
-    cache's (k_bits, v_bits, group_size).
+    are the target cache's (``PagedTargetCache``, which says what an early
+    eviction goes by); ``draft_kw`` the draft cache's (k_bits, v_bits,
+    group_size).  Raises RuntimeError where the target's logits leave no token.
     """
     if input_ids.shape[0] != 1:
         raise ValueError("the packed draft cache serves one sequence length: generate one sequence at a time.")

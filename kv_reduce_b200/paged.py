@@ -138,6 +138,15 @@ class PagedKVCache:
 
     With ``track_weights`` the attention adds up what weight every token got
     (per layer), and ``evict`` brings the sequences down to a budget by it.
+    The totals are those of all queries that ``attention`` was called with:
+    ``crop`` forgets the removed tokens' own totals, but what their queries
+    added to the tokens before them stays (drafted tokens that a verification
+    refused have voted), and an attention that did not run here, a prompt's
+    say, has not been counted.
+
+    ``max_pages``: pages a sequence may come to, the table's width (default:
+    the whole pool).  The table and the weights take batch * max_pages entries
+    and are kept on the host too, so in a large pool give it.
     """
 
     def __init__(self, num_layers: int, batch: int, kv_heads: int, head_dim: int, *, num_pages: int,
@@ -259,7 +268,9 @@ class PagedKVCache:
     def evict(self, keep: int, *, recent: int = 0, first: int = 0) -> bool:
         """Bring every sequence down to ``keep`` tokens (see ``paged_evict``),
         each layer by its own weights; the rows move to fresh pages.  False,
-        and nothing done, while no sequence is longer."""
+        and nothing done, while no sequence is longer.  Tokens that no counted
+        query has seen weigh 0, and of equal weights the first are kept: call
+        it once a few steps have run over a prompt, or with ``recent``."""
         if self.token_weights is None:
             raise ValueError("evict needs a cache made with track_weights=True.")
         if keep <= 0 or recent < 0 or first < 0 or first + recent > keep:
