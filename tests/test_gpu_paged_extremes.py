@@ -130,3 +130,10 @@ def test_sequences_longer_than_a_short_table(kvr, HQ, H, D, T):  # noqa: F811
                 assert torch.allclose(out[2:].float(), alone.float(), rtol=u, atol=u) and not alone.isnan().any()
             else:
                 assert out[2].isnan().all()
+
+
+@pytest.mark.parametrize("HQ,H,D,T", [(12, 2, 128, 200), (8, 2, 64, 131), (4, 4, 128, 300), (7, 1, 64, 150)])
+def test_chunks_of_a_prompt(kvr, HQ, H, D, T):  # noqa: F811
+    """Hundreds of new tokens, as the target's hook sends them."""
+    check(kvr, make([1000, T, T - 40, 1, 0], HQ, H, D, T, 16, seed=T))
+    check(kvr, make([777, T + 3], HQ, H, D, T, 24, "fp16", seed=T), 90, 5)
