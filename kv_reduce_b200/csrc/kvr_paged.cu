@@ -31,12 +31,13 @@
 //  * A sequence that several CTAs share is joined by the last of them to
 //    arrive, in the order of the CTAs: the result does not depend on timing.
 //
-// Measured (16-bit types, against a copy's 6547 GB/s): 16 sequences of 16K to
-// 32K, 32 query and 8 KV heads of 128, 1.61 GB in 238 us, 6780 GB/s; 64 of 4K
-// to 16K with 5 new tokens each, 12 and 2 heads of 128, 0.67 GB in 119 us,
-// 5630 GB/s; 32 of up to 8K, 32 and 8 heads of 64, 0.27 GB in 50 us, 5400
-// GB/s; one of 32K, 12 and 2 heads of 128, 34 MB in 17 us, of which about 5
-// are the start (lengths, page numbers, first tiles) and 4 the join.
+// Measured (16-bit types, against a copy's 6547 GB/s, on several GPUs): 16
+// sequences of 16K to 32K, 32 query and 8 KV heads of 128, 1.61 GB in 239 to
+// 244 us, 6600 to 6740 GB/s; 64 of 4K to 16K with 5 new tokens each, 12 and 2
+// heads of 128, 0.67 GB in 121 to 132 us, 5080 to 5530 GB/s; 32 of up to 8K, 32
+// and 8 heads of 64, 0.27 GB in 51 us, 5270 GB/s; one of 32K, 12 and 2 heads
+// of 128, 34 MB in 17 us, of which about 5 are the start (lengths, page
+// numbers, first tiles) and 4 the join.
 #include "kvr_ring.cuh"
 
 #include <cuda.h>
