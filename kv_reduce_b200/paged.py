@@ -171,8 +171,9 @@ class PagedKVCache:
         self._pages: List[List[int]] = [[] for _ in range(self.batch)]
         self._lengths = [0] * self.batch
         self._width = 0      # pages of the longest sequence
-        # what the last advance gave each sequence, whether that differed, and the counts that the device has
-        self._new, self._ragged = [0] * self.batch, False
+        # what advance gave each sequence, whether that differed, whether a step has used it, and the counts that the
+        # device has
+        self._new, self._ragged, self._used = [0] * self.batch, False, True
         self.new_counts = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
         self._counts_of = list(self._new)
 
@@ -198,7 +199,8 @@ class PagedKVCache:
         """Lengthen the sequences (by one number, or one each) and give them
         pages; the rows are written by ``append``.  Where the numbers differ,
         ``append`` and ``attention`` take the largest as T and each sequence's
-        new tokens as the last of the T."""
+        new tokens as the last of the T.  Numbers given before the rows were
+        written add up."""
         more = [int(tokens)] * self.batch if isinstance(tokens, int) else [int(t) for t in tokens]
         if len(more) != self.batch or min(more) < 0:
             raise ValueError(f"advance needs a number of tokens >= 0 for each of {self.batch} sequences.")
@@ -210,7 +212,9 @@ class PagedKVCache:
         for pages, n in zip(self._pages, need):
             pages.extend(self._free.pop() for _ in range(n))
         self._lengths = [n + m for n, m in zip(self._lengths, more)]
-        self._new, self._ragged = more, min(more) != max(more)
+        if not self._used:       # rows made room for earlier and not written yet
+            more = [n + m for n, m in zip(self._new, more)]
+        self._new, self._ragged, self._used = more, min(more) != max(more), False
         self._upload(any(n > 0 for n in need))
 
     def crop(self, lengths: Union[int, Sequence[int]]) -> None:
@@ -243,10 +247,11 @@ class PagedKVCache:
         """Write the tokens that ``advance`` made room for: key and value
         [batch, kv_heads, T, head_dim], T the most that a sequence was given,
         each sequence's own the last of them."""
-        if key.shape[2] != max(self._new):
+        if key.shape[2] > max(self._new):
             raise ValueError(f"append takes the {max(self._new)} tokens that advance made room for, not {key.shape[2]}.")
+        self._used = True
         paged_append(key, value, self.key_pages[layer], self.value_pages[layer], self.block_table, self.lengths,
-                     self._counts() if min(self._new) != max(self._new) else None)
+                     self._counts() if min(self._new) < key.shape[2] else None)
 
     def attention(self, layer: int, query: torch.Tensor, *, scale: Optional[float] = None, window: int = 0,
                   sinks: int = 0) -> torch.Tensor:
@@ -254,6 +259,7 @@ class PagedKVCache:
         head_dim].  After an ``advance`` by different numbers the queries of a
         sequence are its new tokens' only, the last of the T; the outputs
         before them are zeros."""
+        self._used = True
         weights, table = None, self.block_table
         if self.token_weights is not None:
             weights = self.token_weights[layer]
@@ -300,6 +306,6 @@ class PagedKVCache:
         for pages in self._pages:
             self._free.extend(reversed(pages))
         self._pages, self._lengths = fresh, left
-        self._new, self._ragged = [0] * self.batch, False
+        self._new, self._ragged, self._used = [0] * self.batch, False, True
         self._upload(True)
         return True

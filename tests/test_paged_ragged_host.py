@@ -27,14 +27,20 @@ def test_counts_follow_the_advances(calls):
     assert step(7) == [None, None]
     c.advance([1, 5, 0])
     assert step(5) == [[1, 5, 0], [1, 5, 0]]
-    for T in (1, 4, 6):                       # rows that advance made no room for, or left without
-        with pytest.raises(ValueError):
-            c.append(0, torch.zeros(3, 1, T, 64), torch.zeros(3, 1, T, 64))
+    with pytest.raises(ValueError):           # rows that advance made no room for
+        c.append(0, torch.zeros(3, 1, 6, 64), torch.zeros(3, 1, 6, 64))
+    assert step(1) == [[1, 5, 0], [1, 5, 0]]
     c.advance([2, 2, 2])
     assert step(2) == [None, None]
     c.advance(4)
     c.crop([n - x for n, x in zip(c.seq_lengths(), (4, 1, 3))])
     assert step(3) == [[0, 3, 1], None]       # what is left of the four; the queries stay the newest of every sequence
+    c.advance(2)
+    c.advance([3, 3, 0])                      # two advances, one append
+    assert step(5) == [[5, 5, 2], [5, 5, 2]]
+    c.advance(1)
+    c.advance(3)
+    assert step(4) == [None, None] and step(2) == [None, None]
     c.crop(0)
     with pytest.raises(ValueError):
         c.append(0, torch.zeros(3, 1, 1, 64), torch.zeros(3, 1, 1, 64))
