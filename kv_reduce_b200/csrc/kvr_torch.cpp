@@ -82,11 +82,14 @@ struct PlanKey {
 };
 std::map<PlanKey, std::array<int64_t, 3>> g_plans;
 
-void attach_scratch(kvr_decode_args& a, const at::Device& dev, cudaStream_t stream) {
+// Held until the call's launch is in the stream: another thread's call on it
+// may replace the buffers with larger ones.
+[[nodiscard]] std::unique_lock<std::mutex> attach_scratch(kvr_decode_args& a, const at::Device& dev,
+                                                          cudaStream_t stream) {
   PlanKey key{{a.batch, a.q_heads, a.kv_heads, a.head_dim, a.seq_len, a.prefix_len, a.group_size, a.key_bits,
                a.value_bits, a.split_tokens, a.n_layers, dev.index()}};
   std::array<int64_t, 3> plan;
-  std::lock_guard<std::mutex> lock(g_mu);
+  std::unique_lock<std::mutex> lock(g_mu);
   auto it = g_plans.find(key);
   if (it == g_plans.end()) {
     int ns = 0;
@@ -105,6 +108,7 @@ void attach_scratch(kvr_decode_args& a, const at::Device& dev, cudaStream_t stre
   a.workspace = s.workspace.data_ptr();
   a.workspace_bytes = (size_t)s.workspace.numel();
   a.counters = s.counters.data_ptr<int>();
+  return lock;
 }
 
 constexpr int64_t kLayoutKeysOk = 1, kLayoutValuesOk = 2;
@@ -221,7 +225,7 @@ at::Tensor decode_attention(const at::Tensor& query, const at::Tensor& key_paylo
   // a positive split is rounded up to block_tokens (then to 32 by the library)
   a.split_tokens = split > 0 ? (int)((split + block - 1) / block * block) : 0;
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-  attach_scratch(a, dev, stream);
+  const auto scratch = attach_scratch(a, dev, stream);
   raise_status("kvr_decode_attention", kvr_decode_attention(&a, stream));
   return out;
 }
@@ -315,7 +319,7 @@ at::Tensor& decode_step_out(const at::Tensor& query, const at::Tensor& k_new, co
   a.value_meta_bh_stride = value_scale.stride(1);
   a.split_tokens = (int)split;
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-  attach_scratch(a, dev, stream);
+  const auto scratch = attach_scratch(a, dev, stream);
   raise_status("kvr_decode_step",
                kvr_decode_step(&a, static_cast<const uint16_t*>(k.data_ptr()),
                                static_cast<const uint16_t*>(v.data_ptr()), lengths.data_ptr<int>(), (int)cap_res,

@@ -59,3 +59,34 @@ def test_threads_on_one_stream(kvr):
     assert wrong == [0] * len(calls)
     for call, w in zip(calls, want):               # and nothing is left behind
         assert all(torch.equal(a, b) for a, b in zip(call(), w))
+
+
+def test_decode_threads_whose_scratch_grows(kvr):
+    """Packed decodes of rising sizes beside small ones, on one stream: a call's
+    buffers are its own until it is launched, though another outgrows them."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    calls = []
+    for B, S in ((1, 600), (2, 3000), (8, 3000), (16, 6000), (24, 9000)):
+        k, v = (torch.randn(B, 2, S, 128, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+        q = torch.randn(B, 12, 1, 128, device="cuda", generator=g).to(torch.bfloat16)
+        pk, pv = kvr.pack_kivi_kv(k, v, k_bits=4, v_bits=4, group_size=32, residual_length=128)
+        calls.append(lambda q=q, pk=pk, pv=pv: kvr.packed_kv_decode_attention(q, pk, pv))
+    s = torch.cuda.Stream()                        # (a stream of its own: nothing has grown its scratch yet)
+    s.wait_stream(torch.cuda.current_stream())
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(3)
+
+    def loop(order):
+        start.wait()
+        with torch.cuda.stream(s):
+            got = [(i, calls[i]()) for i in order]
+            wrong.append(int(torch.stack([(x != want[i]).sum() for i, x in got]).sum()))
+
+    threads = [threading.Thread(target=loop, args=(o,)) for o in ([0] * 200, [0, 1] * 100,
+                                                                 [0] * 40 + [1] * 40 + [2] * 40 + [3] * 40 + [4] * 40)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [0] * 3
