@@ -154,7 +154,8 @@ constexpr float kUnseen = -FLT_MAX;
 // x factor - m of two rows, the product rounded first.  Fused, it would keep the
 // digits that are rounded off in m and in tiles that a mask cuts: half the
 // spacing of numbers like m, which from 2^27 on is more than the exponents'
-// range.
+// range.  (m is taken off by a multiplication with -1 and an addition: a packed
+// mul.rn and add.rn do come out fused.)
 __device__ __forceinline__ void two_exponents(float& x0, float& x1, float factor, float2 m) {
   asm("{\n.reg .b64 x, f, m, one;\nmov.b64 x, {%0, %1};\nmov.b64 f, {%2, %2};\nmov.b64 m, {%3, %4};\n"
       "mov.b64 one, {%5, %5};\nmul.rn.f32x2 x, x, f;\nfma.rn.f32x2 x, m, one, x;\nmov.b64 {%0, %1}, x;\n}\n"

@@ -47,11 +47,11 @@ def check_few(kvr, data, few):  # noqa: F811
     assert (lse[few].double() - want_lse).abs().max().item() <= 2 ** -14
 
 
-def far_scores(lengths, HQ, H, D, T, dtype, size, seed):
+def far_scores(lengths, HQ, H, D, T, dtype, size, seed, page=16, width=None):
     """Scores of about `size` (either sign), products of two numbers that the
     type holds, so exact: a few equal ones on top and the others a step or
     more below."""
-    q, k, v, table, n = make(lengths, HQ, H, D, T, 16, dtype, seed=seed, garbage=False)
+    q, k, v, table, n = make(lengths, HQ, H, D, T, page, dtype, seed=seed, garbage=False, max_pages=width)
     root = 2.0 ** round(math.log2(abs(size)) / 2)
     q.zero_()
     k.zero_()
@@ -80,6 +80,23 @@ def test_scores_far_from_zero(kvr, HQ, H, D, T, window, dtype, size):  # noqa: F
     empty = want_lse == -math.inf
     assert torch.equal(lse == -math.inf, empty)
     assert ((lse.double() - want_lse).abs() <= 2.0 ** -22 * want_lse.abs() + 2 ** -14)[~empty].all()
+
+
+@pytest.mark.parametrize("dtype,size", [("bf16", 2.0 ** 20), ("bf16", -2.0 ** 30), ("bf16", 2.0 ** 118), ("fp16", 2.0 ** 28)])
+@pytest.mark.parametrize("page", [16, 2])
+@pytest.mark.parametrize("HQ,H,D,T", [(12, 2, 128, 5), (16, 2, 128, 9), (16, 2, 64, 9)])
+def test_scores_far_from_zero_in_wide_tables(kvr, HQ, H, D, T, page, dtype, size):  # noqa: F811
+    """The same in tiles of 32 and 64 rows, and with rows copied one by one."""
+    q, k, v, table, n = far_scores([1500, 130, 1, 4000], HQ, H, D, T, dtype, size, HQ, page, 160000 // page)
+    w = torch.zeros(4, table.shape[1] * page, device="cuda")
+    out, lse = kvr.paged_decode_attention(q, k, v, table, n, scale=1.0, return_lse=True, token_weights=w)
+    want, _, want_lse, want_w = reference(q, k, v, table, n, scale=1.0)
+    size_v = reference(q, k, v.abs(), table, n, scale=1.0)[1]
+    u = 2.0 ** -9 if dtype == "bf16" else 2.0 ** -12
+    assert ((out.double() - want).abs() <= (2 * u + 2 ** -12) * size_v + 1e-7).all()
+    empty = want_lse == -math.inf
+    assert ((lse.double() - want_lse).abs() <= 2.0 ** -22 * want_lse.abs() + 2 ** -14)[~empty].all()
+    assert ((w.double() - want_w).abs() <= 2 ** -14 * want_w + 1e-6).all()
 
 
 @pytest.mark.parametrize("dtype,size", [("bf16", x) for x in (2.0 ** 12, 2.0 ** 20, -2.0 ** 30, 2.0 ** 118, -2.0 ** 118)] +
