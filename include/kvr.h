@@ -440,7 +440,8 @@ int kvr_paged_append(const kvr_paged_append_args* a, kvr_stream_t stream);
  *   every cached token got, summed over heads and queries, is added to it
  *   (a second launch; needs `scores`.  Scores are held for a part of the
  *   batch at a time, 2 GiB or one sequence's; a batch of more takes a pair
- *   of launches per part).
+ *   of launches per part, each cut over the GPU by itself, so that the last
+ *   bits of its rows may differ from those of a call without weights).
  * Supported: D in {64, 128}, table_width*page_size <= 2^30.
  * kvr_paged_attention_plan gives the bytes of workspace, the ints of
  * counters (zero before the first launch, left zero by every completed one)
